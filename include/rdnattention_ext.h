@@ -200,6 +200,92 @@ RDNA_API int32_t rdna_attention_call_plan(
 RDNA_API int32_t rdna_kernel_timer_enable(int32_t on);
 RDNA_API int32_t rdna_kernel_timer_read(double* total_ms, int64_t* launches);
 
+/* ---------------------------------------------------------------------------
+ * Paged key/value caches.  The reference has none.
+ *
+ * Keys and values live in pages of page_size tokens (a power of two): element
+ * (page, token, head, channel) of the keys at key + page * key_stride[0] + token *
+ * key_stride[1] + head * key_stride[2] + channel, strides in elements, multiples of
+ * 16 bytes; the values likewise.  Key j of sequence b is token j % page_size of page
+ * block_tables[b * table_stride + j / page_size].  int8 pages have a float scale per
+ * (page, token, head), strides in floats: the value is int8 * scale.
+ *
+ * seq_lens, block_tables and cu_seqlens are device memory that the host does not
+ * read.  The newest rows of sequence b are the rows cu_seqlens[b] .. cu_seqlens[b +
+ * 1] - 1 of a call's row tensors [num_rows, heads, head_dim] (cu_seqlens null:
+ * num_rows / num_seqs each), n of them its keys seq_lens[b] - n .. seq_lens[b] - 1.
+ * Rows behind the last sequence belong to none.  A length beyond the page table is
+ * taken as the table's, a negative one as 0; the entry of a page that does not exist
+ * never leads outside the pages (nothing is written for it, and what a call that
+ * reads through it returns for that sequence is unspecified).
+ * ------------------------------------------------------------------------- */
+#define RDNA_DTYPE_F16 0
+#define RDNA_DTYPE_BF16 1
+#define RDNA_DTYPE_INT8 2
+
+typedef struct rdna_paged_cache {
+    void* key;
+    void* value;
+    float* key_scale;   /* int8 pages only, else null */
+    float* value_scale;
+    const int32_t* block_tables; /* [num_seqs, table_width] */
+    const int32_t* seq_lens;     /* [num_seqs], the newest rows among them */
+    const int32_t* cu_seqlens;   /* [num_seqs + 1], or null */
+    int64_t key_stride[3];       /* page, token, head */
+    int64_t value_stride[3];
+    int64_t key_scale_stride[3];
+    int64_t value_scale_stride[3];
+    int64_t table_stride;
+    uint32_t num_pages, page_size, table_width, num_seqs, num_kv_heads, head_dim;
+    int32_t dtype; /* RDNA_DTYPE_*; int8 at head_dim 64 and 128 */
+} rdna_paged_cache;
+
+/* Writes the newest rows' keys and values [num_rows, num_kv_heads, head_dim] (dtype:
+ * fp16 or bf16; strides of rows and heads in elements) to their places in the pages;
+ * int8 pages get the row quantised with its own scale (largest magnitude / 127, as
+ * rdna_quantize_int8 does per token).  With rot_cos / rot_sin (float [rot_rows,
+ * rot_dim / 2], 16-byte aligned) the first rot_dim channels of every key are rotated
+ * first, by the angles of its index in the sequence or of positions[row]: channels
+ * (2i, 2i + 1) by column i (rot_interleaved) or (i, i + rot_dim / 2); positions
+ * outside the tables are taken as their first or last row.  With query, the query
+ * rows [num_rows, num_heads, head_dim] are rotated likewise into query_out (which may
+ * be query).  Rows without a place write nothing; their query rows come out as they
+ * are (rotated if positions are given, and the row is a sequence's).  rot_dim is a
+ * multiple of 16. */
+RDNA_API int32_t rdna_paged_append(
+    const rdna_paged_cache* cache, const void* key, const void* value, int64_t key_stride_row, int64_t key_stride_h,
+    int64_t value_stride_row, int64_t value_stride_h, uint32_t num_rows, int32_t dtype, const void* query,
+    void* query_out, int64_t query_stride_row, int64_t query_stride_h, int64_t query_out_stride_row,
+    int64_t query_out_stride_h, uint32_t num_heads, const int32_t* positions, const void* rot_cos,
+    const void* rot_sin, uint32_t rot_rows, uint32_t rot_dim, int32_t rot_interleaved, void* hip_stream);
+
+/* softmax(scale Q K^T) V of the newest rows over the pages, head_dim a multiple of 32
+ * up to 256, query and output fp16 or bf16 (dtype; the pages' own type, or any with
+ * int8 pages).  causal and window_size as in rdna_attention_forward.  A row that sees
+ * no key is zeros.  max_rows_per_seq: most rows of a sequence as far as the caller
+ * knows (num_rows if not); it picks kernels and decides no result.
+ *
+ * With tree_mask ([num_seqs, tree_n, tree_n] bytes, 0 or 1, strides of sequences and
+ * rows in bytes) the newest rows are drafts: row i sees every key before the drafts
+ * and draft j where tree_mask[b][i][j]; causal and window_size must be off.
+ *
+ * The rows of output behind the last sequence are left as they are, or set to zeros
+ * (zero_tail).  The scratch is stream-ordered like the split-K partials'. */
+RDNA_API int32_t rdna_paged_attention(
+    const rdna_paged_cache* cache, const void* query, void* output, int64_t query_stride_row, int64_t query_stride_h,
+    int64_t output_stride_row, int64_t output_stride_h, uint32_t num_rows, uint32_t num_heads, int32_t dtype,
+    uint32_t max_rows_per_seq, float scale, int32_t causal, int32_t window_size, const uint8_t* tree_mask,
+    int64_t tree_stride_seq, int64_t tree_stride_row, uint32_t tree_n, int32_t zero_tail, void* hip_stream);
+
+/* Keeps accepted drafts: for every sequence, key and value prefix_lens[b] + i become
+ * those of prefix_lens[b] + path[b * path_stride + i], i < path_lens[b] (at most
+ * path_n <= 1024), all of them read before the first is written; entries below 0
+ * and keys beyond the table move nothing.  cache->seq_lens and cu_seqlens are not
+ * looked at.  At most 65535 sequences. */
+RDNA_API int32_t rdna_paged_commit(const rdna_paged_cache* cache, const int32_t* prefix_lens, const int32_t* path,
+                                   int64_t path_stride, uint32_t path_n, const int32_t* path_lens,
+                                   void* hip_stream);
+
 /* Library version string ("0.1.0-gfx950"). */
 RDNA_API const char* rdna_version(void);
 

@@ -678,6 +678,10 @@ def flash_attn_int8qk_quantized(query, key, value, is_causal: bool = False, wind
     return output
 
 
+# paged caches (an extension): in a module of their own, offered here
+from rdnattention.paged import (SUPPORTED_HEAD_DIMS_PAGED, paged_append, paged_attention, paged_commit,  # noqa: E402
+                                paged_tree_attention)
+
 __all__ = ["flash_attn", "flash_attn_int8qk", "flash_attn_int8qk_quantized", "quantize_int8_perchannel_v",
            "quantize_int8_qk_pertoken", "has_device", "RDNAttentionError", "SUPPORTED_HEAD_DIMS",
            "SUPPORTED_HEAD_DIMS_INT8", "__version__"]

@@ -15,6 +15,7 @@
 #include "rdnattention_ext.h"
 #include "fa_host.hpp"
 #include "fa_internal.hpp"
+#include "paged_host.hpp"
 
 #include <hip/hip_runtime.h>
 
@@ -213,6 +214,10 @@ int32_t forward_i8_impl(const void* q, const void* k, const void* v, void* outpu
 }
 
 } // namespace
+
+void rdna_amd::set_api_error(const char* fmt, const std::string& detail) {
+    set_error(fmt, detail);
+}
 
 RDNA_API int32_t rdna_has_device(void) {
     return rdna::hasDevice() ? 1 : 0;

@@ -31,7 +31,7 @@ constexpr size_t region_bytes(size_t bytes) {
 
 // What a scratch buffer holds; calls keep one cached buffer per (device,
 // stream, purpose), so buffers of one call never alias.
-enum class ScratchUse : int { RotatedK = 0, SplitKPartials = 1, QuantPartials = 2, Int8Scores = 3 };
+enum class ScratchUse : int { RotatedK = 0, SplitKPartials = 1, QuantPartials = 2, Int8Scores = 3, PagedPartials = 4 };
 
 // Scratch memory for one call (scratch.cpp).  Without a region: the buffer
 // cached for (device, stream, use); a call that finds it large enough makes

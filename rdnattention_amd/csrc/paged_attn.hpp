@@ -1,0 +1,279 @@
+// Shared by the two paged attention kernels (device code): element types, the
+// walk over a workgroup's share of the work, row pointers into the pages, and
+// what a shared item leaves for the merge.
+#pragma once
+
+#include "fa_common.hpp"
+#include "fa_splitk.hpp"
+#include "paged_host.hpp"
+
+namespace rdna_amd {
+
+template <class T>
+struct PagedVec {
+    typedef T v8 __attribute__((ext_vector_type(8)));
+    typedef T v4 __attribute__((ext_vector_type(4)));
+};
+
+template <class T>
+__device__ __forceinline__ f16x paged_mfma(typename PagedVec<T>::v8 a, typename PagedVec<T>::v8 b, f16x c) {
+    if constexpr (sizeof(T) == 2 && __is_same(T, _Float16)) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+    } else {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+    }
+}
+
+// What a share of the work leaves where an item has several: slot w holds the
+// part of workgroup w's first item that began before w, slot n_wg + w the part of
+// its last item that goes on behind it (rows of ROWS: O unnormalised in fp32,
+// then (m, l) with m in log2 units).  The record of workgroup w names the item
+// that starts in it and goes on, for the merge.
+struct PagedRecord {
+    int32_t rows;   // 0: none
+    int32_t q0;     // first token of the sequence
+    int32_t r0;     // first row of the item
+    int32_t h;      // kv head
+    int32_t w_last; // the last workgroup of the item
+    int32_t unused[3];
+};
+
+struct PagedAttnParams {
+    PagedPages c;
+    PagedWork work;
+    const char* q;
+    char* o;
+    int64_t q_st, q_sh, o_st, o_sh; // bytes
+    float scale_log2e;              // |scale| log2(e)
+    float q_sign;
+    int32_t zero_tail;
+    int32_t Hq;
+    const uint8_t* tree; // null: no tree
+    int64_t tree_sb, tree_sr;
+    int32_t tree_n;
+    float* part_o;
+    float* part_ml;
+    PagedRecord* records;
+};
+
+// 16-byte chunk swizzle of row r of a tile of unpadded rows (see dec_swz of the
+// split-K kernel: rows that start in the same bank differ in it, so 16-row
+// ds_read_b128 and 4-row transpose reads hit distinct banks).
+template <int D>
+__device__ __forceinline__ int paged_swz(int r) {
+    if constexpr (D % 64 == 32) {
+        return (r >> 2) & 3;
+    } else if constexpr (D % 128 == 64) {
+        return (((r >> 1) & 3) << 1) | ((r >> 3) & 1);
+    } else {
+        return ((r & 7) << 1) | ((r >> 3) & 1);
+    }
+}
+
+// A row of zeros: stands for keys that no row of the item sees, so that what the
+// pages hold there (a key behind the sequence's last may be anything) never
+// meets a weight of zero as infinity or NaN.
+__device__ __attribute__((aligned(16))) const uint32_t kPagedZeroRow[256 / 2] = {};
+
+// HBM -> LDS copies with a 64-bit address per lane (see dma_load16)
+__device__ __forceinline__ void dma_gather16(uint64_t addr, uint32_t lds_byte_addr) {
+    asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off"
+                 :
+                 : "v"(addr), "s"(lds_byte_addr)
+                 : "memory", "m0");
+}
+__device__ __forceinline__ void dma_gather16_nt(uint64_t addr, uint32_t lds_byte_addr) {
+    asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off nt"
+                 :
+                 : "v"(addr), "s"(lds_byte_addr)
+                 : "memory", "m0");
+}
+
+__device__ __forceinline__ int32_t uniform(int32_t x) {
+    return __builtin_amdgcn_readfirstlane(x);
+}
+
+// A workgroup's walk over its units, the same in every wave.
+template <int ROWS, int BN>
+struct PagedWalk {
+    const PagedWork& w;
+    int32_t wg;
+    int32_t left = 0;  // units of the share not yet taken
+    int32_t at = 0;    // unit of the item to begin with
+    int32_t start = 0; // call-wide number of that unit
+    int32_t share = 1;
+    int32_t b = 0, h = 0, rt = 0, n_rt = 0;
+    PagedSeq seq;
+    PagedTile tile;
+
+    __device__ __forceinline__ explicit PagedWalk(const PagedWork& work) : w(work) {
+        // Workgroup id runs on XCD id % 8: neighbouring shares, which have heads (and
+        // with many row tiles also keys) in common, on one XCD.
+        const int32_t id = blockIdx.x;
+        wg = (w.n_wg & 7) == 0 ? (id & 7) * (w.n_wg >> 3) + (id >> 3) : id;
+        const int lane = threadIdx.x & 63;
+        const int32_t B = w.seqs.B;
+        int32_t total = 0, mine = 0;
+        for (int32_t i = 0; i < B; i += 64) {
+            mine = 0;
+            if (i + lane < B) {
+                mine = paged_head_units<ROWS, BN>(w, paged_seq(w.seqs, i + lane)) * w.Hkv;
+            }
+            total += wave_sum(mine);
+        }
+        total = uniform(total);
+        share = paged_share(w, total);
+        start = (int32_t)((int64_t)wg * share < total ? wg * share : total);
+        left = mask_imin(share, total - start);
+        if (left <= 0) {
+            left = 0;
+            return;
+        }
+        // the sequence that unit `start` is in
+        int32_t before = 0;
+        for (int32_t i = 0; i < B; i += 64) {
+            if (B > 64) {
+                mine = 0;
+                if (i + lane < B) {
+                    mine = paged_head_units<ROWS, BN>(w, paged_seq(w.seqs, i + lane)) * w.Hkv;
+                }
+            }
+            int32_t sum = mine;
+#pragma unroll
+            for (int d = 1; d < 64; d <<= 1) {
+                const int32_t x = __shfl_up(sum, d);
+                sum += lane >= d ? x : 0;
+            }
+            const uint64_t past = __builtin_amdgcn_ballot_w64(before + sum > start);
+            if (past != 0) {
+                const int l = __builtin_ctzll(past);
+                b = i + l;
+                before += __shfl(sum, l) - __shfl(mine, l);
+                break;
+            }
+            before += __shfl(sum, 63);
+        }
+        b = uniform(b);
+        at = start - uniform(before);
+        load_seq();
+        const int32_t per_head = uniform(paged_head_units<ROWS, BN>(w, seq));
+        if (per_head == 0) {
+            left = 0;
+            return;
+        }
+        h = mask_imin(at / per_head, w.Hkv - 1);
+        at -= h * per_head;
+        rt = 0;
+        load_tile();
+        while (at >= tile.units && rt + 1 < n_rt) {
+            at -= tile.units;
+            rt++;
+            load_tile();
+        }
+    }
+
+    static __device__ __forceinline__ int32_t wave_sum(int32_t x) {
+#pragma unroll
+        for (int d = 32; d > 0; d >>= 1) {
+            x += __shfl_xor(x, d);
+        }
+        return x;
+    }
+
+    __device__ __forceinline__ void load_seq() {
+        seq = paged_seq(w.seqs, b);
+        seq.q0 = uniform(seq.q0);
+        seq.n = uniform(seq.n);
+        seq.len = uniform(seq.len);
+        n_rt = paged_row_tiles<ROWS>(w, seq.n);
+    }
+    __device__ __forceinline__ void load_tile() {
+        tile = paged_tile<ROWS, BN>(w, seq, rt);
+    }
+
+    // Every loop here ends by itself, whatever the lengths hold (a caller may, by
+    // mistake, be changing them).
+    // The part of the current item that this share has: units [at, at + count()).
+    __device__ __forceinline__ bool more() const {
+        return left > 0;
+    }
+    __device__ __forceinline__ int32_t count() const {
+        return mask_imin(left, tile.units - at);
+    }
+    __device__ __forceinline__ bool whole() const {
+        return at == 0 && left >= tile.units;
+    }
+    // Slot of a part that is not the whole item, and, of the first part, the last
+    // workgroup.
+    __device__ __forceinline__ int32_t slot() const {
+        return at == 0 ? w.n_wg + wg : wg;
+    }
+    __device__ __forceinline__ int32_t last_wg() const {
+        return (start + tile.units - 1) / share;
+    }
+    __device__ __forceinline__ void next() {
+        const int32_t n = count();
+        left -= n;
+        start += n;
+        at = 0;
+        if (left > 0) {
+            if (++rt == n_rt) {
+                rt = 0;
+                if (++h == w.Hkv) {
+                    h = 0;
+                    do {
+                        if (++b >= w.seqs.B) {
+                            left = 0;
+                            return;
+                        }
+                        load_seq();
+                    } while (n_rt == 0);
+                }
+            }
+            load_tile();
+        }
+    }
+};
+
+// Masks the scores s[0 .. 16 N - 1] of keys key0 + 32 (e / 16) + 8 (e % 16 / 4) + e
+// % 4 that row `row` of the mask (n columns, drafts from `prefix` on) does not see.
+// Every byte is loaded, at a column inside the row, and then selected on: eight
+// loads are in flight together.  (With the load behind the comparison this compiler, clang
+// of ROCm 7.2, keeps score and result in one register and stores -inf over the
+// scores that are seen.)
+template <int N>
+__device__ __forceinline__ void tree_mask_scores(f16x (&s)[N], const uint8_t* row, int32_t n, int32_t prefix,
+                                                 int32_t key0) {
+#pragma unroll
+    for (int t = 0; t < 2 * N; t++) { // eight at a time: their registers
+        uint32_t bit[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const int32_t j = key0 + 16 * t + 8 * (e >> 2) + (e & 3) - prefix;
+            bit[e] = row[max(min(j, n - 1), 0)];
+        }
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const int32_t j = key0 + 16 * t + 8 * (e >> 2) + (e & 3) - prefix;
+            const bool hidden = (j >= n) | ((j >= 0) & (bit[e] == 0));
+            const int i = 8 * (t & 1) + e;
+            s[t >> 1][i] = hidden ? -INFINITY : s[t >> 1][i];
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    }
+}
+
+// Zeros for the rows behind the last sequence, dealt to the workgroups.
+template <int D>
+__device__ __forceinline__ void zero_tail_rows(const PagedAttnParams& p) {
+    constexpr int CH = D / 8;
+    const int32_t per_row = p.Hq * CH;
+    for (int32_t t = paged_rows_end(p.work.seqs) + blockIdx.x; t < p.work.seqs.total; t += gridDim.x) {
+        for (int32_t i = threadIdx.x; i < per_row; i += blockDim.x) {
+            const int32_t h = i / CH;
+            *reinterpret_cast<i4*>(p.o + t * p.o_st + h * p.o_sh + 16 * (i - h * CH)) = i4{0, 0, 0, 0};
+        }
+    }
+}
+
+} // namespace rdna_amd

@@ -1,0 +1,149 @@
+// Where the rows and keys of a paged call are: plain integer code, device
+// functions when compiled as HIP, ordinary inline functions otherwise (host
+// tests check them, tests/cxx/paged_rows_check.cpp).
+//
+// A call has B sequences.  Sequence b has `len` keys in its pages, the last n
+// of them its newest rows: row i is key len - n + i.  The lengths, row ranges
+// and page tables are device memory that the host does not see, so every value
+// is bounded here and no access leaves a buffer, whatever they hold.
+//
+// The attention kernels deal a call's key tiles to their workgroups in equal
+// shares: the rows (n tokens of G query heads each) of every (sequence, kv
+// head) fall into row tiles of ROWS rows, a row tile is an item of as many
+// units as it sees key tiles of BN keys (one if none, for its zeros), and
+// workgroup w takes the units [w * per, (w + 1) * per) of the items in order
+// (sequence, kv head, row tile).  At most two of a workgroup's items are shared
+// with others: the first and the last.
+#pragma once
+
+#include "fa_mask.hpp"
+
+#include <cstdint>
+
+namespace rdna_amd {
+
+struct PagedSeqs {
+    const int32_t* lens; // [B] keys in the cache
+    const int32_t* cu;   // [B + 1] first row of each sequence, or null: `rows` each
+    int32_t B;
+    int32_t rows;
+    int32_t total;    // rows of the query tensor
+    int32_t max_keys; // keys that a row of the page table covers
+};
+
+struct PagedSeq {
+    int32_t q0;  // first row in the query tensor
+    int32_t n;   // rows
+    int32_t len; // keys
+};
+
+RDNA_MASK_FN int32_t rows_clamp(int32_t x, int32_t lo, int32_t hi) {
+    return mask_imin(mask_imax(x, lo), hi);
+}
+
+// Rows that belong to a sequence: [0, paged_rows_end).
+RDNA_MASK_FN int32_t paged_rows_end(const PagedSeqs& s) {
+    return s.cu != nullptr ? rows_clamp(s.cu[s.B], 0, s.total) : s.total;
+}
+
+RDNA_MASK_FN PagedSeq paged_seq(const PagedSeqs& s, int32_t b) {
+    PagedSeq r;
+    r.len = rows_clamp(s.lens[b], 0, s.max_keys);
+    if (s.cu != nullptr) {
+        r.q0 = rows_clamp(s.cu[b], 0, s.total);
+        r.n = rows_clamp(s.cu[b + 1], r.q0, s.total) - r.q0;
+    } else {
+        r.q0 = b * s.rows;
+        r.n = s.rows;
+    }
+    return r;
+}
+
+// The sequence that row t belongs to, -1 for a row behind the last one.
+RDNA_MASK_FN int32_t paged_seq_of_row(const PagedSeqs& s, int32_t t) {
+    if (s.cu == nullptr) {
+        return t / s.rows;
+    }
+    int32_t lo = 0, hi = s.B; // the first b with cu[b + 1] > t
+    while (lo < hi) {
+        const int32_t mid = (lo + hi) >> 1;
+        if (s.cu[mid + 1] > t) {
+            hi = mid;
+        } else {
+            lo = mid + 1;
+        }
+    }
+    return lo < s.B && s.cu[lo] <= t ? lo : -1;
+}
+
+// Visibility of a sequence's keys (see MaskSpec); a tree's prefix and drafts
+// are one range here, its mask comes on top.
+struct PagedMask {
+    int32_t causal;
+    int32_t window;
+};
+
+RDNA_MASK_FN MaskSpec paged_mask(const PagedMask& m, const PagedSeq& s) {
+    return MaskSpec{s.len, s.len - s.n, m.causal, m.window};
+}
+
+// Work of a call: sequences with more than min_rows and at most max_rows rows
+// (tokens times G) are dealt to n_wg workgroups.
+struct PagedWork {
+    PagedSeqs seqs;
+    PagedMask mask;
+    int32_t Hkv, G;
+    int32_t min_rows, max_rows;
+    int32_t n_wg;
+    int32_t min_units; // smallest share
+};
+
+// Row tiles of a sequence, 0 where another launch works on it.
+template <int ROWS>
+RDNA_MASK_FN int32_t paged_row_tiles(const PagedWork& w, int32_t n) {
+    const int32_t rows = n * w.G;
+    return rows > w.min_rows && rows <= w.max_rows ? (rows + ROWS - 1) / ROWS : 0;
+}
+
+// Key tiles of row tile rt: `units` from tile `first` on; nothing visible: units
+// 1 and lo > hi.
+struct PagedTile {
+    int32_t lo, hi; // keys that some row sees
+    int32_t first, units;
+};
+
+template <int ROWS, int BN>
+RDNA_MASK_FN PagedTile paged_tile(const PagedWork& w, const PagedSeq& s, int32_t rt) {
+    const int32_t i_lo = rt * ROWS / w.G;
+    const int32_t i_hi = (mask_imin((rt + 1) * ROWS, s.n * w.G) - 1) / w.G;
+    PagedTile t;
+    visible_key_range(paged_mask(w.mask, s), i_lo, i_hi, t.lo, t.hi);
+    if (t.hi < t.lo) {
+        t.lo = 0;
+        t.hi = -1;
+        t.first = 0;
+        t.units = 1;
+    } else {
+        t.first = t.lo / BN;
+        t.units = t.hi / BN + 1 - t.first;
+    }
+    return t;
+}
+
+// Units of one kv head of a sequence.
+template <int ROWS, int BN>
+RDNA_MASK_FN int32_t paged_head_units(const PagedWork& w, const PagedSeq& s) {
+    const int32_t n = paged_row_tiles<ROWS>(w, s.n);
+    int32_t u = 0;
+    for (int32_t rt = 0; rt < n; rt++) {
+        u += paged_tile<ROWS, BN>(w, s, rt).units;
+    }
+    return u;
+}
+
+// Share of each workgroup of `total` units.
+RDNA_MASK_FN int32_t paged_share(const PagedWork& w, int32_t total) {
+    return mask_imax((total + w.n_wg - 1) / w.n_wg, w.min_units);
+}
+
+} // namespace rdna_amd
