@@ -89,6 +89,91 @@ __device__ __forceinline__ void dma_gather16_nt(uint64_t addr, uint32_t lds_byte
                  : "memory", "m0");
 }
 
+__device__ __forceinline__ void dma_gather4(uint64_t addr, uint32_t lds_byte_addr) {
+    asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dword %0, off"
+                 :
+                 : "v"(addr), "s"(lds_byte_addr)
+                 : "memory", "m0");
+}
+
+typedef int i2v __attribute__((ext_vector_type(2)));
+
+// 8 signed bytes -> T, exactly.  fp16: a byte u = v + 128 below the exponent byte of
+// 1024 is 1024 + u, less 1152 it is v, five instructions per 4 values; bf16: through
+// fp32, whose upper half holds all 8 bits.
+template <class T>
+__device__ __forceinline__ typename PagedVec<T>::v8 widen_int8(i2v w) {
+    typename PagedVec<T>::v8 y;
+    if constexpr (__is_same(T, _Float16)) {
+        const h2 off = {(_Float16)1152.0f, (_Float16)1152.0f};
+#pragma unroll
+        for (int c = 0; c < 2; c++) {
+            const uint32_t u = (uint32_t)w[c] ^ 0x80808080u;
+            const h2 a = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)) - off;
+            const h2 b = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) - off;
+            y[4 * c] = a[0];
+            y[4 * c + 1] = a[1];
+            y[4 * c + 2] = b[0];
+            y[4 * c + 3] = b[1];
+        }
+    } else {
+        typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+        u4 r;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const uint32_t u = (uint32_t)w[i >> 1] ^ 0x80808080u;
+            const float a = (float)((u >> (16 * (i & 1))) & 0xffu) - 128.0f;
+            const float b = (float)((u >> (16 * (i & 1) + 8)) & 0xffu) - 128.0f;
+            r[i] = __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
+        }
+        y = __builtin_bit_cast(decltype(y), r);
+    }
+    return y;
+}
+
+// ds_read_b64_tr_b8: within each 16-lane group, lane i receives as byte k the byte i
+// % 8 of the 8-byte word whose address lane 2k + i / 8 supplies.
+__device__ __forceinline__ i2v read_tr8(const char* p) {
+    typedef __attribute__((address_space(3))) i2v lds_i2;
+    const auto* lp = reinterpret_cast<const __attribute__((address_space(3))) char*>(
+        (uint32_t)reinterpret_cast<uintptr_t>(p));
+    return __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i2*)lp);
+}
+
+// The values' scales of int8 pages, in the weights of P V: p v = (p s) (v / s), with
+// p s rounded to fp16 where p would be.  So that the products keep fp16's range
+// whatever the scales' size, they carry a power of two: relative to the largest
+// scale so far, at 2^7 (weights reach 2^8, products 2^15); O follows when it grows.
+// A value whose scale is less than 2^-21 of the largest one seen with it loses bits,
+// at most 2^-32 of the largest value per key.
+struct ValueScale {
+    int e = -1000; // the largest scale is below 2^e
+
+    // p[4 i + j] *= s[i][j], 2^(7 - e) times; s the scales of the lane's scores, the
+    // same in each half of the wave
+    template <int N, int NDT>
+    __device__ __forceinline__ void weigh(float (&p)[4 * N], const f4 (&s)[N], f16x (&o)[NDT]) {
+        float mx = max_tree<4 * N>([&](int i) { return fabsf(s[i >> 2][i & 3]); });
+        mx = pair_max(mx);
+        const int top = __builtin_amdgcn_readfirstlane(mx > 0.0f ? __builtin_amdgcn_frexp_expf(mx) : -1000);
+        if (top > e) {
+            const float f = ldexpf(1.0f, e - top);
+#pragma unroll
+            for (int i = 0; i < NDT; i++) {
+                o[i] *= f;
+            }
+            e = top;
+        }
+#pragma unroll
+        for (int i = 0; i < 4 * N; i++) {
+            p[i] *= ldexpf(s[i >> 2][i & 3], 7 - e);
+        }
+    }
+    __device__ __forceinline__ float factor() const {
+        return ldexpf(1.0f, e - 7);
+    }
+};
+
 __device__ __forceinline__ int32_t uniform(int32_t x) {
     return __builtin_amdgcn_readfirstlane(x);
 }

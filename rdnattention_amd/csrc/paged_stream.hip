@@ -16,9 +16,10 @@
 //   * the lengths are on the device: every workgroup derives its share of all
 //     key tiles from them (PagedWalk), equal for any mix of lengths, and the
 //     heads it shares with others are merged by a second launch
-//   * int8 pages go through registers: a tile is loaded one tile ahead,
-//     dequantised with its rows' scales to the queries' type and stored to the
-//     same LDS tile
+//   * int8 pages are copied as they are (half the bytes, two tiles deep) and
+//     widened exactly as they become MFMA operands; a key's scale multiplies its
+//     scores, a value's scale its weights, in fp32 (see ValueScale), so the pages
+//     cost no rounding beyond the 16-bit kernels'
 #include "paged_attn.hpp"
 
 #include "paged_launch.hpp"
@@ -32,25 +33,38 @@ constexpr float kRescale = 8.0f;
 
 template <int D, bool I8>
 struct StreamCfg {
-    // one K and one V tile per wave, 128 D bytes, and its addresses: eight waves up
-    // to D = 128, six to 192, four above (one wave per SIMD, whose O alone takes 128
-    // registers at 256)
-    static constexpr int WAVES = I8 && D == 128 ? 4 : D <= 128 ? 8 : (D <= 160 ? 6 : 4);
+    // K and V tiles of each wave, 128 D bytes (of int8: two of each, as much), and
+    // their addresses: eight waves up to D = 128, then four (one wave per SIMD, whose
+    // O alone takes 128 registers at 256)
+    static constexpr int WAVES = D <= 128 ? 8 : 4;
     static constexpr int THREADS = 64 * WAVES;
     static constexpr int WAVES_PER_SIMD = D <= 32 ? 4 : (D <= 64 && !I8 ? 3 : (WAVES > 4 ? 2 : 1));
-    static constexpr int RB = 2 * D;
-    static constexpr int KCH = D / 8;
+    static constexpr int SLOTS = I8 ? 2 : 1;
+    static constexpr int RB = I8 ? D : 2 * D; // row bytes
+    static constexpr int KCH = RB / 16;
     static constexpr int TILE_BYTES = kTile * RB;
-    // table entries (64 dwords), K and V row addresses (32 x 8 bytes each)
-    static constexpr int AUX_BYTES = I8 ? 0 : 256 + 2 * 256;
-    static constexpr int WAVE_BYTES = 2 * TILE_BYTES + AUX_BYTES;
+    // per slot 64 table entries (and of int8 32 key and 32 value scales); K and V
+    // row addresses (32 x 8 bytes each)
+    static constexpr int TAB_BYTES = 256 * SLOTS;
+    static constexpr int SCALE_BYTES = I8 ? 256 * SLOTS : 0;
+    static constexpr int WAVE_BYTES = 2 * SLOTS * TILE_BYTES + TAB_BYTES + SCALE_BYTES + 2 * 256;
     static constexpr int NS = D / 16;
     static constexpr int NDT = D / 32;
     static constexpr int DMA = TILE_BYTES / 1024;
-    static constexpr int NCH = I8 ? kTile * D / 1024 : 1; // 16-byte chunks of an int8 tile per lane
+    // copies of a K tile with its scales and a later tile's entries, and of a V tile
+    static constexpr int K_COPIES = DMA + (I8 ? 1 : 0) + 1;
+    static constexpr int V_COPIES = DMA;
     static_assert(WAVES * WAVE_BYTES <= 160 * 1024, "tiles fit the LDS");
     static_assert(finish_lds_bytes(D, WAVES) <= WAVES * WAVE_BYTES, "the merge reuses the tile area");
+    static_assert(SLOTS * (K_COPIES + V_COPIES) < 64, "vmcnt counts them");
 };
+
+// 16-byte chunk swizzle of row r of an int8 tile: rows of 64 or 128 bytes, the 64
+// banks 256, so rows r and r + 4 or r + 2 start in the same bank
+template <int D>
+__device__ __forceinline__ int swz8(int r) {
+    return D == 64 ? (r >> 2) & 3 : (r >> 1) & 7;
+}
 
 template <class T, int D, bool I8>
 __global__ __launch_bounds__((StreamCfg<D, I8>::THREADS), (StreamCfg<D, I8>::WAVES_PER_SIMD)) void paged_stream(
@@ -58,6 +72,10 @@ __global__ __launch_bounds__((StreamCfg<D, I8>::THREADS), (StreamCfg<D, I8>::WAV
     using C = StreamCfg<D, I8>;
     using V8 = typename PagedVec<T>::v8;
     using V4 = typename PagedVec<T>::v4;
+    // weights and values meet in P: int8 values are exact in fp16, whose weights
+    // round finer than bf16's
+    using P = std::conditional_t<I8, _Float16, T>;
+    using P8 = typename PagedVec<P>::v8;
     __shared__ __attribute__((aligned(16))) char dsm[C::WAVES * C::WAVE_BYTES];
 
     const int tid = threadIdx.x;
@@ -65,13 +83,12 @@ __global__ __launch_bounds__((StreamCfg<D, I8>::THREADS), (StreamCfg<D, I8>::WAV
     const int lane = tid & 63;
     const int l32 = lane & 31;
     const int g = lane >> 5;
-    char* const sk = dsm + wave * C::WAVE_BYTES;
-    char* const sv = sk + C::TILE_BYTES;
-    const uint32_t lds_k = (uint32_t)reinterpret_cast<uintptr_t>(sk);
-    const uint32_t lds_v = lds_k + C::TILE_BYTES;
-    const uint32_t lds_tab = lds_v + C::TILE_BYTES;
-    uint32_t* const tab = reinterpret_cast<uint32_t*>(sv + C::TILE_BYTES);
-    uint64_t* const krow_at = reinterpret_cast<uint64_t*>(tab + 64);
+    // slot i: K tile, V tile; then table entries, scales, row addresses
+    char* const wsm = dsm + wave * C::WAVE_BYTES;
+    char* const aux = wsm + 2 * C::SLOTS * C::TILE_BYTES;
+    const uint32_t lds_w = (uint32_t)reinterpret_cast<uintptr_t>(wsm);
+    const uint32_t lds_aux = lds_w + 2 * C::SLOTS * C::TILE_BYTES;
+    uint64_t* const krow_at = reinterpret_cast<uint64_t*>(aux + C::TAB_BYTES + C::SCALE_BYTES);
     uint64_t* const vrow_at = krow_at + kTile;
 
     if (p.zero_tail != 0) {
@@ -87,7 +104,7 @@ __global__ __launch_bounds__((StreamCfg<D, I8>::THREADS), (StreamCfg<D, I8>::WAV
     for (int j = 0; j < C::DMA; j++) {
         const int n = 64 * j + lane;
         const int r = n / C::KCH;
-        src[j] = (uint32_t)(r * 8) | (uint32_t)(((n - r * C::KCH) ^ paged_swz<D>(r)) * 16) << 16;
+        src[j] = (uint32_t)(r * 8) | (uint32_t)(((n - r * C::KCH) ^ (I8 ? swz8<D>(r) : paged_swz<D>(r))) * 16) << 16;
     }
     const uint32_t page_mask = (1u << p.c.lps) - 1u;
 
@@ -126,17 +143,22 @@ __global__ __launch_bounds__((StreamCfg<D, I8>::THREADS), (StreamCfg<D, I8>::WAV
         const char* const vbase = p.c.v + h * p.c.v_sh;
         const int32_t* const table = p.c.table + walk.b * p.c.table_s;
 
-        // ---- 16-bit pages: copies to LDS
         i32x4_t tab_rsrc = make_rsrc_v(table, (uint32_t)p.c.width * 4u);
 #pragma unroll
         for (int e = 0; e < 4; e++) {
             tab_rsrc[e] = uniform(tab_rsrc[e]);
         }
+        // slot of tile j
+        auto slot_of = [&](int j) { return C::SLOTS == 1 ? 0 : j & (C::SLOTS - 1); };
+        auto issue_tab = [&](int j) {
+            dma_load4(tab_rsrc, (uint32_t)((tile_key(j) + l32) >> p.c.lps) * 4u, lds_aux + 256 * slot_of(j));
+        };
         uint64_t v_next = 0; // address of V row l32 of the tile whose K was issued last
-        auto issue_tab = [&](int j) { dma_load4(tab_rsrc, (uint32_t)((tile_key(j) + l32) >> p.c.lps) * 4u, lds_tab); };
-        auto issue_k = [&](int j) { // its table entries have landed
+        // K tile j, its scales, and then (its own entries read) the entries of the
+        // tile that follows it in its slot
+        auto issue_k = [&](int j) {
             const int key = tile_key(j) + l32;
-            const uint32_t pg = tab[lane];
+            const uint32_t pg = reinterpret_cast<const uint32_t*>(aux)[64 * slot_of(j) + lane];
             const bool seen = key >= item.lo && key <= item.hi;
             const uint64_t pe = pg < (uint32_t)p.c.pages ? pg : 0u;
             const uint64_t off = (uint32_t)key & page_mask;
@@ -147,87 +169,49 @@ __global__ __launch_bounds__((StreamCfg<D, I8>::THREADS), (StreamCfg<D, I8>::WAV
             if (g == 0) {
                 krow_at[l32] = seen ? ka : zero;
             }
+            const uint32_t lds = lds_w + (uint32_t)slot_of(j) * (2 * C::TILE_BYTES);
 #pragma unroll
             for (int d = 0; d < C::DMA; d++) {
                 const uint64_t row = *reinterpret_cast<const uint64_t*>(reinterpret_cast<const char*>(krow_at) +
                                                                         (src[d] & 0xffffu));
-                dma_gather16_nt(row + (src[d] >> 16), lds_k + 1024 * d);
+                dma_gather16_nt(row + (src[d] >> 16), lds + 1024 * d);
             }
+            if constexpr (I8) { // lanes 0 - 31: the keys', 32 - 63: the values'
+                const uint64_t ks = reinterpret_cast<uint64_t>(p.c.ks) +
+                                    4 * (pe * (uint64_t)p.c.ks_sp + off * (uint64_t)p.c.ks_st + h * (uint64_t)p.c.ks_sh);
+                const uint64_t vs = reinterpret_cast<uint64_t>(p.c.vs) +
+                                    4 * (pe * (uint64_t)p.c.vs_sp + off * (uint64_t)p.c.vs_st + h * (uint64_t)p.c.vs_sh);
+                dma_gather4(seen ? (g == 0 ? ks : vs) : zero, lds_aux + C::TAB_BYTES + 256 * slot_of(j));
+            }
+            __builtin_amdgcn_s_waitcnt(waitcnt_lgkm(0)); // the entries are read
+            issue_tab(j + C::SLOTS);
         };
-        auto issue_v = [&]() {
+        auto issue_v = [&](int j) {
             if (g == 0) {
                 vrow_at[l32] = v_next;
             }
+            const uint32_t lds = lds_w + (uint32_t)slot_of(j) * (2 * C::TILE_BYTES) + C::TILE_BYTES;
 #pragma unroll
             for (int d = 0; d < C::DMA; d++) {
                 const uint64_t row = *reinterpret_cast<const uint64_t*>(reinterpret_cast<const char*>(vrow_at) +
                                                                         (src[d] & 0xffffu));
-                dma_gather16_nt(row + (src[d] >> 16), lds_v + 1024 * d);
-            }
-        };
-
-        // ---- int8 pages: through registers, the entries two tiles ahead, the rows one
-        constexpr int RCH = D / 16; // 16-byte chunks per int8 row
-        int32_t ent[C::NCH];
-        i4 kraw[C::NCH], vraw[C::NCH];
-        float ksc[C::NCH], vsc[C::NCH];
-        auto load_entries = [&](int j) {
-#pragma unroll
-            for (int c = 0; c < C::NCH; c++) {
-                const int e = (tile_key(j) + (64 * c + lane) / RCH) >> p.c.lps;
-                ent[c] = table[min(e, p.c.width - 1)];
-            }
-        };
-        auto load_raw = [&](int j) {
-#pragma unroll
-            for (int c = 0; c < C::NCH; c++) {
-                const int key = tile_key(j) + (64 * c + lane) / RCH;
-                const bool seen = key >= item.lo && key <= item.hi;
-                const int64_t pg = (uint32_t)ent[c] < (uint32_t)p.c.pages ? ent[c] : 0;
-                const int64_t off = (uint32_t)key & page_mask;
-                const int ch = 16 * (lane % RCH);
-                kraw[c] = __builtin_nontemporal_load(
-                    reinterpret_cast<const i4*>(kbase + pg * p.c.k_sp + off * p.c.k_st + ch));
-                vraw[c] = __builtin_nontemporal_load(
-                    reinterpret_cast<const i4*>(vbase + pg * p.c.v_sp + off * p.c.v_st + ch));
-                const float a = p.c.ks[pg * p.c.ks_sp + off * p.c.ks_st + h * p.c.ks_sh];
-                const float b = p.c.vs[pg * p.c.vs_sp + off * p.c.vs_st + h * p.c.vs_sh];
-                ksc[c] = seen ? a : 0.0f;
-                vsc[c] = seen ? b : 0.0f;
-            }
-        };
-        auto store_raw = [&]() {
-#pragma unroll
-            for (int c = 0; c < C::NCH; c++) {
-                const int r = (64 * c + lane) / RCH;
-                const int cl = 2 * (lane % RCH);
-                V8 a[2], b[2];
-#pragma unroll
-                for (int e = 0; e < 16; e++) {
-                    a[e >> 3][e & 7] = (T)((float)(int8_t)(kraw[c][e >> 2] >> (8 * (e & 3))) * ksc[c]);
-                    b[e >> 3][e & 7] = (T)((float)(int8_t)(vraw[c][e >> 2] >> (8 * (e & 3))) * vsc[c]);
-                }
-#pragma unroll
-                for (int i = 0; i < 2; i++) {
-                    *reinterpret_cast<V8*>(sk + r * C::RB + (((cl + i) ^ paged_swz<D>(r)) << 4)) = a[i];
-                    *reinterpret_cast<V8*>(sv + r * C::RB + (((cl + i) ^ paged_swz<D>(r)) << 4)) = b[i];
-                }
+                dma_gather16_nt(row + (src[d] >> 16), lds + 1024 * d);
             }
         };
 
         // The first tiles leave before the Q loads; the wait for Q drains them, once.
         if (my_tiles > 0) {
-            if constexpr (I8) {
-                load_entries(0);
-                load_raw(0);
-                load_entries(1);
-            } else {
-                issue_tab(0);
-                __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
-                issue_k(0);
-                __builtin_amdgcn_s_waitcnt(waitcnt_lgkm(0)); // the entries are read
-                issue_tab(1);
-                issue_v();
+#pragma unroll
+            for (int j = 0; j < C::SLOTS; j++) {
+                issue_tab(j);
+            }
+            __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
+#pragma unroll
+            for (int j = 0; j < C::SLOTS; j++) {
+                if (j < my_tiles) {
+                    issue_k(j);
+                    issue_v(j);
+                }
             }
         }
         V8 qreg[C::NS];
@@ -242,9 +226,7 @@ __global__ __launch_bounds__((StreamCfg<D, I8>::THREADS), (StreamCfg<D, I8>::WAV
                 qreg[s] = col_valid ? (p.q_sign < 0.0f ? -qreg[s] : qreg[s]) : V8{};
             }
         }
-        if constexpr (!I8) {
-            __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
-        }
+        __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
 
         f16x oacc[C::NDT];
 #pragma unroll
@@ -253,38 +235,54 @@ __global__ __launch_bounds__((StreamCfg<D, I8>::THREADS), (StreamCfg<D, I8>::WAV
         }
         float m_run = -INFINITY, l_run = 0.0f;
 
+        ValueScale vscale;
+
         for (int j = 0; j < my_tiles; j++) {
             const int kt0 = tile_key(j);
-            const bool more = j + 1 < my_tiles;
-            if constexpr (I8) {
-                store_raw();
-                if (more) {
-                    load_raw(j + 1);
-                    load_entries(j + 2);
-                }
+            const bool more = j + C::SLOTS < my_tiles; // a tile is issued into this one's slot
+            const bool next = C::SLOTS > 1 && j + 1 < my_tiles; // the other slot is in flight
+            // K(j) landed (and the entries of tile j + SLOTS): V(j) is younger, and the
+            // other slot's tiles
+            if (next) {
+                __builtin_amdgcn_s_waitcnt(waitcnt_vm(C::V_COPIES + (C::SLOTS - 1) * (C::K_COPIES + C::V_COPIES)));
             } else {
-                // K(j) and the entries of j + 1 landed: only V(j) is younger
-                __builtin_amdgcn_s_waitcnt(waitcnt_vm(C::DMA));
+                __builtin_amdgcn_s_waitcnt(waitcnt_vm(C::V_COPIES));
             }
+            const char* const sk = wsm + slot_of(j) * (2 * C::TILE_BYTES);
+            const char* const sv = sk + C::TILE_BYTES;
 
             // S^T[key][col] = K Q^T
             f16x sacc[1] = {f16x{}};
+            f4 vs[I8 ? 4 : 1]; // the values' scales, of the keys of this lane's scores
             {
                 const char* krow = sk + l32 * C::RB;
-                const int sw = paged_swz<D>(l32);
 #pragma unroll
                 for (int s = 0; s < C::NS; s++) {
-                    const V8 a = *reinterpret_cast<const V8*>(krow + (((2 * s + g) ^ sw) << 4));
+                    V8 a;
+                    if constexpr (I8) {
+                        a = widen_int8<T>(*reinterpret_cast<const i2v*>(krow + ((s ^ swz8<D>(l32)) << 4) + 8 * g));
+                    } else {
+                        a = *reinterpret_cast<const V8*>(krow + (((2 * s + g) ^ paged_swz<D>(l32)) << 4));
+                    }
                     sacc[0] = paged_mfma<T>(a, qreg[s], sacc[0]);
                 }
-            }
-            if constexpr (!I8) {
-                if (more) {
-                    __builtin_amdgcn_s_waitcnt(waitcnt_lgkm(0)); // every read of K(j) has returned
-                    issue_k(j + 1);
-                    __builtin_amdgcn_s_waitcnt(waitcnt_lgkm(0)); // the entries are read
-                    issue_tab(j + 2);
+                if constexpr (I8) {
+                    const f4* sc = reinterpret_cast<const f4*>(aux + C::TAB_BYTES + 256 * slot_of(j)) + g;
+                    f4 ks[4];
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        ks[i] = sc[2 * i];
+                        vs[i] = sc[8 + 2 * i];
+                    }
+#pragma unroll
+                    for (int e = 0; e < 16; e++) {
+                        sacc[0][e] *= ks[e >> 2][e & 3];
+                    }
                 }
+            }
+            if (more) {
+                __builtin_amdgcn_s_waitcnt(waitcnt_lgkm(0)); // every read of K(j) has returned
+                issue_k(j + C::SLOTS);
             }
             {
                 const int a = row_lo - kt0 - 4 * g;
@@ -314,50 +312,60 @@ __global__ __launch_bounds__((StreamCfg<D, I8>::THREADS), (StreamCfg<D, I8>::WAV
                 }
             }
             const float m_use = (m_run == -INFINITY) ? 0.0f : m_run;
-            V8 pb[2];
+            float pv[16];
             float ps[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int e = 0; e < 16; e++) {
-                const float pv = fast_exp2(fmaf(sacc[0][e], p.scale_log2e, -m_use));
-                ps[e & 3] += pv;
-                pb[e >> 3][e & 7] = (T)pv;
+                pv[e] = fast_exp2(fmaf(sacc[0][e], p.scale_log2e, -m_use));
+                ps[e & 3] += pv[e];
             }
             l_run += (ps[0] + ps[1]) + (ps[2] + ps[3]);
+            if constexpr (I8) {
+                vscale.weigh<4>(pv, vs, oacc);
+            }
+            P8 pb[2];
+#pragma unroll
+            for (int e = 0; e < 16; e++) {
+                pb[e >> 3][e & 7] = (P)pv[e];
+            }
 
-            if constexpr (!I8) {
-                // V(j) landed: only K(j + 1) and the entries of j + 2 are younger
-                if (more) {
-                    __builtin_amdgcn_s_waitcnt(waitcnt_vm(C::DMA + 1));
-                } else {
-                    __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
-                }
+            // V(j) landed: the other slot's tiles are younger, and what was issued above
+            if (more) {
+                __builtin_amdgcn_s_waitcnt(
+                    waitcnt_vm(C::K_COPIES + (C::SLOTS - 1) * (C::K_COPIES + C::V_COPIES)));
+            } else if (next) {
+                __builtin_amdgcn_s_waitcnt(waitcnt_vm((C::SLOTS - 1) * (C::K_COPIES + C::V_COPIES)));
+            } else {
+                __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
             }
             // O^T += V^T P^T; V^T operand through transpose reads
-            {
-                const int j16 = lane & 15;
+            const int j16 = lane & 15;
 #pragma unroll
-                for (int u = 0; u < 2; u++) {
+            for (int u = 0; u < 2; u++) {
 #pragma unroll
-                    for (int dt = 0; dt < C::NDT; dt++) {
+                for (int dt = 0; dt < C::NDT; dt++) {
+                    P8 a;
+                    if constexpr (I8) {
+                        const int r = 16 * u + 8 * (j16 >> 3) + 4 * g + ((j16 >> 1) & 3);
+                        const int c = 2 * dt + ((lane >> 4) & 1);
+                        a = widen_int8<P>(read_tr8(sv + r * C::RB + ((c ^ swz8<D>(r)) << 4) + 8 * (j16 & 1)));
+                    } else {
                         h4 half4[2];
 #pragma unroll
                         for (int hh = 0; hh < 2; hh++) {
                             const int r = 16 * u + 8 * hh + 4 * g + (j16 >> 2);
                             const int d = 32 * dt + 16 * ((lane >> 4) & 1) + 4 * (j16 & 3);
-                            const char* addr =
-                                sv + r * C::RB + (((d >> 3) ^ paged_swz<D>(r)) << 4) + ((d & 7) << 1);
+                            const char* addr = sv + r * C::RB + (((d >> 3) ^ paged_swz<D>(r)) << 4) + ((d & 7) << 1);
                             half4[hh] = lds_read_tr16(reinterpret_cast<const _Float16*>(addr));
                         }
-                        const h8 a = __builtin_shufflevector(half4[0], half4[1], 0, 1, 2, 3, 4, 5, 6, 7);
-                        oacc[dt] = paged_mfma<T>(__builtin_bit_cast(V8, a), pb[u], oacc[dt]);
+                        a = __builtin_bit_cast(P8, __builtin_shufflevector(half4[0], half4[1], 0, 1, 2, 3, 4, 5, 6, 7));
                     }
+                    oacc[dt] = paged_mfma<P>(a, pb[u], oacc[dt]);
                 }
             }
-            if constexpr (!I8) {
-                if (more) {
-                    __builtin_amdgcn_s_waitcnt(waitcnt_lgkm(0)); // every read of V(j) has returned
-                    issue_v();
-                }
+            if (more) {
+                __builtin_amdgcn_s_waitcnt(waitcnt_lgkm(0)); // every read of V(j) has returned
+                issue_v(j + C::SLOTS);
             }
         }
         __builtin_amdgcn_s_waitcnt(0);
@@ -384,6 +392,9 @@ __global__ __launch_bounds__((StreamCfg<D, I8>::THREADS), (StreamCfg<D, I8>::WAV
                 lsum += sm_ml[(w * 32 + l32) * 2 + 1] * part_weight(sm_ml[(w * 32 + l32) * 2], mref);
             }
             float scale_w = part_weight(m_run, mref);
+            if constexpr (I8) {
+                scale_w *= vscale.factor();
+            }
             if (whole) {
                 scale_w *= lsum > 0.0f ? 1.0f / lsum : 0.0f;
             }

@@ -28,7 +28,8 @@ struct TileCfg {
     static constexpr int RB = 2 * D;
     static constexpr int KCH = D / 8;
     static constexpr int TILE_BYTES = kBN * RB;
-    static constexpr int TAB_BYTES = I8 ? 0 : WAVES * 256;
+    // the waves' table entries; of int8 the scales of two slots' keys and values
+    static constexpr int TAB_BYTES = I8 ? 2 * 2 * kBN * 4 : WAVES * 256;
     static constexpr int NS = D / 16;
     static constexpr int NDT = D / 32;
     static constexpr int DMA = TILE_BYTES / 1024;                  // 1 KB copies of a tile
@@ -44,6 +45,8 @@ __global__ __launch_bounds__((TileCfg<D, I8>::THREADS), (TileCfg<D, I8>::WAVES_P
     using C = TileCfg<D, I8>;
     using V8 = typename PagedVec<T>::v8;
     using V4 = typename PagedVec<T>::v4;
+    using P = std::conditional_t<I8, _Float16, T>; // weights and values, see paged_stream
+    using P8 = typename PagedVec<P>::v8;
     // K and V of slot 0, of slot 1; the waves' table entries
     __shared__ __attribute__((aligned(16))) char dsm[4 * C::TILE_BYTES + C::TAB_BYTES];
 
@@ -144,8 +147,10 @@ __global__ __launch_bounds__((TileCfg<D, I8>::THREADS), (TileCfg<D, I8>::WAVES_P
             }
         };
 
-        // ---- int8 pages: through registers, dequantised to the queries' type
+        // ---- int8 pages: through registers, widened exactly (once for all waves); the
+        // scales beside them
         constexpr int RCH = D / 16;
+        float* const scales = reinterpret_cast<float*>(dsm + 4 * C::TILE_BYTES); // [slot][keys, values][kBN]
         auto chunk_row = [&](int c) { return (C::THREADS * c + tid) / RCH % kBN; };
         int32_t ent[C::NCH];
         i4 kraw[C::NCH], vraw[C::NCH];
@@ -179,20 +184,18 @@ __global__ __launch_bounds__((TileCfg<D, I8>::THREADS), (TileCfg<D, I8>::WAVES_P
             for (int c = 0; c < C::NCH; c++) {
                 const int r = chunk_row(c);
                 const int cl = 2 * (tid % RCH);
-                V8 a[2], b[2];
-#pragma unroll
-                for (int e = 0; e < 16; e++) {
-                    a[e >> 3][e & 7] = (T)((float)(int8_t)(kraw[c][e >> 2] >> (8 * (e & 3))) * ksc[c]);
-                    b[e >> 3][e & 7] = (T)((float)(int8_t)(vraw[c][e >> 2] >> (8 * (e & 3))) * vsc[c]);
-                }
                 if (C::CHUNKS % C::THREADS != 0 && C::THREADS * c + tid >= C::CHUNKS) {
                     continue;
                 }
 #pragma unroll
                 for (int x = 0; x < 2; x++) {
                     char* const at = sk + r * C::RB + (((cl + x) ^ paged_swz<D>(r)) << 4);
-                    *reinterpret_cast<V8*>(at) = a[x];
-                    *reinterpret_cast<V8*>(at + C::TILE_BYTES) = b[x];
+                    *reinterpret_cast<V8*>(at) = widen_int8<T>(i2v{kraw[c][2 * x], kraw[c][2 * x + 1]});
+                    *reinterpret_cast<P8*>(at + C::TILE_BYTES) = widen_int8<P>(i2v{vraw[c][2 * x], vraw[c][2 * x + 1]});
+                }
+                if (cl == 0) {
+                    scales[(i & 1) * 2 * kBN + r] = ksc[c];
+                    scales[(i & 1) * 2 * kBN + kBN + r] = vsc[c];
                 }
             }
         };
@@ -235,6 +238,7 @@ __global__ __launch_bounds__((TileCfg<D, I8>::THREADS), (TileCfg<D, I8>::WAVES_P
             oacc[dt] = f16x{};
         }
         float m_run = -INFINITY, l_run = 0.0f;
+        ValueScale vscale;
 
         for (int i = 0; i < nt; i++) {
             // this wave's copies of tile i (and the entries of i + 1) have landed; behind
@@ -261,6 +265,17 @@ __global__ __launch_bounds__((TileCfg<D, I8>::THREADS), (TileCfg<D, I8>::WAVES_P
                         const V8 a =
                             *reinterpret_cast<const V8*>(sk + r * C::RB + (((2 * s + g) ^ paged_swz<D>(r)) << 4));
                         sacc[kt] = paged_mfma<T>(a, qreg[s], sacc[kt]);
+                    }
+                }
+                if constexpr (I8) {
+                    const f4* sc = reinterpret_cast<const f4*>(scales + (i & 1) * 2 * kBN) + g;
+#pragma unroll
+                    for (int x = 0; x < 8; x++) {
+                        const f4 ks = sc[2 * x];
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            sacc[x >> 2][4 * (x & 3) + e] *= ks[e];
+                        }
                     }
                 }
                 if (what == 2) {
@@ -291,15 +306,28 @@ __global__ __launch_bounds__((TileCfg<D, I8>::THREADS), (TileCfg<D, I8>::WAVES_P
                     }
                 }
                 const float m_use = (m_run == -INFINITY) ? 0.0f : m_run;
-                V8 pb[4];
+                float pv[32];
                 float ps[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                 for (int e = 0; e < 32; e++) {
-                    const float pv = fast_exp2(fmaf(sacc[e >> 4][e & 15], p.scale_log2e, -m_use));
-                    ps[e & 3] += pv;
-                    pb[e >> 3][e & 7] = (T)pv;
+                    pv[e] = fast_exp2(fmaf(sacc[e >> 4][e & 15], p.scale_log2e, -m_use));
+                    ps[e & 3] += pv[e];
                 }
                 l_run += (ps[0] + ps[1]) + (ps[2] + ps[3]);
+                if constexpr (I8) {
+                    const f4* sc = reinterpret_cast<const f4*>(scales + (i & 1) * 2 * kBN + kBN) + g;
+                    f4 vs[8];
+#pragma unroll
+                    for (int x = 0; x < 8; x++) {
+                        vs[x] = sc[2 * x];
+                    }
+                    vscale.weigh<8>(pv, vs, oacc);
+                }
+                P8 pb[4];
+#pragma unroll
+                for (int e = 0; e < 32; e++) {
+                    pb[e >> 3][e & 7] = (P)pv[e];
+                }
                 const int j16 = lane & 15;
 #pragma unroll
                 for (int u = 0; u < 4; u++) {
@@ -315,7 +343,7 @@ __global__ __launch_bounds__((TileCfg<D, I8>::THREADS), (TileCfg<D, I8>::WAVES_P
                             half4[hh] = lds_read_tr16(reinterpret_cast<const _Float16*>(addr));
                         }
                         const h8 a = __builtin_shufflevector(half4[0], half4[1], 0, 1, 2, 3, 4, 5, 6, 7);
-                        oacc[dt] = paged_mfma<T>(__builtin_bit_cast(V8, a), pb[u], oacc[dt]);
+                        oacc[dt] = paged_mfma<P>(__builtin_bit_cast(P8, a), pb[u], oacc[dt]);
                     }
                 }
             }
@@ -331,8 +359,9 @@ __global__ __launch_bounds__((TileCfg<D, I8>::THREADS), (TileCfg<D, I8>::WAVES_P
         __syncthreads(); // the next item's copies overwrite the slots
 
         const float l_tot = pair_sum(l_run);
+        const float unit = I8 ? vscale.factor() : 1.0f; // of O
         if (whole) {
-            const float inv = l_tot > 0.0f ? 1.0f / l_tot : 0.0f;
+            const float inv = l_tot > 0.0f ? unit / l_tot : 0.0f;
             if (col_valid) {
                 char* const orow = p.o + (int64_t)(seq.q0 + tok) * p.o_st + head * p.o_sh;
 #pragma unroll
@@ -349,7 +378,7 @@ __global__ __launch_bounds__((TileCfg<D, I8>::THREADS), (TileCfg<D, I8>::WAVES_P
             const int64_t slot = walk.slot();
             if (col_valid) {
                 store_partial<C::NDT>(oacc, m_run, l_tot, g == 0, p.part_o, p.part_ml, slot * C::ROWS + col, D, 0, g,
-                                      [](int) { return f4{1.0f, 1.0f, 1.0f, 1.0f}; });
+                                      [&](int) { return f4{unit, unit, unit, unit}; });
             }
             if (walk.at == 0) {
                 rec = PagedRecord{n_rows, seq.q0, r0, h, walk.last_wg(), {}};

@@ -122,17 +122,19 @@ def reference(q, k, v, ok, scale, dtype, i8):
 
     With u half a step of `dtype`: the weights p are rounded to it (u A, A = sum
     p |v|; below fp16's normal range by at most 2^-25 each, relative to a largest
-    weight of at least 1 before the division by the sum), int8 keys and values
-    are rounded to it when they are dequantised (u A of the values; scores off by
-    u scale |q| |k|), the scores are sums of d products in 32 bits ((d + 2) 2^-24
-    of the sum of magnitudes, and their own size times 2^-22 in the exponent,
-    whose function is good to 2^-21; sums and the merge of parts 2^-18 of A in
-    all), a change ds of the scores changes the output by at most 2 ds A, and the
-    output is rounded once (u |out|; 2^-25 in fp16's subnormal range)."""
+    weight of at least 1 before the division by the sum), the scores are sums of d
+    products in 32 bits ((d + 2) 2^-24 of the sum of magnitudes, and their own size
+    times 2^-22 in the exponent, whose function is good to 2^-21; sums and the merge
+    of parts 2^-18 of A in all), a change ds of the scores changes the output by at
+    most 2 ds A, and the output is rounded once (u |out|; 2^-25 in fp16's subnormal
+    range).  int8 keys and values are exact, their scales meet the scores and the
+    weights in 32 bits (2^-23 more), and the weights are fp16's, within 2^-31 of the
+    largest value each where they are small."""
+    u = _round_unit(dtype)
+    w = _round_unit(torch.float16) if i8 else u
+    sub = 2.0 ** -25 if dtype == torch.float16 else 0.0
     n, hq, d = q.shape
     length, hkv, _ = k.shape
-    u = _round_unit(dtype)
-    sub = 2.0 ** -25 if dtype == torch.float16 else 0.0
     out = torch.zeros(n, hq, d, dtype=torch.float64)
     tol = torch.full((n, hq, d), max(sub, 1e-30), dtype=torch.float64)
     if length == 0 or n == 0:
@@ -148,11 +150,11 @@ def reference(q, k, v, ok, scale, dtype, i8):
         p[seen] = torch.softmax(s[seen], -1)
         o = p @ vh
         a = p @ vh.abs()
-        ds = (mag * ((d + 2) * 2.0 ** -24 + 2.0 ** -22 + (u if i8 else 0.0))).masked_fill(~ok, 0.0).amax(-1, keepdim=True)
+        ds = (mag * ((d + 2) * 2.0 ** -24 + 2.0 ** -22 + (2.0 ** -23 if i8 else 0.0))).masked_fill(~ok, 0.0).amax(-1, keepdim=True)
         ds = ds + 2.0 ** -21
-        vsum = (ok.double() @ vh.abs())
+        vsum = ok.double() @ (torch.full_like(vh, float(vh.abs().max()) * 2.0 ** -31) if i8 else vh.abs() * sub)
         out[:, h] = o
-        tol[:, h] += u * a * (2 if i8 else 1) + 2 * ds * a + 2.0 ** -18 * a + u * o.abs() * 1.01 + sub * vsum
+        tol[:, h] += w * a + 2 * ds * a + 2.0 ** -18 * a + u * o.abs() * 1.01 + vsum
     return out, tol
 
 

@@ -382,6 +382,25 @@ def test_same_bits_every_time(gpu):
             assert torch.equal(ra.paged_attention(q, k, v, table, lens), first)
 
 
+@pytest.mark.parametrize("ns", [[1, 1, 1], [70, 64, 90]])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_int8_scales_of_any_size(gpu, ns, dtype):
+    """Scales from 2^-40 to 2^6, growing and falling along the keys, zeros and
+    negative ones among them: the weights they meet stay in fp16's range."""
+    pool = Pool([600, 64, 90], 2, 64, 16, dtype, True, seed=26)
+    for b, lo, hi in ((0, -40, 6), (1, -30, -10), (2, 6, -40)):
+        n = pool.lens[b]
+        at = pool.where(b, torch.arange(n))
+        pool.vs[at] = torch.exp2(torch.linspace(lo, hi, n))[:, None].expand(n, 2)
+    at = pool.where(0, torch.arange(0, 600, 7))
+    pool.vs[at] = 0.0
+    at = pool.where(0, torch.arange(3, 600, 11))
+    pool.vs[at] = -pool.vs[at]
+    at = pool.where(2, torch.arange(0, 90, 5))
+    pool.ks[at] = -pool.ks[at]
+    run(gpu, pool, ns, 4, name="scales")
+
+
 def test_large_scores(gpu):
     """Scores of hundreds of log2 units: the running maximum moves often, most
     weights vanish."""
