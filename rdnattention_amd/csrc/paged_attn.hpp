@@ -25,16 +25,16 @@ __device__ __forceinline__ f16x paged_mfma(typename PagedVec<T>::v8 a, typename 
 }
 
 // What a share of the work leaves where an item has several: slot w holds the
-// part of workgroup w's first item that began before w, slot n_wg + w the part of
-// its last item that goes on behind it (rows of ROWS: O unnormalised in fp32,
-// then (m, l) with m in log2 units).  The record of workgroup w names the item
+// part of worker w's first item that began before w, slot n_wg + w the part of
+// its last item that goes on behind it (slot_rows rows: O unnormalised in fp32,
+// then (m, l) with m in log2 units).  The record of worker w names the item
 // that starts in it and goes on, for the merge.
 struct PagedRecord {
     int32_t rows;   // 0: none
     int32_t q0;     // first token of the sequence
     int32_t r0;     // first row of the item
     int32_t h;      // kv head
-    int32_t w_last; // the last workgroup of the item
+    int32_t w_last; // the last worker of the item
     int32_t unused[3];
 };
 
@@ -51,6 +51,7 @@ struct PagedAttnParams {
     const uint8_t* tree; // null: no tree
     int64_t tree_sb, tree_sr;
     int32_t tree_n;
+    int32_t slot_rows; // rows of a slot
     float* part_o;
     float* part_ml;
     PagedRecord* records;
@@ -174,11 +175,38 @@ struct ValueScale {
     }
 };
 
+// use(j, op(j)) for j < N, op (an LDS read of an MFMA operand) DEPTH ahead of use.
+// Left to itself the compiler reads each operand as it is needed and waits for it.
+template <int N, int DEPTH, class Op, class Use>
+__device__ __forceinline__ void operand_stream(Op&& op, Use&& use) {
+    decltype(op(0)) ring[DEPTH];
+#pragma unroll
+    for (int j = 0; j < DEPTH && j < N; j++) {
+        ring[j] = op(j);
+    }
+#pragma unroll
+    for (int j = 0; j < N; j++) {
+        const auto a = ring[j % DEPTH];
+        if (j + DEPTH < N) {
+            ring[j % DEPTH] = op(j + DEPTH);
+        }
+        use(j, a);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+}
+
+// Number `i` of n, where workgroup id runs on XCD id % 8, so that neighbouring numbers
+// are on one XCD.
+__device__ __forceinline__ int32_t by_xcd(int32_t id, int32_t n) {
+    return (n & 7) == 0 ? (id & 7) * (n >> 3) + (id >> 3) : id;
+}
+
 __device__ __forceinline__ int32_t uniform(int32_t x) {
     return __builtin_amdgcn_readfirstlane(x);
 }
 
-// A workgroup's walk over its units, the same in every wave.
+// A worker's (a workgroup's, or a wave's) walk over its units, the same in every wave
+// of it.
 template <int ROWS, int BN>
 struct PagedWalk {
     const PagedWork& w;
@@ -191,22 +219,19 @@ struct PagedWalk {
     PagedSeq seq;
     PagedTile tile;
 
-    __device__ __forceinline__ explicit PagedWalk(const PagedWork& work) : w(work) {
-        // Workgroup id runs on XCD id % 8: neighbouring shares, which have heads (and
-        // with many row tiles also keys) in common, on one XCD.
-        const int32_t id = blockIdx.x;
-        wg = (w.n_wg & 7) == 0 ? (id & 7) * (w.n_wg >> 3) + (id >> 3) : id;
+    __device__ __forceinline__ PagedWalk(const PagedWork& work, int32_t worker) : w(work), wg(worker) {
         const int lane = threadIdx.x & 63;
         const int32_t B = w.seqs.B;
-        int32_t total = 0, mine = 0;
-        for (int32_t i = 0; i < B; i += 64) {
-            mine = 0;
-            if (i + lane < B) {
-                mine = paged_head_units<ROWS, BN>(w, paged_seq(w.seqs, i + lane)) * w.Hkv;
-            }
-            total += wave_sum(mine);
+        auto units_of = [&](int32_t i) {
+            return i < B ? paged_head_units<ROWS, BN>(w, paged_seq(w.seqs, i)) * w.Hkv : 0;
+        };
+        // units of all sequences; of the first 64 (often all) the sums stay
+        const int32_t mine = units_of(lane);
+        const int32_t sum = wave_prefix(mine);
+        int32_t total = __builtin_amdgcn_readlane(sum, 63);
+        for (int32_t i = 64; i < B; i += 64) {
+            total += __builtin_amdgcn_readlane(wave_prefix(units_of(i + lane)), 63);
         }
-        total = uniform(total);
         share = paged_share(w, total);
         start = (int32_t)((int64_t)wg * share < total ? wg * share : total);
         left = mask_imin(share, total - start);
@@ -215,28 +240,20 @@ struct PagedWalk {
             return;
         }
         // the sequence that unit `start` is in
-        int32_t before = 0;
+        int32_t before = 0, m = mine, s = sum;
         for (int32_t i = 0; i < B; i += 64) {
-            if (B > 64) {
-                mine = 0;
-                if (i + lane < B) {
-                    mine = paged_head_units<ROWS, BN>(w, paged_seq(w.seqs, i + lane)) * w.Hkv;
-                }
+            if (i > 0) {
+                m = units_of(i + lane);
+                s = wave_prefix(m);
             }
-            int32_t sum = mine;
-#pragma unroll
-            for (int d = 1; d < 64; d <<= 1) {
-                const int32_t x = __shfl_up(sum, d);
-                sum += lane >= d ? x : 0;
-            }
-            const uint64_t past = __builtin_amdgcn_ballot_w64(before + sum > start);
+            const uint64_t past = __builtin_amdgcn_ballot_w64(before + s > start);
             if (past != 0) {
                 const int l = __builtin_ctzll(past);
                 b = i + l;
-                before += __shfl(sum, l) - __shfl(mine, l);
+                before += __builtin_amdgcn_readlane(s, l) - __builtin_amdgcn_readlane(m, l);
                 break;
             }
-            before += __shfl(sum, 63);
+            before += __builtin_amdgcn_readlane(s, 63);
         }
         b = uniform(b);
         at = start - uniform(before);
@@ -257,11 +274,16 @@ struct PagedWalk {
         }
     }
 
-    static __device__ __forceinline__ int32_t wave_sum(int32_t x) {
-#pragma unroll
-        for (int d = 32; d > 0; d >>= 1) {
-            x += __shfl_xor(x, d);
-        }
+    // Sums of x over this lane and those below it: within rows of 16 lanes by shifts,
+    // then row 0's last into row 1 and row 2's into row 3, then lane 31's into the
+    // upper half.
+    static __device__ __forceinline__ int32_t wave_prefix(int32_t x) {
+        x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true); // row_shr:1
+        x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true);
+        x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true);
+        x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true);
+        x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false); // row_bcast:15
+        x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false); // row_bcast:31
         return x;
     }
 

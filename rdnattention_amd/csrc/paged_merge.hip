@@ -21,9 +21,10 @@ struct MergeParams {
     int64_t o_st, o_sh;
     int32_t n_wg, rows, D, G; // rows of a slot
     int32_t rpb;              // rows of a workgroup
+    int32_t weights;          // room for each in LDS
 };
 
-// Workgroup (w, y): rows y * rpb ... of the item that starts in workgroup w and
+// Workgroup (w, y): rows y * rpb ... of the item that starts in worker w and
 // goes on behind it, if there is one: the log-sum-exp merge of its parts, in
 // fp32, rounded once.  Bound by latency: the lanes of a wave take the parts'
 // weights side by side, then groups of threads the parts' O, four loads in
@@ -31,7 +32,7 @@ struct MergeParams {
 template <class T>
 __global__ __launch_bounds__(kMergeThreads) void paged_merge_rows(MergeParams p) {
     using V4 = typename PagedVec<T>::v4;
-    __shared__ __attribute__((aligned(16))) float wgt[kMergeRows * kPagedMaxWg];
+    __shared__ __attribute__((aligned(16))) float wgt[kPagedMaxWorkers];
     __shared__ __attribute__((aligned(16))) f4 red[kMergeThreads];
     const int w = blockIdx.x;
     const PagedRecord rec = p.records[w];
@@ -58,7 +59,7 @@ __global__ __launch_bounds__(kMergeThreads) void paged_merge_rows(MergeParams p)
             const float2 v = ml[slot(s) + row0 + r];
             const float e = part_weight(v.x, mx);
             sum += v.y * e;
-            wgt[r * kPagedMaxWg + s] = v.y != 0.0f ? e : -1.0f;
+            wgt[r * p.weights + s] = v.y != 0.0f ? e : -1.0f;
         }
 #pragma unroll
         for (int off = 32; off > 0; off >>= 1) {
@@ -66,7 +67,7 @@ __global__ __launch_bounds__(kMergeThreads) void paged_merge_rows(MergeParams p)
         }
         const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
         for (int s = lane; s < n; s += 64) {
-            wgt[r * kPagedMaxWg + s] *= wgt[r * kPagedMaxWg + s] < 0.0f ? 1.0f : inv;
+            wgt[r * p.weights + s] *= wgt[r * p.weights + s] < 0.0f ? 1.0f : inv;
         }
     }
     __syncthreads();
@@ -89,11 +90,11 @@ __global__ __launch_bounds__(kMergeThreads) void paged_merge_rows(MergeParams p)
             }
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                add(x[i], wgt[r * kPagedMaxWg + s + i * per]);
+                add(x[i], wgt[r * p.weights + s + i * per]);
             }
         }
         for (; s < n; s += per) {
-            add(*reinterpret_cast<const f4*>(o + slot(s) * p.D), wgt[r * kPagedMaxWg + s]);
+            add(*reinterpret_cast<const f4*>(o + slot(s) * p.D), wgt[r * p.weights + s]);
         }
     }
     if (per > 1) {
@@ -115,7 +116,7 @@ __global__ __launch_bounds__(kMergeThreads) void paged_merge_rows(MergeParams p)
 
 } // namespace
 
-int paged_merge(const PagedAttnArgs& a, const PagedAttnParams& p, int rows, hipStream_t stream, std::string& err) {
+int paged_merge(const PagedAttnArgs& a, const PagedAttnParams& p, hipStream_t stream, std::string& err) {
     MergeParams m;
     m.part_o = p.part_o;
     m.part_ml = p.part_ml;
@@ -124,13 +125,13 @@ int paged_merge(const PagedAttnArgs& a, const PagedAttnParams& p, int rows, hipS
     m.o_st = p.o_st;
     m.o_sh = p.o_sh;
     m.n_wg = p.work.n_wg;
-    m.rows = rows;
+    m.rows = p.slot_rows;
     m.D = a.D;
     m.G = p.work.G;
     // few rows with many parts: a row per workgroup
-    m.rpb = rows <= 32 ? 1 : std::min(kMergeRows, kMergeThreads / (a.D / 4));
-    const int64_t most = std::min<int64_t>(rows, (int64_t)p.work.seqs.total * m.G);
-    const dim3 grid((uint32_t)m.n_wg, (uint32_t)((most + m.rpb - 1) / m.rpb));
+    m.rpb = p.slot_rows <= 32 ? 1 : std::min({kMergeRows, kMergeThreads / (a.D / 4), kPagedMaxWorkers / m.n_wg});
+    m.weights = kPagedMaxWorkers / m.rpb;
+    const dim3 grid((uint32_t)m.n_wg, (uint32_t)((m.rows + m.rpb - 1) / m.rpb));
     if (a.type == PagedType::F16) {
         hipLaunchKernelGGL(paged_merge_rows<_Float16>, grid, dim3(kMergeThreads), 0, stream, m);
     } else {

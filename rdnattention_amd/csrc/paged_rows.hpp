@@ -7,12 +7,12 @@
 // and page tables are device memory that the host does not see, so every value
 // is bounded here and no access leaves a buffer, whatever they hold.
 //
-// The attention kernels deal a call's key tiles to their workgroups in equal
-// shares: the rows (n tokens of G query heads each) of every (sequence, kv
+// The attention kernels deal a call's key tiles to their workers (workgroups, or
+// waves) in equal shares: the rows (n tokens of G query heads each) of every (sequence, kv
 // head) fall into row tiles of ROWS rows, a row tile is an item of as many
 // units as it sees key tiles of BN keys (one if none, for its zeros), and
-// workgroup w takes the units [w * per, (w + 1) * per) of the items in order
-// (sequence, kv head, row tile).  At most two of a workgroup's items are shared
+// worker w takes the units [w * per, (w + 1) * per) of the items in order
+// (sequence, kv head, row tile).  At most two of a worker's items are shared
 // with others: the first and the last.
 #pragma once
 
@@ -88,7 +88,7 @@ RDNA_MASK_FN MaskSpec paged_mask(const PagedMask& m, const PagedSeq& s) {
 }
 
 // Work of a call: sequences with more than min_rows and at most max_rows rows
-// (tokens times G) are dealt to n_wg workgroups.
+// (tokens times G) are dealt to n_wg workers.
 struct PagedWork {
     PagedSeqs seqs;
     PagedMask mask;
@@ -141,7 +141,7 @@ RDNA_MASK_FN int32_t paged_head_units(const PagedWork& w, const PagedSeq& s) {
     return u;
 }
 
-// Share of each workgroup of `total` units.
+// Share of each worker of `total` units.
 RDNA_MASK_FN int32_t paged_share(const PagedWork& w, int32_t total) {
     return mask_imax((total + w.n_wg - 1) / w.n_wg, w.min_units);
 }

@@ -64,7 +64,8 @@ __global__ __launch_bounds__((TileCfg<D, I8>::THREADS), (TileCfg<D, I8>::WAVES_P
         zero_tail_rows<D>(p);
     }
     PagedRecord rec = {};
-    PagedWalk<C::ROWS, kBN> walk(p.work);
+    // row tiles of one head, which read the same keys, through one L2
+    PagedWalk<C::ROWS, kBN> walk(p.work, by_xcd(blockIdx.x, p.work.n_wg));
 
     while (walk.more()) {
         const PagedSeq seq = walk.seq;
@@ -377,7 +378,7 @@ __global__ __launch_bounds__((TileCfg<D, I8>::THREADS), (TileCfg<D, I8>::WAVES_P
         } else {
             const int64_t slot = walk.slot();
             if (col_valid) {
-                store_partial<C::NDT>(oacc, m_run, l_tot, g == 0, p.part_o, p.part_ml, slot * C::ROWS + col, D, 0, g,
+                store_partial<C::NDT>(oacc, m_run, l_tot, g == 0, p.part_o, p.part_ml, slot * p.slot_rows + col, D, 0, g,
                                       [&](int) { return f4{unit, unit, unit, unit}; });
             }
             if (walk.at == 0) {
@@ -401,7 +402,7 @@ int paged_tile_attention(const PagedAttnArgs& a, PagedAttnParams& p, const Paged
         constexpr int D = decltype(d)::value;
         constexpr bool I8 = decltype(i8)::value;
         using C = TileCfg<D, I8>;
-        return paged_launch<C::ROWS, kBN>(a, reinterpret_cast<const void*>(&paged_tiles<T, D, I8>), C::THREADS, 4, p, l,
+        return paged_launch<C::ROWS, kBN>(a, reinterpret_cast<const void*>(&paged_tiles<T, D, I8>), C::THREADS, 1, 4, p, l,
                                           stream, err, [&](dim3 grid) {
                                               hipLaunchKernelGGL((paged_tiles<T, D, I8>), grid, dim3(C::THREADS), 0,
                                                                  stream, p);

@@ -119,6 +119,16 @@ def test_many_sequences(gpu):
     run(gpu, pool, ns, 4, name="200 sequences, chunks among them")
 
 
+@pytest.mark.parametrize("dtype,i8,d", [(F16, False, 128), (BF16, False, 96), (F16, True, 128)])
+def test_many_heads(gpu, dtype, i8, d):
+    """512 kv heads and more of all sequences: workgroups of four waves, most of
+    them with several whole heads."""
+    lens = [(53 * b) % 400 + 1 for b in range(130)]
+    lens[7], lens[100] = 3000, 0
+    pool = Pool(lens, 4, d, 16, dtype, i8, seed=30)
+    run(gpu, pool, [1] * 130, 8, uniform=True, name="many heads")
+
+
 @pytest.mark.parametrize("causal", [True, False])
 @pytest.mark.parametrize("window", [-1, 1, 2, 17, 64, 100, 5000, 2 ** 31 - 1])
 def test_masks(gpu, causal, window):
