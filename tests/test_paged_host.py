@@ -42,9 +42,30 @@ _hold = ctypes.create_string_buffer(4096 + 64)
 _P = (ctypes.addressof(_hold) + 63) // 64 * 64
 
 
-def cache(**kw):
-    from rdnattention.paged import _Cache
+class _Cache(ctypes.Structure):
+    """rdna_paged_cache (include/rdnattention_ext.h)."""
 
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("key", "value", "key_scale", "value_scale", "block_tables", "seq_lens",
+                                                "cu_seqlens")] +
+                [(f"{n}_stride_{a}", ctypes.c_int64) for n in ("key", "value", "key_scale", "value_scale")
+                 for a in ("page", "token", "head")] +
+                [("table_stride", ctypes.c_int64)] +
+                [(n, ctypes.c_uint32) for n in ("num_pages", "page_size", "table_width", "num_seqs", "num_kv_heads",
+                                                "head_dim")] +
+                [("dtype", ctypes.c_int32)])
+
+
+def test_packed_cache_has_the_layout_of_the_struct():
+    from rdnattention.paged import _CACHE
+
+    values = list(range(1, 28))
+    names = [n for n, _ in _Cache._fields_]
+    assert len(names) == len(values)
+    c = _Cache.from_buffer_copy(_CACHE.pack(*values).ljust(ctypes.sizeof(_Cache), b"\0"))
+    assert [getattr(c, n) for n in names] == values
+
+
+def cache(**kw):
     c = _Cache(key=_P, value=_P, block_tables=_P, seq_lens=_P, num_pages=4, page_size=16, table_width=3, num_seqs=2,
                num_kv_heads=2, head_dim=64, dtype=0, table_stride=3)
     for n in ("key", "value"):
@@ -59,7 +80,7 @@ def attention(lib, c, **kw):
     a = dict(query=_P, output=_P, qs=256, qh=64, os=256, oh=64, rows=4, heads=4, dtype=0, most=4, scale=0.1, causal=1,
              window=-1, tree=None, tsb=0, tsr=0, tn=0, zero=0)
     a.update(kw)
-    rc = lib.rdna_paged_attention(c, *a.values(), None)
+    rc = lib.rdna_paged_attention(ctypes.addressof(c) if c is not None else None, *a.values(), None)
     return rc, lib.rdna_get_error().decode()
 
 
@@ -67,14 +88,14 @@ def append(lib, c, **kw):
     a = dict(key=_P, value=_P, ks=128, kh=64, vs=128, vh=64, rows=4, dtype=0, query=None, out=None, qs=256, qh=64,
              os=256, oh=64, heads=4, pos=None, cos=None, sin=None, rot_rows=8, rot_dim=64, pairs=1)
     a.update(kw)
-    rc = lib.rdna_paged_append(c, *a.values(), None)
+    rc = lib.rdna_paged_append(ctypes.addressof(c) if c is not None else None, *a.values(), None)
     return rc, lib.rdna_get_error().decode()
 
 
 def commit(lib, c, **kw):
     a = dict(prefix=_P, path=_P, stride=4, n=4, lens=_P)
     a.update(kw)
-    rc = lib.rdna_paged_commit(c, *a.values(), None)
+    rc = lib.rdna_paged_commit(ctypes.addressof(c) if c is not None else None, *a.values(), None)
     return rc, lib.rdna_get_error().decode()
 
 
