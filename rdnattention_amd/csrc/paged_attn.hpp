@@ -76,24 +76,45 @@ __device__ __forceinline__ int paged_swz(int r) {
 // meets a weight of zero as infinity or NaN.
 __device__ __attribute__((aligned(16))) const uint32_t kPagedZeroRow[256 / 2] = {};
 
+// A value that is the same in every lane, in a scalar register.
+__device__ __forceinline__ int32_t uniform(int32_t x) {
+    return __builtin_amdgcn_readfirstlane(x);
+}
+__device__ __forceinline__ uint64_t uniform64(uint64_t x) {
+    return ((uint64_t)(uint32_t)uniform((int32_t)(x >> 32)) << 32) | (uint32_t)uniform((int32_t)(uint32_t)x);
+}
+
+// Lane x's value of all lanes.
+__device__ __forceinline__ uint64_t readlane64(uint64_t v, int x) {
+    return ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int32_t)(v >> 32), x) << 32) |
+           (uint32_t)__builtin_amdgcn_readlane((int32_t)(uint32_t)v, x);
+}
+
 // HBM -> LDS copies with a 64-bit address per lane (see dma_load16)
 __device__ __forceinline__ void dma_gather16(uint64_t addr, uint32_t lds_byte_addr) {
     asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off"
                  :
-                 : "v"(addr), "s"(lds_byte_addr)
+                 : "v"(addr), "s"(uniform((int32_t)lds_byte_addr))
+                 : "memory", "m0");
+}
+// ... at a wave-uniform address and 32 bits per lane
+__device__ __forceinline__ void dma_uniform16(uint64_t base, uint32_t off, uint32_t lds_byte_addr) {
+    asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1"
+                 :
+                 : "v"(off), "s"(uniform64(base)), "s"(uniform((int32_t)lds_byte_addr))
                  : "memory", "m0");
 }
 __device__ __forceinline__ void dma_gather16_nt(uint64_t addr, uint32_t lds_byte_addr) {
     asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off nt"
                  :
-                 : "v"(addr), "s"(lds_byte_addr)
+                 : "v"(addr), "s"(uniform((int32_t)lds_byte_addr))
                  : "memory", "m0");
 }
 
 __device__ __forceinline__ void dma_gather4(uint64_t addr, uint32_t lds_byte_addr) {
     asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dword %0, off"
                  :
-                 : "v"(addr), "s"(lds_byte_addr)
+                 : "v"(addr), "s"(uniform((int32_t)lds_byte_addr))
                  : "memory", "m0");
 }
 
@@ -175,6 +196,67 @@ struct ValueScale {
     }
 };
 
+// 16 bytes of LDS
+template <class V>
+__device__ __forceinline__ V lds_read(uint32_t at) {
+    return *reinterpret_cast<const __attribute__((address_space(3))) V*>(at);
+}
+__device__ __forceinline__ h4 lds_read_tr16(uint32_t at) {
+    typedef __attribute__((address_space(3))) fp16x4_raw lds_h4;
+    return __builtin_bit_cast(h4, __builtin_amdgcn_ds_read_tr16_b64_v4f16(
+                                      (lds_h4*)reinterpret_cast<const __attribute__((address_space(3))) char*>(at)));
+}
+
+// max of three, and of s[0 .. 16 N - 1]: the instruction itself, since fmaxf gets a
+// canonicalising instruction in front for every operand that may be a NaN.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
+template <int N>
+__device__ __forceinline__ float scores_max(const f16x (&s)[N]) {
+    float m[4]; // independent chains
+#pragma unroll
+    for (int c = 0; c < 4; c++) {
+        m[c] = max3(s[0][c], s[0][4 + c], s[0][8 + c]);
+    }
+#pragma unroll
+    for (int c = 0; c < 4; c++) {
+        if constexpr (N == 1) {
+            m[c] = max3(m[c], s[0][12 + c], s[0][12 + c]);
+        } else {
+            m[c] = max3(m[c], s[0][12 + c], s[1][c]);
+        }
+    }
+    if constexpr (N == 2) {
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+            m[c] = max3(m[c], s[1][4 + c], s[1][8 + c]);
+        }
+        m[0] = max3(m[0], s[1][12], s[1][13]);
+        m[1] = max3(m[1], s[1][14], s[1][15]);
+    }
+    return pair_max(max3(max3(m[0], m[1], m[2]), m[3], m[3]));
+}
+
+// acc + the sum of the eight weights of v
+template <class T>
+__device__ __forceinline__ float sum8(typename PagedVec<T>::v8 v, float acc) {
+    typedef T v2 __attribute__((ext_vector_type(2)));
+    const v2 one = {(T)1.0f, (T)1.0f};
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
+        const v2 pr = {v[e], v[e + 1]};
+        if constexpr (__is_same(T, _Float16)) {
+            acc = __builtin_amdgcn_fdot2(pr, one, acc, false);
+        } else {
+            acc = __builtin_amdgcn_fdot2_f32_bf16(pr, one, acc, false);
+        }
+    }
+    return acc;
+}
+
 // use(j, op(j)) for j < N, op (an LDS read of an MFMA operand) DEPTH ahead of use.
 // Left to itself the compiler reads each operand as it is needed and waits for it.
 template <int N, int DEPTH, class Op, class Use>
@@ -201,49 +283,65 @@ __device__ __forceinline__ int32_t by_xcd(int32_t id, int32_t n) {
     return (n & 7) == 0 ? (id & 7) * (n >> 3) + (id >> 3) : id;
 }
 
-__device__ __forceinline__ int32_t uniform(int32_t x) {
-    return __builtin_amdgcn_readfirstlane(x);
-}
 
 // A worker's (a workgroup's, or a wave's) walk over its units, the same in every wave
-// of it.
-template <int ROWS, int BN>
+// of it.  Sequences are counted one to a lane, and the row tiles of a longer one (MANY:
+// there may be some) one to a lane again: one lane's count of the 64 row tiles of a
+// prompt, three times over, had taken 18 us.  An item costs its units and EXTRA (the time before
+// its first and after its last key tile, in key tiles), and the shares are of equal cost:
+// a worker with the many short row tiles at a prompt's begin has fewer key tiles.
+template <int ROWS, int BN, bool MANY, int EXTRA>
 struct PagedWalk {
     const PagedWork& w;
     int32_t wg;
-    int32_t left = 0;  // units of the share not yet taken
-    int32_t at = 0;    // unit of the item to begin with
-    int32_t start = 0; // call-wide number of that unit
+    int32_t left = 0;  // cost of the share not yet taken
+    int32_t at = 0;    // of the item's cost, what earlier shares have
+    int32_t start = 0; // of the call's cost, what lies before
     int32_t share = 1;
     int32_t b = 0, h = 0, rt = 0, n_rt = 0;
     PagedSeq seq;
     PagedTile tile;
 
-    __device__ __forceinline__ PagedWalk(const PagedWork& work, int32_t worker) : w(work), wg(worker) {
+    __device__ __forceinline__ PagedWalk(const PagedWork& work, int32_t worker) : w(work), wg(uniform(worker)) {
         const int lane = threadIdx.x & 63;
         const int32_t B = w.seqs.B;
-        auto units_of = [&](int32_t i) {
-            return i < B ? paged_head_units<ROWS, BN>(w, paged_seq(w.seqs, i)) * w.Hkv : 0;
+        auto cost_of = [&](int32_t i) {
+            const PagedSeq s = i < B ? paged_seq(w.seqs, i) : PagedSeq{0, 0, 0};
+            const int32_t n = paged_row_tiles<ROWS>(w, s.n);
+            int32_t u = 0;
+            if (!MANY || n <= kFewTiles) {
+                u = paged_head_units<ROWS, BN>(w, s) + n * EXTRA;
+            }
+            if constexpr (MANY) {
+                for (uint64_t more = __builtin_amdgcn_ballot_w64(n > kFewTiles); more != 0; more &= more - 1) {
+                    const int l = __builtin_ctzll(more);
+                    const int32_t of = head_cost(PagedSeq{0, __builtin_amdgcn_readlane(s.n, l),
+                                                           __builtin_amdgcn_readlane(s.len, l)});
+                    u = lane == l ? of : u;
+                }
+            }
+            return u * w.Hkv;
         };
-        // units of all sequences; of the first 64 (often all) the sums stay
-        const int32_t mine = units_of(lane);
+        // costs of all sequences; of the first 64 (often all) the sums stay
+        const int32_t mine = cost_of(lane);
         const int32_t sum = wave_prefix(mine);
         int32_t total = __builtin_amdgcn_readlane(sum, 63);
         for (int32_t i = 64; i < B; i += 64) {
-            total += __builtin_amdgcn_readlane(wave_prefix(units_of(i + lane)), 63);
+            total += __builtin_amdgcn_readlane(wave_prefix(cost_of(i + lane)), 63);
         }
-        share = paged_share(w, total);
+        share = uniform(paged_share(w, total));
         start = (int32_t)((int64_t)wg * share < total ? wg * share : total);
-        left = mask_imin(share, total - start);
+        start = uniform(start);
+        left = uniform(mask_imin(share, total - start));
         if (left <= 0) {
             left = 0;
             return;
         }
-        // the sequence that unit `start` is in
+        // the sequence that `start` is in
         int32_t before = 0, m = mine, s = sum;
         for (int32_t i = 0; i < B; i += 64) {
             if (i > 0) {
-                m = units_of(i + lane);
+                m = cost_of(i + lane);
                 s = wave_prefix(m);
             }
             const uint64_t past = __builtin_amdgcn_ballot_w64(before + s > start);
@@ -258,20 +356,48 @@ struct PagedWalk {
         b = uniform(b);
         at = start - uniform(before);
         load_seq();
-        const int32_t per_head = uniform(paged_head_units<ROWS, BN>(w, seq));
+        const int32_t per_head = MANY ? head_cost(seq) : uniform(paged_head_units<ROWS, BN>(w, seq) + n_rt * EXTRA);
         if (per_head == 0) {
             left = 0;
             return;
         }
-        h = mask_imin(at / per_head, w.Hkv - 1);
+        h = uniform(mask_imin(at / per_head, w.Hkv - 1));
         at -= h * per_head;
         rt = 0;
-        load_tile();
-        while (at >= tile.units && rt + 1 < n_rt) {
-            at -= tile.units;
-            rt++;
-            load_tile();
+        if constexpr (MANY) {
+            // the row tile that `at` of the head is in
+            for (int32_t first = 0; first < n_rt; first += 64) {
+                const int32_t u = tile_cost(seq, n_rt, first + lane);
+                const int32_t sum = wave_prefix(u);
+                const uint64_t past = __builtin_amdgcn_ballot_w64(sum > at);
+                if (past != 0) {
+                    const int l = __builtin_ctzll(past);
+                    rt = first + l;
+                    at -= __builtin_amdgcn_readlane(sum, l) - __builtin_amdgcn_readlane(u, l);
+                    break;
+                }
+                at -= __builtin_amdgcn_readlane(sum, 63);
+            }
+            rt = uniform(rt);
+            at = uniform(at);
         }
+        load_tile();
+    }
+
+    static constexpr int32_t kFewTiles = 2;
+
+    // Cost of row tile i of n.
+    __device__ __forceinline__ int32_t tile_cost(const PagedSeq& s, int32_t n, int32_t i) const {
+        return i < n ? paged_tile<ROWS, BN>(w, s, i).units + EXTRA : 0;
+    }
+    // Cost of one kv head of a sequence that is the same in every lane.
+    __device__ __forceinline__ int32_t head_cost(const PagedSeq& s) const {
+        const int32_t n = paged_row_tiles<ROWS>(w, s.n);
+        int32_t u = 0;
+        for (int32_t first = 0; first < n; first += 64) {
+            u += tile_cost(s, n, first + (int)(threadIdx.x & 63));
+        }
+        return __builtin_amdgcn_readlane(wave_prefix(u), 63);
     }
 
     // Sums of x over this lane and those below it: within rows of 16 lanes by shifts,
@@ -292,34 +418,48 @@ struct PagedWalk {
         seq.q0 = uniform(seq.q0);
         seq.n = uniform(seq.n);
         seq.len = uniform(seq.len);
-        n_rt = paged_row_tiles<ROWS>(w, seq.n);
+        n_rt = uniform(paged_row_tiles<ROWS>(w, seq.n));
     }
     __device__ __forceinline__ void load_tile() {
         tile = paged_tile<ROWS, BN>(w, seq, rt);
+        tile.lo = uniform(tile.lo);
+        tile.hi = uniform(tile.hi);
+        tile.first = uniform(tile.first);
+        tile.units = uniform(tile.units);
+        if (at + left <= EXTRA) {
+            left = 0; // none of the item's units
+        }
     }
 
     // Every loop here ends by itself, whatever the lengths hold (a caller may, by
     // mistake, be changing them).
-    // The part of the current item that this share has: units [at, at + count()).
+    // The part of the current item that this share has: units [begin(), begin() +
+    // count()).
     __device__ __forceinline__ bool more() const {
         return left > 0;
     }
+    __device__ __forceinline__ int32_t begin() const {
+        return mask_imax(at - EXTRA, 0);
+    }
     __device__ __forceinline__ int32_t count() const {
-        return mask_imin(left, tile.units - at);
+        return at + cost() - EXTRA - begin();
     }
     __device__ __forceinline__ bool whole() const {
-        return at == 0 && left >= tile.units;
+        return begin() == 0 && at + cost() == tile.units + EXTRA;
     }
     // Slot of a part that is not the whole item, and, of the first part, the last
     // workgroup.
     __device__ __forceinline__ int32_t slot() const {
-        return at == 0 ? w.n_wg + wg : wg;
+        return begin() == 0 ? w.n_wg + wg : wg;
     }
     __device__ __forceinline__ int32_t last_wg() const {
-        return (start + tile.units - 1) / share;
+        return (start - at + tile.units + EXTRA - 1) / share;
+    }
+    __device__ __forceinline__ int32_t cost() const {
+        return mask_imin(left, tile.units + EXTRA - at);
     }
     __device__ __forceinline__ void next() {
-        const int32_t n = count();
+        const int32_t n = cost();
         left -= n;
         start += n;
         at = 0;

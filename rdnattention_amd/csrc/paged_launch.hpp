@@ -33,21 +33,21 @@ inline int paged_workgroups(int64_t resident, int per_group, int64_t units, int 
     return (int)n;
 }
 
-// Units of a call at most.
-template <int ROWS, int BN>
+// Cost of a call at most (see PagedWalk).
+template <int ROWS, int BN, int EXTRA>
 int64_t paged_max_units(const PagedWork& w) {
     const int64_t tiles = (int64_t)w.seqs.total * w.G / ROWS + w.seqs.B;
-    return tiles * w.Hkv * (w.seqs.max_keys / BN + 1);
+    return tiles * w.Hkv * (w.seqs.max_keys / BN + 1 + EXTRA);
 }
 
 constexpr size_t paged_scratch_bytes(int n_wg, int rows, int D) {
     return (size_t)n_wg * (2 * (size_t)rows * (D + 2) * sizeof(float) + sizeof(PagedRecord));
 }
 
-template <int ROWS, int BN, class Go>
+template <int ROWS, int BN, int EXTRA, class Go>
 int paged_launch(const PagedAttnArgs& a, const void* kernel, int threads, int per_group, int min_units, PagedAttnParams& p,
                  const PagedLaunch& l, hipStream_t stream, std::string& err, Go&& go) {
-    const int64_t units = paged_max_units<ROWS, BN>(p.work);
+    const int64_t units = paged_max_units<ROWS, BN, EXTRA>(p.work);
     if (units > INT32_MAX) {
         err = "the call has too many rows and page table entries (" + std::to_string(units) + " key tiles at most)";
         return -1;

@@ -101,7 +101,7 @@ __global__ __launch_bounds__((StreamCfg<D, I8, WV>::THREADS), (StreamCfg<D, I8, 
     // read faster.  (us, neighbours on one XCD / spread: int8 32 x 8192 keys of 8 heads
     // 117 / 124, 32 ragged ones 143 / 154; fp16 16 x 18432 of 8 heads, D = 128 204 / 197,
     // D = 64 124 / 118, 8 x 16384 of 16 heads 182 / 173, ragged 193 / 193.)
-    PagedWalk<kRows, kTile> walk(p.work, I8 ? by_xcd(blockIdx.x, p.work.n_wg) : (int32_t)blockIdx.x);
+    PagedWalk<kRows, kTile, false, 0> walk(p.work, I8 ? by_xcd(blockIdx.x, p.work.n_wg) : (int32_t)blockIdx.x);
 
     // lane i of copy j writes LDS bytes 1024 j + 16 i of the tile: stored chunk n %
     // KCH of row n / KCH, n = 64 j + i, which holds chunk (n % KCH) ^ swz(row)
@@ -118,9 +118,9 @@ __global__ __launch_bounds__((StreamCfg<D, I8, WV>::THREADS), (StreamCfg<D, I8, 
         const PagedSeq seq = walk.seq;
         const PagedTile item = walk.tile;
         const bool whole = walk.whole();
-        const int h = walk.h;
+        const int h = uniform(walk.h);
         const int G = p.work.G;
-        const int r0 = walk.rt * kRows;
+        const int r0 = uniform(walk.rt) * kRows;
         const int n_rows = min(kRows, seq.n * G - r0);
 
         // column l32 <-> row r0 + l32: token (r0 + l32) / G, head h G + (r0 + l32) % G
@@ -141,8 +141,8 @@ __global__ __launch_bounds__((StreamCfg<D, I8, WV>::THREADS), (StreamCfg<D, I8, 
             tree_row = p.tree + walk.b * p.tree_sb + (tok < p.tree_n ? tok : 0) * p.tree_sr;
         }
 
-        const int t0 = item.first + walk.at;
-        const int nt = item.hi >= item.lo ? walk.count() : 0;
+        const int t0 = uniform(item.first + walk.begin());
+        const int nt = uniform(item.hi >= item.lo ? walk.count() : 0);
         const int my_tiles = nt > wave ? (nt - wave + C::WAVES - 1) / C::WAVES : 0;
         auto tile_key = [&](int j) { return (t0 + wave + C::WAVES * j) * kTile; };
         const char* const kbase = p.c.k + h * p.c.k_sh;
@@ -163,7 +163,7 @@ __global__ __launch_bounds__((StreamCfg<D, I8, WV>::THREADS), (StreamCfg<D, I8, 
         auto issue_tab = [&](int batch) {
             const int t = (batch << log_b) + (lane >> log_n);
             const int key = tile_key(t) + ((lane & ((1 << log_n) - 1)) << p.c.lps);
-            dma_load4(tab_rsrc, (uint32_t)(key >> p.c.lps) * 4u, lds_aux + 256 * (batch & 1));
+            dma_load4(tab_rsrc, (uint32_t)(key >> p.c.lps) * 4u, (uint32_t)uniform((int)lds_aux + 256 * (batch & 1)));
         };
         // The row addresses of tile j, from its entries: lanes 0 - 31 leave K row l32's,
         // the others V row l32's.  One tile ahead, before the S of another is computed,
@@ -419,7 +419,7 @@ __global__ __launch_bounds__((StreamCfg<D, I8, WV>::THREADS), (StreamCfg<D, I8, 
                 }
             }
             const int64_t slot = (int64_t)walk.slot() * p.slot_rows;
-            if (!whole && walk.at == 0) {
+            if (!whole && walk.begin() == 0) {
                 rec = PagedRecord{n_rows, seq.q0, r0, h, walk.last_wg(), {}};
             }
             __syncthreads();
@@ -474,7 +474,7 @@ int paged_stream_attention(const PagedAttnArgs& a, PagedAttnParams& p, const Pag
         constexpr bool I8 = decltype(i8)::value;
         auto go = [&](auto waves) {
             constexpr int WV = decltype(waves)::value;
-            return paged_launch<kRows, kTile>(a, reinterpret_cast<const void*>(&paged_stream<T, D, I8, WV>), 64 * WV, 1,
+            return paged_launch<kRows, kTile, 0>(a, reinterpret_cast<const void*>(&paged_stream<T, D, I8, WV>), 64 * WV, 1,
                                               WV, p, l, stream, err, [&](dim3 grid) {
                                                   hipLaunchKernelGGL((paged_stream<T, D, I8, WV>), grid, dim3(64 * WV),
                                                                      0, stream, p);

@@ -5,38 +5,70 @@
 // Bound by the matrix cores where the rows fill the tiles.  A workgroup's waves
 // hold 32 rows each of one kv head's rows (token after token, the G heads of a
 // token side by side, so a chunk of few tokens fills the tiles too) and share
-// 64-key tiles of K and V in LDS, two slots deep: the next tile's copies are
-// issued as the present one is begun, one barrier per tile.  A row of a tile is
-// found through the page table as in paged_stream.hip, the work dealt in equal
-// shares of key tiles (PagedWalk), which also splits the keys of a call of few
-// row tiles over the chip.
+// 64-key tiles of K and V in LDS.  A row of a tile is found through the page
+// table as in paged_stream.hip, the work dealt in equal shares of key tiles
+// (PagedWalk), which also splits the keys of a call of few row tiles over the chip.
+//
+// Step i of a wave: M(i), O += V(i - 1)^T P(i - 1) and S(i) = K(i) Q^T, one stream
+// of MFMAs; then X(i), the softmax of S(i) to P(i).  Up to D = 128 there are two groups
+// of four waves, A and B, one of each on every SIMD, half a step apart, so that one
+// feeds the matrix core while the other runs its softmax, barrier to barrier:
+//
+//   phase     0    1    2    3    4   ...
+//   group A  M(0) X(0) M(1) X(1) M(2)
+//   group B   -   M(0) X(0) M(1) X(1)
+//
+// K(i) and V(i - 1) are read in phases 2i and 2i + 1 and have two slots each.  A copies
+// the values, V(i) in its X(i) (phase 2i + 1; V(i - 2) was last read in 2i - 1), and
+// awaits them at that phase's end.  B copies the keys, K(i + 2) in its X(i) (2i + 2;
+// K(i) was last read in 2i + 1), and awaits them at the end of its M(i + 1).  Above
+// D = 128, where one wave fills a SIMD, a step is one phase of four waves.
+//
+// Q goes through LDS too (up to D = 128, where there is room), in whole lines: loaded
+// straight into the MFMA layout every line was fetched several times over, 4 us of an
+// item's time.  The next item's Q and first table entries are copied during an item.
 #include "paged_launch.hpp"
 
 namespace rdna_amd {
 namespace {
 
 constexpr int kBN = 64;
+constexpr int kItemCost = 5; // key tiles that an item's begin and end take the time of: 8 us of 1.9 us each
 constexpr float kRescale = 8.0f;
+
+// for lambdas that are called more than once: called, they would keep what they
+// capture in memory
+#define RDNA_INLINE __attribute__((always_inline))
 
 template <int D, bool I8>
 struct TileCfg {
     // eight waves; above D = 128 four, one per SIMD, whose O takes up to 128 registers
-    static constexpr int WAVES = D <= 128 ? 8 : 4;
+    static constexpr bool PAIR = D <= 128;
+    static constexpr int WAVES = PAIR ? 8 : 4;
     static constexpr int THREADS = 64 * WAVES;
-    static constexpr int WAVES_PER_SIMD = D <= 32 ? 4 : (D <= 128 ? 2 : 1);
+    static constexpr int WAVES_PER_SIMD = PAIR ? 2 : 1;
     static constexpr int ROWS = 32 * WAVES;
+    static constexpr bool KEEP = PAIR && !I8; // operand addresses in registers
+    static constexpr bool Q_LDS = PAIR;
+    static constexpr int DEPTH = D <= 224 ? 4 : 3; // MFMA operands in flight
     static constexpr int RB = 2 * D;
     static constexpr int KCH = D / 8;
     static constexpr int TILE_BYTES = kBN * RB;
-    // the waves' table entries; of int8 the scales of two slots' keys and values
-    static constexpr int TAB_BYTES = I8 ? 2 * 2 * kBN * 4 : WAVES * 256;
+    // four batches of 64 table entries per wave, of this item and the next; of int8 the
+    // key and value scales of four tiles
+    static constexpr int TAB_BYTES = I8 ? 4 * 2 * kBN * 4 : WAVES * 2048;
+    static constexpr int Q_BYTES = 32 * RB; // of a wave
+    static constexpr int LDS_BYTES = 4 * TILE_BYTES + TAB_BYTES + (Q_LDS ? WAVES * Q_BYTES : 0);
     static constexpr int NS = D / 16;
     static constexpr int NDT = D / 32;
-    static constexpr int DMA = TILE_BYTES / 1024;                  // 1 KB copies of a tile
-    static constexpr int PER = (DMA + WAVES - 1) / WAVES;          // of a wave
-    static constexpr int CHUNKS = kBN * D / 16;                    // 16-byte chunks of an int8 tile
-    static constexpr int NCH = (CHUNKS + THREADS - 1) / THREADS;   // per thread
-    static_assert(4 * TILE_BYTES + TAB_BYTES <= 160 * 1024, "tiles fit the LDS");
+    // the swizzle moves chunks within groups of SWZ: operand addresses repeat, SWZ / 2
+    // steps of s and SWZ / 4 of dt further, 16 SWZ bytes on
+    static constexpr int SWZ = D % 64 == 32 ? 4 : (D % 128 == 64 ? 8 : 16);
+    static constexpr int KA = SWZ / 2 < NS ? SWZ / 2 : NS;
+    static constexpr int VA = SWZ / 4 < NDT ? SWZ / 4 : NDT;
+    static constexpr int PER = TILE_BYTES / 4096;  // 1 KB copies of a tile, of each of the four waves that have it
+    static constexpr int NCH = D < 64 ? 1 : D / 64; // int8: 16-byte chunks of a tile, of each of their threads
+    static_assert(LDS_BYTES <= 160 * 1024, "tiles fit the LDS");
 };
 
 template <class T, int D, bool I8>
@@ -47,40 +79,123 @@ __global__ __launch_bounds__((TileCfg<D, I8>::THREADS), (TileCfg<D, I8>::WAVES_P
     using V4 = typename PagedVec<T>::v4;
     using P = std::conditional_t<I8, _Float16, T>; // weights and values, see paged_stream
     using P8 = typename PagedVec<P>::v8;
-    // K and V of slot 0, of slot 1; the waves' table entries
-    __shared__ __attribute__((aligned(16))) char dsm[4 * C::TILE_BYTES + C::TAB_BYTES];
+    // the K slots, the V slots, the waves' table entries (int8: the scales), the waves' Q
+    __shared__ __attribute__((aligned(16))) char dsm[C::LDS_BYTES];
 
     const int tid = threadIdx.x;
     const int wave = uniform(tid >> 6);
     const int lane = tid & 63;
     const int l32 = lane & 31;
     const int g = lane >> 5;
+    const bool second = C::PAIR && wave >= 4; // group B
+    constexpr int V_SLOTS = 2 * C::TILE_BYTES;
     const uint32_t lds0 = (uint32_t)reinterpret_cast<uintptr_t>(dsm);
-    const uint32_t* const tab = reinterpret_cast<const uint32_t*>(dsm + 4 * C::TILE_BYTES) + 64 * wave;
-    const uint32_t lds_tab = lds0 + 4 * C::TILE_BYTES + 256 * wave;
+    constexpr int TABS = 2 * V_SLOTS;
+    constexpr int QS = TABS + C::TAB_BYTES;
     const uint32_t page_mask = (1u << p.c.lps) - 1u;
+
+    // LDS addresses of the MFMA operands in slot 0: K by s (+ 32 rows: kt), V by (dt, hh)
+    // (+ 16 rows: u; the swizzle has a period of 16 rows).  Where registers are short they are
+    // made for every tile, from an opaque copy of the lane so that they are not kept.
+    auto addresses = [&](int ln, uint32_t (&ka)[C::KA], uint32_t (&va)[2 * C::VA]) RDNA_INLINE {
+        const int row = ln & 31, j16 = ln & 15;
+#pragma unroll
+        for (int s = 0; s < C::KA; s++) {
+            ka[s] = lds0 + row * C::RB + (((2 * s + (ln >> 5)) ^ paged_swz<D>(row)) << 4);
+        }
+#pragma unroll
+        for (int x = 0; x < 2 * C::VA; x++) {
+            const int r = 8 * (x & 1) + 4 * (ln >> 5) + (j16 >> 2);
+            const int d = 32 * (x >> 1) + 16 * ((ln >> 4) & 1) + 4 * (j16 & 3);
+            va[x] = lds0 + V_SLOTS + r * C::RB + (((d >> 3) ^ paged_swz<D>(r)) << 4) + ((d & 7) << 1);
+        }
+    };
+    uint32_t ka0[C::KA], va0[2 * C::VA];
+    if constexpr (C::KEEP) {
+        addresses(lane, ka0, va0);
+    }
 
     if (p.zero_tail != 0) {
         zero_tail_rows<D>(p);
     }
     PagedRecord rec = {};
     // row tiles of one head, which read the same keys, through one L2
-    PagedWalk<C::ROWS, kBN> walk(p.work, by_xcd(blockIdx.x, p.work.n_wg));
+    PagedWalk<C::ROWS, kBN, true, kItemCost> walk(p.work, by_xcd(blockIdx.x, p.work.n_wg));
 
+    const int log_n = max(0, 6 - p.c.lps); // table entries of a tile
+    const int log_b = 6 - log_n;           // tiles of a batch of 64
+    auto tab_rsrc = [&](int b) RDNA_INLINE {
+        i32x4_t r = make_rsrc_v(p.c.table + b * p.c.table_s, (uint32_t)p.c.width * 4u);
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            r[e] = uniform(r[e]);
+        }
+        return r;
+    };
+    // entries of a batch of the item in half `odd` of the wave's, from key tile t0 on
+    auto issue_tab = [&](i32x4_t rsrc, int odd, int t0, int batch) RDNA_INLINE {
+        const int t = (batch << log_b) + (lane >> log_n);
+        const int key = (t0 + t) * kBN + ((lane & ((1 << log_n) - 1)) << p.c.lps);
+        dma_load4(rsrc, (uint32_t)(key >> p.c.lps) * 4u,
+                  (uint32_t)uniform((int)lds0 + TABS + 2048 * wave + 1024 * odd + 256 * (batch & 3)));
+    };
+    // An item's row `col` of the wave's rows, the first one for those behind the last.
+    auto token_head = [&](const auto& w, int& tok, int& head) RDNA_INLINE {
+        const int r0 = uniform(w.rt) * C::ROWS, col = 32 * wave + l32;
+        const bool valid = r0 + col < w.seq.n * p.work.G;
+        const int r = valid ? r0 + col : r0;
+        tok = r / p.work.G;
+        head = uniform(w.h) * p.work.G + r - tok * p.work.G;
+        return valid;
+    };
+    auto q_row = [&](const auto& w, int tok, int head) RDNA_INLINE {
+        return p.q + (int64_t)(w.seq.q0 + tok) * p.q_st + head * p.q_sh;
+    };
+    // What an item needs first: Q (copy n's byte 16 lane is chunk 64 n + lane of the
+    // wave's 32 rows; the lane of row r has its address) and two batches of entries.
+    auto prefetch = [&](const auto& w, int odd) RDNA_INLINE {
+        if constexpr (!I8) {
+            const i32x4_t rsrc = tab_rsrc(w.b);
+            const int t0 = uniform(w.tile.first + w.begin());
+            issue_tab(rsrc, odd, t0, 0);
+            issue_tab(rsrc, odd, t0, 1);
+        }
+        if constexpr (C::Q_LDS) {
+            int tok, head;
+            token_head(w, tok, head);
+            const uint64_t mine = reinterpret_cast<uint64_t>(q_row(w, tok, head));
+            const uint32_t lo = (uint32_t)mine, hi = (uint32_t)(mine >> 32);
+            int ln = lane;
+            asm volatile("" : "+v"(ln));
+#pragma unroll
+            for (int n = 0; n < C::NS; n++) {
+                const int c = 64 * n + ln;
+                const int r = c / C::KCH;
+                const uint64_t row = (uint64_t)(uint32_t)__builtin_amdgcn_ds_bpermute(4 * r, (int)hi) << 32 |
+                                     (uint32_t)__builtin_amdgcn_ds_bpermute(4 * r, (int)lo);
+                dma_gather16(row + (uint32_t)((c - r * C::KCH) ^ paged_swz<D>(r)) * 16u,
+                             (uint32_t)uniform((int)lds0 + QS + wave * C::Q_BYTES + 1024 * n));
+            }
+        }
+    };
+
+    int odd = 0;
+    if (walk.more()) {
+        prefetch(walk, odd);
+    }
     while (walk.more()) {
         const PagedSeq seq = walk.seq;
         const PagedTile item = walk.tile;
         const bool whole = walk.whole();
-        const int h = walk.h;
+        const int h = uniform(walk.h);
         const int G = p.work.G;
-        const int r0 = walk.rt * C::ROWS;
+        const int r0 = uniform(walk.rt) * C::ROWS;
         const int n_rows = min(C::ROWS, seq.n * G - r0);
         const int wr0 = 32 * wave; // of the item
         const int col = wr0 + l32;
-        const bool col_valid = col < n_rows;
         const bool active = wr0 < n_rows; // the wave
-        const int tok = col_valid ? (r0 + col) / G : r0 / G;
-        const int head = h * G + (col_valid ? r0 + col - tok * G : 0);
+        int tok, head;
+        const bool col_valid = token_head(walk, tok, head);
         const MaskSpec mask = paged_mask(p.work.mask, seq);
         int row_lo, row_hi;
         row_key_bounds(mask, tok, row_lo, row_hi);
@@ -101,136 +216,175 @@ __global__ __launch_bounds__((TileCfg<D, I8>::THREADS), (TileCfg<D, I8>::WAVES_P
                    : TileClasses{1, 0, 1, 0};
         const int tree_from = p.tree != nullptr ? prefix : INT32_MAX; // keys from here on are under the tree's mask
 
-        const int t0 = item.first + walk.at;
-        const int nt = item.hi >= item.lo ? walk.count() : 0;
+        const int t0 = uniform(item.first + walk.begin());
+        const int nt = uniform(item.hi >= item.lo ? walk.count() : 0);
         const char* const kbase = p.c.k + h * p.c.k_sh;
         const char* const vbase = p.c.v + h * p.c.v_sh;
-        const int32_t* const table = p.c.table + walk.b * p.c.table_s;
+        const uint32_t* const tab = reinterpret_cast<const uint32_t*>(dsm + TABS) + 512 * wave + 256 * odd;
 
-        // ---- 16-bit pages: copy d of a tile writes its LDS bytes 1024 d + 16 lane;
-        // wave w has copies w, w + WAVES, ...
-        i32x4_t tab_rsrc = make_rsrc_v(table, (uint32_t)p.c.width * 4u);
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-            tab_rsrc[e] = uniform(tab_rsrc[e]);
-        }
-        auto issue_tab = [&](int i) {
-            dma_load4(tab_rsrc, (uint32_t)(((t0 + i) * kBN + lane) >> p.c.lps) * 4u, lds_tab);
+        // ---- staging of 16-bit pages.  Copy d of a tile writes its LDS bytes 1024 d + 16
+        // lane; wave w has copies w % 4, w % 4 + 4, ...
+        // Copy d of keys or values (base, page and token strides) of tile t: each lane
+        // finds its row.
+        auto copy = [&](int t, int d, uint32_t lds, const char* base, int64_t sp, int64_t st) RDNA_INLINE {
+            const int key0 = (t0 + t) * kBN;
+            int ln = lane;
+            asm volatile("" : "+v"(ln)); // no constants of every copy in registers
+            const int n = 64 * d + ln;
+            const int r = n / C::KCH;
+            const bool seen = key0 + r >= item.lo && key0 + r <= item.hi;
+            const uint32_t pg = tab[64 * ((t >> log_b) & 3) + ((t & ((1 << log_b) - 1)) << log_n) + (r >> p.c.lps)];
+            const uint64_t pe = pg < (uint32_t)p.c.pages ? pg : 0u;
+            const uint64_t off = (uint32_t)(key0 + r) & page_mask;
+            const uint64_t row = reinterpret_cast<uint64_t>(base) + pe * (uint64_t)sp + off * (uint64_t)st;
+            dma_gather16((seen ? row : reinterpret_cast<uint64_t>(kPagedZeroRow)) +
+                             (uint32_t)((n - r * C::KCH) ^ paged_swz<D>(r)) * 16u,
+                         lds);
         };
-        auto issue_tile = [&](int i) { // its entries have landed
-            const uint32_t slot = lds0 + (uint32_t)(i & 1) * (2 * C::TILE_BYTES);
-            uint64_t ka[C::PER], va[C::PER];
-#pragma unroll
-            for (int c = 0; c < C::PER; c++) {
-                const int d = wave + C::WAVES * c;
-                const int n = 64 * (d < C::DMA ? d : 0) + lane;
-                const int r = n / C::KCH;
-                const uint32_t chunk = (uint32_t)((n - r * C::KCH) ^ paged_swz<D>(r)) * 16u;
-                const int key = (t0 + i) * kBN + r;
-                const bool seen = key >= item.lo && key <= item.hi;
-                const uint32_t pg = tab[r];
-                const uint64_t pe = pg < (uint32_t)p.c.pages ? pg : 0u;
-                const uint64_t off = (uint32_t)key & page_mask;
-                const uint64_t zero = reinterpret_cast<uint64_t>(kPagedZeroRow);
-                ka[c] = (seen ? reinterpret_cast<uint64_t>(kbase) + pe * (uint64_t)p.c.k_sp + off * (uint64_t)p.c.k_st
-                              : zero) + chunk;
-                va[c] = (seen ? reinterpret_cast<uint64_t>(vbase) + pe * (uint64_t)p.c.v_sp + off * (uint64_t)p.c.v_st
-                              : zero) + chunk;
+        // Where each copy's rows lie in one page, and every key of the tile is seen by a row
+        // of the item: lane x finds the first row of copy x, and a copy's address is one
+        // scalar and the lane's constant part.  (Finding them in turn took 20 us of the
+        // 770 of B4 Hq32 Hkv8 S4096 D128 causal.)
+        constexpr int CROWS = 1024 / C::RB;
+        const bool one_page = 1024 % C::RB == 0 && (1 << p.c.lps) >= CROWS && (uint64_t)p.c.k_sp < (1ull << 32) &&
+                              (uint64_t)p.c.v_sp < (1ull << 32) && p.c.k_st < (1 << 26) && p.c.v_st < (1 << 26);
+        auto stage_copies = [&](bool values, int t) RDNA_INLINE {
+            if (t >= nt) {
+                return;
             }
-            __builtin_amdgcn_s_waitcnt(waitcnt_lgkm(0)); // the entries are read
+            if ((C::PAIR || !values) && t > 0 && (t & ((1 << log_b) - 1)) == 0) {
+                issue_tab(tab_rsrc(walk.b), odd, t0, (t >> log_b) + 1); // over entries of three batches ago
+            }
+            const char* const base = values ? vbase : kbase;
+            const int64_t sp = values ? p.c.v_sp : p.c.k_sp;
+            const int64_t st = values ? p.c.v_st : p.c.k_st;
+            const uint32_t slot = lds0 + (values ? V_SLOTS : 0) + (uint32_t)(t & 1) * C::TILE_BYTES;
+            const int key0 = (t0 + t) * kBN;
+            if (one_page && key0 >= item.lo && key0 + kBN - 1 <= item.hi) {
+                int ln = lane;
+                asm volatile("" : "+v"(ln));
+                const int r = CROWS * ((wave & 3) + 4 * ln) & (kBN - 1);
+                const uint32_t pg = tab[64 * ((t >> log_b) & 3) + ((t & ((1 << log_b) - 1)) << log_n) + (r >> p.c.lps)];
+                const uint32_t pe = pg < (uint32_t)p.c.pages ? pg : 0u;
+                const uint32_t off = (uint32_t)(key0 + r) & page_mask;
+                const uint64_t row = reinterpret_cast<uint64_t>(base) + (uint64_t)pe * (uint32_t)sp +
+                                     (uint64_t)off * (uint32_t)st;
+                const int crow = lane / C::KCH;
 #pragma unroll
-            for (int c = 0; c < C::PER; c++) {
-                const int d = wave + C::WAVES * c;
-                if (C::DMA % C::WAVES == 0 || d < C::DMA) {
-                    dma_gather16(ka[c], slot + 1024 * d);
-                    dma_gather16(va[c], slot + C::TILE_BYTES + 1024 * d);
+                for (int x = 0; x < C::PER; x++) {
+                    const int d = (wave & 3) + 4 * x;
+                    dma_uniform16(readlane64(row, x),
+                                  (uint32_t)crow * (uint32_t)st +
+                                      (uint32_t)((lane % C::KCH) ^ paged_swz<D>(CROWS * d + crow)) * 16u,
+                                  slot + 1024 * d);
+                }
+            } else {
+#pragma unroll
+                for (int x = 0; x < C::PER; x++) {
+                    const int d = (wave & 3) + 4 * x;
+                    copy(t, d, slot + 1024 * d, base, sp, st);
                 }
             }
         };
-
-        // ---- int8 pages: through registers, widened exactly (once for all waves); the
-        // scales beside them
+        // int8 pages: through registers, widened exactly (once for all waves); the next
+        // tile's loads leave as this one's are stored.  With the keys go the scales of
+        // keys and values, which X(i) reads.
         constexpr int RCH = D / 16;
-        float* const scales = reinterpret_cast<float*>(dsm + 4 * C::TILE_BYTES); // [slot][keys, values][kBN]
-        auto chunk_row = [&](int c) { return (C::THREADS * c + tid) / RCH % kBN; };
+        float* const scales = reinterpret_cast<float*>(dsm + TABS); // [tile % 4][keys, values][kBN]
+        auto chunk_row = [&](int c) { return (256 * c + (tid & 255)) / RCH; };
         int32_t ent[C::NCH];
-        i4 kraw[C::NCH], vraw[C::NCH];
+        i4 raw[C::NCH];
         float ksc[C::NCH], vsc[C::NCH];
-        auto load_entries = [&](int i) {
+        auto load_entries = [&](int t) RDNA_INLINE {
 #pragma unroll
             for (int c = 0; c < C::NCH; c++) {
-                const int e = ((t0 + i) * kBN + chunk_row(c)) >> p.c.lps;
-                ent[c] = table[min(e, p.c.width - 1)];
+                const int e = ((t0 + t) * kBN + chunk_row(c)) >> p.c.lps;
+                ent[c] = p.c.table[walk.b * p.c.table_s + min(e, p.c.width - 1)];
             }
         };
-        auto load_raw = [&](int i) {
+        auto load_raw = [&](int t) RDNA_INLINE {
+            const char* const base = second ? kbase : vbase;
+            const int64_t sp = second ? p.c.k_sp : p.c.v_sp;
+            const int64_t st = second ? p.c.k_st : p.c.v_st;
 #pragma unroll
             for (int c = 0; c < C::NCH; c++) {
-                const int key = (t0 + i) * kBN + chunk_row(c);
+                const int key = (t0 + t) * kBN + chunk_row(c);
                 const bool seen = key >= item.lo && key <= item.hi;
                 const int64_t pg = (uint32_t)ent[c] < (uint32_t)p.c.pages ? ent[c] : 0;
                 const int64_t off = (uint32_t)key & page_mask;
-                const int ch = 16 * (tid % RCH);
-                kraw[c] = *reinterpret_cast<const i4*>(kbase + pg * p.c.k_sp + off * p.c.k_st + ch);
-                vraw[c] = *reinterpret_cast<const i4*>(vbase + pg * p.c.v_sp + off * p.c.v_st + ch);
-                const float a = p.c.ks[pg * p.c.ks_sp + off * p.c.ks_st + h * p.c.ks_sh];
-                const float b = p.c.vs[pg * p.c.vs_sp + off * p.c.vs_st + h * p.c.vs_sh];
-                ksc[c] = seen ? a : 0.0f;
-                vsc[c] = seen ? b : 0.0f;
+                raw[c] = *reinterpret_cast<const i4*>(base + pg * sp + off * st + 16 * (tid % RCH));
+                if (second) {
+                    const float a = p.c.ks[pg * p.c.ks_sp + off * p.c.ks_st + h * p.c.ks_sh];
+                    const float b = p.c.vs[pg * p.c.vs_sp + off * p.c.vs_st + h * p.c.vs_sh];
+                    ksc[c] = seen ? a : 0.0f;
+                    vsc[c] = seen ? b : 0.0f;
+                }
             }
         };
-        auto store_raw = [&](int i) {
-            char* const sk = dsm + (i & 1) * (2 * C::TILE_BYTES);
+        auto stage_int8 = [&](int t) RDNA_INLINE {
+            int td = tid & 255;
+            asm volatile("" : "+v"(td)); // no addresses kept in registers
 #pragma unroll
             for (int c = 0; c < C::NCH; c++) {
-                const int r = chunk_row(c);
-                const int cl = 2 * (tid % RCH);
-                if (C::CHUNKS % C::THREADS != 0 && C::THREADS * c + tid >= C::CHUNKS) {
-                    continue;
-                }
+                const int r = (256 * c + td) / RCH;
+                const int cl = 2 * (td % RCH);
+                // beyond the last tile the slots are free and hold rows of any page
+                char* const s = dsm + (second ? 0 : V_SLOTS) + (t & 1) * C::TILE_BYTES + r * C::RB;
 #pragma unroll
                 for (int x = 0; x < 2; x++) {
-                    char* const at = sk + r * C::RB + (((cl + x) ^ paged_swz<D>(r)) << 4);
-                    *reinterpret_cast<V8*>(at) = widen_int8<T>(i2v{kraw[c][2 * x], kraw[c][2 * x + 1]});
-                    *reinterpret_cast<P8*>(at + C::TILE_BYTES) = widen_int8<P>(i2v{vraw[c][2 * x], vraw[c][2 * x + 1]});
+                    char* const at = s + (((cl + x) ^ paged_swz<D>(r)) << 4);
+                    const i2v in{raw[c][2 * x], raw[c][2 * x + 1]};
+                    if (second) {
+                        *reinterpret_cast<V8*>(at) = widen_int8<T>(in);
+                    } else {
+                        *reinterpret_cast<P8*>(at) = widen_int8<P>(in);
+                    }
                 }
-                if (cl == 0) {
-                    scales[(i & 1) * 2 * kBN + r] = ksc[c];
-                    scales[(i & 1) * 2 * kBN + kBN + r] = vsc[c];
+                if (second && cl == 0) {
+                    scales[(t & 3) * 2 * kBN + r] = ksc[c];
+                    scales[(t & 3) * 2 * kBN + kBN + r] = vsc[c];
                 }
+            }
+            load_raw(t + 1);
+            load_entries(t + 2);
+        };
+        // keys or values of tile t: with two groups the wave's kind
+        auto stage = [&](bool values, int t) RDNA_INLINE {
+            if constexpr (I8) {
+                stage_int8(t);
+            } else {
+                stage_copies(values, t);
             }
         };
 
+        // ---- prologue: K(0); its Q and entries, on their way since the last item
+        if constexpr (!I8 || C::Q_LDS) {
+            __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
+            asm volatile("" ::: "memory");
+        }
         if (nt > 0) {
             if constexpr (I8) {
                 load_entries(0);
                 load_raw(0);
                 load_entries(1);
-            } else {
-                issue_tab(0);
-                __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
-                issue_tile(0);
-                issue_tab(1);
+            }
+            if (!C::PAIR || second) {
+                stage(false, 0);
             }
         }
         V8 qreg[C::NS];
-        {
-            const char* qrow = p.q + (int64_t)(seq.q0 + tok) * p.q_st + head * p.q_sh + 16 * g;
 #pragma unroll
-            for (int s = 0; s < C::NS; s++) {
-                qreg[s] = *reinterpret_cast<const V8*>(qrow + 32 * s);
-            }
-#pragma unroll
-            for (int s = 0; s < C::NS; s++) {
-                qreg[s] = col_valid ? (p.q_sign < 0.0f ? -qreg[s] : qreg[s]) : V8{};
+        for (int s = 0; s < C::NS; s++) {
+            if constexpr (C::Q_LDS) {
+                qreg[s] = *reinterpret_cast<const V8*>(dsm + QS + wave * C::Q_BYTES + l32 * C::RB +
+                                                       (((2 * s + g) ^ paged_swz<D>(l32)) << 4));
+            } else {
+                qreg[s] = *reinterpret_cast<const V8*>(q_row(walk, tok, head) + 32 * s + 16 * g);
             }
         }
-        if constexpr (I8) {
-            if (nt > 0) {
-                store_raw(0);
-                load_raw(1);
-                load_entries(2);
-            }
+#pragma unroll
+        for (int s = 0; s < C::NS; s++) {
+            qreg[s] = col_valid ? (p.q_sign < 0.0f ? -qreg[s] : qreg[s]) : V8{};
         }
 
         f16x oacc[C::NDT];
@@ -239,125 +393,207 @@ __global__ __launch_bounds__((TileCfg<D, I8>::THREADS), (TileCfg<D, I8>::WAVES_P
             oacc[dt] = f16x{};
         }
         float m_run = -INFINITY, l_run = 0.0f;
+        f16x sacc[2] = {f16x{}, f16x{}};
+        P8 pb[4] = {P8{}, P8{}, P8{}, P8{}};
         ValueScale vscale;
 
-        for (int i = 0; i < nt; i++) {
-            // this wave's copies of tile i (and the entries of i + 1) have landed; behind
-            // the barrier every wave's, and no wave reads tile i - 1 any more
-            __builtin_amdgcn_s_waitcnt(0);
-            __syncthreads();
-            if constexpr (!I8) {
-                if (i + 1 < nt) {
-                    issue_tile(i + 1);
-                    issue_tab(i + 2);
+        // M(i): one stream of MFMAs, operands read ahead; at raised priority, as the
+        // other wave on the SIMD runs its softmax meanwhile.  There are two of it
+        // only, M(0) and the others (M(nt) computes an S of no use, of whatever K's slot
+        // holds): with one for every case O and S take twice the registers.
+        auto mfmas = [&](auto do_pv, int i) RDNA_INLINE {
+            constexpr int NPV = decltype(do_pv)::value ? 4 * C::NDT : 0; // (u, dt)
+            constexpr int NSK = 2 * C::NS;                               // (s, kt)
+            const uint32_t k_slot = (uint32_t)(i & 1) * C::TILE_BYTES;
+            const uint32_t v_slot = (uint32_t)((i + 1) & 1) * C::TILE_BYTES;
+            uint32_t ka[C::KA], va[2 * C::VA];
+            if constexpr (C::KEEP) {
+#pragma unroll
+                for (int x = 0; x < 2 * C::VA; x++) {
+                    va[x] = va0[x];
+                }
+#pragma unroll
+                for (int s = 0; s < C::KA; s++) {
+                    ka[s] = ka0[s];
+                }
+            } else {
+                int ln = lane;
+                asm volatile("" : "+v"(ln));
+                addresses(ln, ka, va);
+            }
+#pragma unroll
+            for (int x = 0; x < 2 * C::VA; x++) {
+                va[x] += v_slot;
+            }
+#pragma unroll
+            for (int s = 0; s < C::KA; s++) {
+                ka[s] += k_slot;
+            }
+            __builtin_amdgcn_s_setprio(1);
+            operand_stream<NPV + NSK, C::DEPTH>(
+                [&](int j) -> h8 {
+                    if (j < NPV) {
+                        const int u = j / C::NDT, dt = j % C::NDT;
+                        const int x = 2 * (dt % C::VA), on = 16 * u * C::RB + dt / C::VA * 16 * C::SWZ;
+                        const h4 lo = lds_read_tr16(va[x] + on);
+                        const h4 hi = lds_read_tr16(va[x + 1] + on);
+                        return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+                    }
+                    const int s = (j - NPV) >> 1, kt = (j - NPV) & 1;
+                    return lds_read<h8>(ka[s % C::KA] + 32 * kt * C::RB + s / C::KA * 16 * C::SWZ);
+                },
+                [&](int j, h8 a) {
+                    if (j < NPV) {
+                        const int u = j / C::NDT, dt = j % C::NDT;
+                        oacc[dt] = paged_mfma<P>(__builtin_bit_cast(P8, a), pb[u], oacc[dt]);
+                    } else {
+                        const int s = (j - NPV) >> 1, kt = (j - NPV) & 1;
+                        sacc[kt] = paged_mfma<T>(__builtin_bit_cast(V8, a), qreg[s], s == 0 ? f16x{} : sacc[kt]);
+                    }
+                });
+            __builtin_amdgcn_s_setprio(0);
+        };
+        auto softmax = [&](int i) RDNA_INLINE {
+            const int kt0 = (t0 + i) * kBN;
+            if constexpr (I8) {
+                const f4* sc = reinterpret_cast<const f4*>(scales + (i & 3) * 2 * kBN) + g;
+#pragma unroll
+                for (int x = 0; x < 8; x++) {
+                    const f4 ks = sc[2 * x];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        sacc[x >> 2][4 * (x & 3) + e] *= ks[e];
+                    }
                 }
             }
-            const char* const sk = dsm + (i & 1) * (2 * C::TILE_BYTES);
-            const char* const sv = sk + C::TILE_BYTES;
-            const int kt0 = (t0 + i) * kBN;
-            const int what = tile_class(cls, t0 + i);
-            if (what != 0) {
-                f16x sacc[2] = {f16x{}, f16x{}};
+            if (tile_class(cls, t0 + i) != 1) { // a tile that the wave's rows do not see: all of it
+                const int a = row_lo - kt0 - 4 * g;
+                const int bnd = row_hi - kt0 - 4 * g;
 #pragma unroll
-                for (int s = 0; s < C::NS; s++) {
-#pragma unroll
-                    for (int kt = 0; kt < 2; kt++) {
-                        const int r = 32 * kt + l32;
-                        const V8 a =
-                            *reinterpret_cast<const V8*>(sk + r * C::RB + (((2 * s + g) ^ paged_swz<D>(r)) << 4));
-                        sacc[kt] = paged_mfma<T>(a, qreg[s], sacc[kt]);
-                    }
+                for (int e = 0; e < 32; e++) {
+                    const int off = 32 * (e >> 4) + 8 * ((e & 15) >> 2) + (e & 3);
+                    sacc[e >> 4][e & 15] = (off < a || off > bnd) ? -INFINITY : sacc[e >> 4][e & 15];
                 }
-                if constexpr (I8) {
-                    const f4* sc = reinterpret_cast<const f4*>(scales + (i & 1) * 2 * kBN) + g;
-#pragma unroll
-                    for (int x = 0; x < 8; x++) {
-                        const f4 ks = sc[2 * x];
-#pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            sacc[x >> 2][4 * (x & 3) + e] *= ks[e];
-                        }
-                    }
+            }
+            if (kt0 + kBN > tree_from) {
+                tree_mask_scores<2>(sacc, tree_row, tree_n, prefix, kt0 + 4 * g);
+            }
+            const float mx = scores_max(sacc);
+            const float m_new = fmaxf(m_run, mx * p.scale_log2e);
+            const bool grow = m_new > m_run + kRescale;
+            if (wave_any(grow)) {
+                const float alpha = grow ? fast_exp2(m_run - m_new) : 1.0f;
+                if (grow) {
+                    m_run = m_new;
                 }
-                if (what == 2) {
-                    const int a = row_lo - kt0 - 4 * g;
-                    const int bnd = row_hi - kt0 - 4 * g;
+                l_run *= alpha;
 #pragma unroll
-                    for (int e = 0; e < 32; e++) {
-                        const int off = 32 * (e >> 4) + 8 * ((e & 15) >> 2) + (e & 3);
-                        sacc[e >> 4][e & 15] = (off < a || off > bnd) ? -INFINITY : sacc[e >> 4][e & 15];
-                    }
+                for (int dt = 0; dt < C::NDT; dt++) {
+                    oacc[dt] *= alpha;
                 }
-                if (kt0 + kBN > tree_from) {
-                    tree_mask_scores<2>(sacc, tree_row, tree_n, prefix, kt0 + 4 * g);
-                }
-                float mx = max_tree<32>([&](int e) { return sacc[e >> 4][e & 15]; });
-                mx = pair_max(mx);
-                const float m_new = fmaxf(m_run, mx * p.scale_log2e);
-                const bool grow = m_new > m_run + kRescale;
-                if (wave_any(grow)) {
-                    const float alpha = grow ? fast_exp2(m_run - m_new) : 1.0f;
-                    if (grow) {
-                        m_run = m_new;
-                    }
-                    l_run *= alpha;
-#pragma unroll
-                    for (int dt = 0; dt < C::NDT; dt++) {
-                        oacc[dt] *= alpha;
-                    }
-                }
-                const float m_use = (m_run == -INFINITY) ? 0.0f : m_run;
+            }
+            const float m_use = (m_run == -INFINITY) ? 0.0f : m_run;
+            float ps[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            if constexpr (I8) {
                 float pv[32];
-                float ps[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                 for (int e = 0; e < 32; e++) {
                     pv[e] = fast_exp2(fmaf(sacc[e >> 4][e & 15], p.scale_log2e, -m_use));
                     ps[e & 3] += pv[e];
                 }
-                l_run += (ps[0] + ps[1]) + (ps[2] + ps[3]);
-                if constexpr (I8) {
-                    const f4* sc = reinterpret_cast<const f4*>(scales + (i & 1) * 2 * kBN + kBN) + g;
-                    f4 vs[8];
+                const f4* sc = reinterpret_cast<const f4*>(scales + (i & 3) * 2 * kBN + kBN) + g;
+                f4 vs[8];
 #pragma unroll
-                    for (int x = 0; x < 8; x++) {
-                        vs[x] = sc[2 * x];
-                    }
-                    vscale.weigh<8>(pv, vs, oacc);
+                for (int x = 0; x < 8; x++) {
+                    vs[x] = sc[2 * x];
                 }
-                P8 pb[4];
+                vscale.weigh<8>(pv, vs, oacc);
 #pragma unroll
                 for (int e = 0; e < 32; e++) {
                     pb[e >> 3][e & 7] = (P)pv[e];
                 }
-                const int j16 = lane & 15;
+            } else {
 #pragma unroll
                 for (int u = 0; u < 4; u++) {
 #pragma unroll
-                    for (int dt = 0; dt < C::NDT; dt++) {
-                        h4 half4[2];
-#pragma unroll
-                        for (int hh = 0; hh < 2; hh++) {
-                            const int r = 16 * u + 8 * hh + 4 * g + (j16 >> 2);
-                            const int d = 32 * dt + 16 * ((lane >> 4) & 1) + 4 * (j16 & 3);
-                            const char* addr =
-                                sv + r * C::RB + (((d >> 3) ^ paged_swz<D>(r)) << 4) + ((d & 7) << 1);
-                            half4[hh] = lds_read_tr16(reinterpret_cast<const _Float16*>(addr));
-                        }
-                        const h8 a = __builtin_shufflevector(half4[0], half4[1], 0, 1, 2, 3, 4, 5, 6, 7);
-                        oacc[dt] = paged_mfma<P>(__builtin_bit_cast(P8, a), pb[u], oacc[dt]);
+                    for (int e = 0; e < 8; e++) {
+                        const int x = 8 * u + e;
+                        pb[u][e] = (P)fast_exp2(fmaf(sacc[x >> 4][x & 15], p.scale_log2e, -m_use));
+                    }
+                    ps[u] = sum8<P>(pb[u], 0.0f); // of the weights as the products take them
+                }
+            }
+            l_run += (ps[0] + ps[1]) + (ps[2] + ps[3]);
+        };
+
+        // Every wave's copies (LDS stores) of the tiles to be read have landed behind a
+        // barrier, and every wave has read what the copies behind it overwrite.
+        using Yes = std::true_type;
+        using No = std::false_type;
+        if (nt > 0) {
+            __builtin_amdgcn_s_waitcnt(0);
+            __syncthreads();
+        }
+        auto ahead = walk;
+        ahead.next();
+        odd ^= 1;
+        if (ahead.more()) {
+            prefetch(ahead, odd);
+        }
+        odd ^= 1;
+        if (nt > 0) {
+            if constexpr (C::PAIR) {
+                // both groups pass 2 nt + 2 barriers from here on
+                if (second) {
+                    stage(false, 1);
+                    __syncthreads();
+                }
+                if (active) {
+                    mfmas(No{}, 0);
+                }
+                for (int i = 0; i < nt; i++) {
+                    if (!I8 && second) {
+                        __builtin_amdgcn_s_waitcnt(waitcnt_vm(0)); // its copies of K(i + 1)
+                    }
+                    __syncthreads();
+                    stage(!second, second ? i + 2 : i);
+                    if (active) {
+                        softmax(i);
+                    }
+                    if (!I8 && !second) {
+                        __builtin_amdgcn_s_waitcnt(waitcnt_vm(0)); // its copies of V(i)
+                    }
+                    __syncthreads();
+                    if (active) {
+                        mfmas(Yes{}, i + 1);
                     }
                 }
-            }
-            if constexpr (I8) {
-                if (i + 1 < nt) {
-                    store_raw(i + 1); // its slot was last read before this tile's barrier
-                    load_raw(i + 2);
-                    load_entries(i + 3);
+                __syncthreads();
+                if (!second) {
+                    __syncthreads();
                 }
+            } else {
+                stage(false, 1);
+                stage(true, 0);
+                if (active) {
+                    mfmas(No{}, 0);
+                }
+                for (int i = 0; i < nt; i++) {
+                    if (active) {
+                        softmax(i);
+                    }
+                    __builtin_amdgcn_s_waitcnt(0); // its copies of K(i + 1), V(i)
+                    __syncthreads();
+                    stage(false, i + 2);
+                    stage(true, i + 1);
+                    if (active) {
+                        mfmas(Yes{}, i + 1);
+                    }
+                }
+                __builtin_amdgcn_s_waitcnt(0);
+                __syncthreads(); // the next item's copies overwrite the slots
             }
         }
-        __builtin_amdgcn_s_waitcnt(0);
-        __syncthreads(); // the next item's copies overwrite the slots
 
         const float l_tot = pair_sum(l_run);
         const float unit = I8 ? vscale.factor() : 1.0f; // of O
@@ -381,11 +617,12 @@ __global__ __launch_bounds__((TileCfg<D, I8>::THREADS), (TileCfg<D, I8>::WAVES_P
                 store_partial<C::NDT>(oacc, m_run, l_tot, g == 0, p.part_o, p.part_ml, slot * p.slot_rows + col, D, 0, g,
                                       [&](int) { return f4{unit, unit, unit, unit}; });
             }
-            if (walk.at == 0) {
+            if (walk.begin() == 0) {
                 rec = PagedRecord{n_rows, seq.q0, r0, h, walk.last_wg(), {}};
             }
         }
         walk.next();
+        odd ^= 1;
     }
     if (tid == 0) {
         p.records[walk.wg] = rec;
@@ -394,7 +631,7 @@ __global__ __launch_bounds__((TileCfg<D, I8>::THREADS), (TileCfg<D, I8>::WAVES_P
 
 } // namespace
 
-// Smallest share: four key tiles.
+// Workers are workgroups; smallest share: four key tiles.
 int paged_tile_attention(const PagedAttnArgs& a, PagedAttnParams& p, const PagedLaunch& l, hipStream_t stream,
                          std::string& err) {
     return paged_for_type(a, [&](auto t, auto d, auto i8) {
@@ -402,7 +639,7 @@ int paged_tile_attention(const PagedAttnArgs& a, PagedAttnParams& p, const Paged
         constexpr int D = decltype(d)::value;
         constexpr bool I8 = decltype(i8)::value;
         using C = TileCfg<D, I8>;
-        return paged_launch<C::ROWS, kBN>(a, reinterpret_cast<const void*>(&paged_tiles<T, D, I8>), C::THREADS, 1, 4, p, l,
+        return paged_launch<C::ROWS, kBN, kItemCost>(a, reinterpret_cast<const void*>(&paged_tiles<T, D, I8>), C::THREADS, 1, 4, p, l,
                                           stream, err, [&](dim3 grid) {
                                               hipLaunchKernelGGL((paged_tiles<T, D, I8>), grid, dim3(C::THREADS), 0,
                                                                  stream, p);

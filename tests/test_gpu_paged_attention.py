@@ -119,6 +119,23 @@ def test_many_sequences(gpu):
     run(gpu, pool, ns, 4, name="200 sequences, chunks among them")
 
 
+@pytest.mark.parametrize("dtype,i8,d", [(F16, False, 128), (BF16, False, 96), (F16, False, 32), (BF16, False, 160),
+                                        (F16, True, 128), (BF16, True, 64)])
+@pytest.mark.parametrize("window", [-1, 40])
+def test_many_row_tiles_per_worker(gpu, dtype, i8, d, window):
+    lens = [1 + (37 * b) % 131 for b in range(150)]
+    pool = Pool(lens, 8, d, 16, dtype, i8, seed=d)
+    run(gpu, pool, lens, 32, window=window, name=f"many prompts {dtype} {i8} {d} {window}")
+
+
+@pytest.mark.parametrize("causal", [True, False])
+def test_more_row_tiles_than_lanes(gpu, causal):
+    lens = [30, 1150, 700]
+    pool = Pool(lens, 1, 32, 64, F16, seed=5)
+    run(gpu, pool, [1, 1150, 300], 16, causal=causal, name=f"long prompt {causal}")
+    run(gpu, pool, [30, 1150, 700], 16, causal=causal, window=90, name=f"long prompt, window {causal}")
+
+
 @pytest.mark.parametrize("dtype,i8,d", [(F16, False, 128), (BF16, False, 96), (F16, True, 128)])
 def test_many_heads(gpu, dtype, i8, d):
     """512 kv heads and more of all sequences: workgroups of four waves, most of
