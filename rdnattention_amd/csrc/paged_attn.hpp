@@ -305,8 +305,9 @@ struct PagedWalk {
     __device__ __forceinline__ PagedWalk(const PagedWork& work, int32_t worker) : w(work), wg(uniform(worker)) {
         const int lane = threadIdx.x & 63;
         const int32_t B = w.seqs.B;
-        auto cost_of = [&](int32_t i) {
-            const PagedSeq s = i < B ? paged_seq(w.seqs, i) : PagedSeq{0, 0, 0};
+        // sequence i and what one kv head of it costs
+        auto cost_of = [&](int32_t i, PagedSeq& s) {
+            s = i < B ? paged_seq(w.seqs, i) : PagedSeq{0, 0, 0};
             const int32_t n = paged_row_tiles<ROWS>(w, s.n);
             int32_t u = 0;
             if (!MANY || n <= kFewTiles) {
@@ -316,18 +317,20 @@ struct PagedWalk {
                 for (uint64_t more = __builtin_amdgcn_ballot_w64(n > kFewTiles); more != 0; more &= more - 1) {
                     const int l = __builtin_ctzll(more);
                     const int32_t of = head_cost(PagedSeq{0, __builtin_amdgcn_readlane(s.n, l),
-                                                           __builtin_amdgcn_readlane(s.len, l)});
+                                                          __builtin_amdgcn_readlane(s.len, l)});
                     u = lane == l ? of : u;
                 }
             }
-            return u * w.Hkv;
+            return u;
         };
-        // costs of all sequences; of the first 64 (often all) the sums stay
-        const int32_t mine = cost_of(lane);
-        const int32_t sum = wave_prefix(mine);
+        // of the first 64 sequences (often all) the sums stay
+        PagedSeq s0;
+        const int32_t mine = cost_of(lane, s0);
+        const int32_t sum = wave_prefix(mine * w.Hkv);
         int32_t total = __builtin_amdgcn_readlane(sum, 63);
         for (int32_t i = 64; i < B; i += 64) {
-            total += __builtin_amdgcn_readlane(wave_prefix(cost_of(i + lane)), 63);
+            PagedSeq s;
+            total += __builtin_amdgcn_readlane(wave_prefix(cost_of(i + lane, s) * w.Hkv), 63);
         }
         share = uniform(paged_share(w, total));
         start = (int32_t)((int64_t)wg * share < total ? wg * share : total);
@@ -338,29 +341,34 @@ struct PagedWalk {
             return;
         }
         // the sequence that `start` is in
-        int32_t before = 0, m = mine, s = sum;
+        int32_t before = 0, per_head = 0;
         for (int32_t i = 0; i < B; i += 64) {
+            PagedSeq s = s0;
+            int32_t m = mine, sums = sum;
             if (i > 0) {
-                m = cost_of(i + lane);
-                s = wave_prefix(m);
+                m = cost_of(i + lane, s);
+                sums = wave_prefix(m * w.Hkv);
             }
-            const uint64_t past = __builtin_amdgcn_ballot_w64(before + s > start);
+            const uint64_t past = __builtin_amdgcn_ballot_w64(before + sums > start);
             if (past != 0) {
                 const int l = __builtin_ctzll(past);
                 b = i + l;
-                before += __builtin_amdgcn_readlane(s, l) - __builtin_amdgcn_readlane(m, l);
+                per_head = __builtin_amdgcn_readlane(m, l);
+                before += __builtin_amdgcn_readlane(sums, l) - per_head * w.Hkv;
+                seq = PagedSeq{__builtin_amdgcn_readlane(s.q0, l), __builtin_amdgcn_readlane(s.n, l),
+                               __builtin_amdgcn_readlane(s.len, l)};
                 break;
             }
-            before += __builtin_amdgcn_readlane(s, 63);
+            before += __builtin_amdgcn_readlane(sums, 63);
         }
         b = uniform(b);
         at = start - uniform(before);
-        load_seq();
-        const int32_t per_head = MANY ? head_cost(seq) : uniform(paged_head_units<ROWS, BN>(w, seq) + n_rt * EXTRA);
-        if (per_head == 0) {
+        per_head = uniform(per_head);
+        if (per_head == 0) { // (lengths that change meanwhile)
             left = 0;
             return;
         }
+        n_rt = uniform(paged_row_tiles<ROWS>(w, seq.n));
         h = uniform(mask_imin(at / per_head, w.Hkv - 1));
         at -= h * per_head;
         rt = 0;

@@ -631,7 +631,7 @@ __global__ __launch_bounds__((TileCfg<D, I8>::THREADS), (TileCfg<D, I8>::WAVES_P
 
 } // namespace
 
-// Workers are workgroups; smallest share: four key tiles.
+// Workers are workgroups; smallest share: two key tiles.
 int paged_tile_attention(const PagedAttnArgs& a, PagedAttnParams& p, const PagedLaunch& l, hipStream_t stream,
                          std::string& err) {
     return paged_for_type(a, [&](auto t, auto d, auto i8) {
@@ -639,7 +639,7 @@ int paged_tile_attention(const PagedAttnArgs& a, PagedAttnParams& p, const Paged
         constexpr int D = decltype(d)::value;
         constexpr bool I8 = decltype(i8)::value;
         using C = TileCfg<D, I8>;
-        return paged_launch<C::ROWS, kBN, kItemCost>(a, reinterpret_cast<const void*>(&paged_tiles<T, D, I8>), C::THREADS, 1, 4, p, l,
+        return paged_launch<C::ROWS, kBN, kItemCost>(a, reinterpret_cast<const void*>(&paged_tiles<T, D, I8>), C::THREADS, 1, 2, p, l,
                                           stream, err, [&](dim3 grid) {
                                               hipLaunchKernelGGL((paged_tiles<T, D, I8>), grid, dim3(C::THREADS), 0,
                                                                  stream, p);
