@@ -285,11 +285,12 @@ __device__ __forceinline__ int32_t by_xcd(int32_t id, int32_t n) {
 
 
 // A worker's (a workgroup's, or a wave's) walk over its units, the same in every wave
-// of it.  Sequences are counted one to a lane, and the row tiles of a longer one (MANY:
-// there may be some) one to a lane again: one lane's count of the 64 row tiles of a
-// prompt, three times over, had taken 18 us.  An item costs its units and EXTRA (the time before
-// its first and after its last key tile, in key tiles), and the shares are of equal cost:
-// a worker with the many short row tiles at a prompt's begin has fewer key tiles.
+// of it.  Sequences are counted one to a lane, and with MANY the row tiles of a longer
+// one one to a lane again: one lane's count of the 64 row tiles of a prompt, three
+// times over, had taken 18 us.  (Without, where a sequence is meant to have one row
+// tile, longer ones are only slower.)  An item costs its units and EXTRA, the time
+// before its first and after its last key tile in key tiles, and the shares are of equal
+// cost: a worker with the many short row tiles at a prompt's begin has fewer key tiles.
 template <int ROWS, int BN, bool MANY, int EXTRA>
 struct PagedWalk {
     const PagedWork& w;
@@ -388,8 +389,15 @@ struct PagedWalk {
             }
             rt = uniform(rt);
             at = uniform(at);
+            load_tile();
+        } else {
+            load_tile();
+            while (at >= tile.units + EXTRA && rt + 1 < n_rt) {
+                at -= tile.units + EXTRA;
+                rt++;
+                load_tile();
+            }
         }
-        load_tile();
     }
 
     static constexpr int32_t kFewTiles = 2;

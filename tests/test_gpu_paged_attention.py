@@ -128,6 +128,14 @@ def test_many_row_tiles_per_worker(gpu, dtype, i8, d, window):
     run(gpu, pool, lens, 32, window=window, name=f"many prompts {dtype} {i8} {d} {window}")
 
 
+@pytest.mark.parametrize("dtype,i8", [(F16, False), (F16, True)])
+@pytest.mark.parametrize("max_q", [0, 1, 8])
+def test_more_rows_than_max_seqlen_q(gpu, dtype, i8, max_q):
+    lens = [300, 9, 700, 64] + [200] * 30
+    pool = Pool(lens, 2, 64, 16, dtype, i8, seed=6)
+    run(gpu, pool, [150, 3, 40, 64] + [33] * 30, 8, max_q=max_q, name=f"max_seqlen_q {max_q} {dtype} {i8}")
+
+
 @pytest.mark.parametrize("causal", [True, False])
 def test_more_row_tiles_than_lanes(gpu, causal):
     lens = [30, 1150, 700]
