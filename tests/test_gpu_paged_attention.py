@@ -405,6 +405,56 @@ def test_two_graphs_and_two_streams(gpu):
         assert all(torch.equal(outs[i], want[i]) for i in range(2))
 
 
+@pytest.mark.parametrize("ns,max_q", [([1] * 40, 1), ([1, 300, 5, 40] * 10, 300)])
+def test_output_over_the_query(gpu, ns, max_q):
+    import rdnattention as ra
+
+    lens = [n + 13 * (b % 40) for b, n in enumerate(ns)]
+    for dtype, d in ((F16, 128), (BF16, 160)):
+        pool = Pool(lens, 2, d, 16, dtype, seed=24)
+        k, v, table, lens_t, _ = pool.on(gpu)
+        q = torch.randn(sum(ns), 16, d, device=gpu).to(dtype)
+        cu = torch.tensor([sum(ns[:i]) for i in range(len(ns) + 1)], dtype=torch.int32, device=gpu)
+        want = ra.paged_attention(q, k, v, table, lens_t, cu_seqlens_q=cu, max_seqlen_q=max_q)
+        got = q.clone()
+        assert ra.paged_attention(got, k, v, table, lens_t, cu_seqlens_q=cu, max_seqlen_q=max_q, out=got) is got
+        assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("own_streams", [True, False])
+def test_two_host_threads(gpu, own_streams):
+    import threading
+
+    import rdnattention as ra
+
+    jobs, failed = [], []
+    for i, ns in enumerate(([1, 1], [1, 200])):
+        pool = Pool([900, 1500], 2, 64, 16, F16, seed=30 + i)
+        k, v, table, lens, _ = pool.on(gpu)
+        q = torch.randn(sum(ns), 8, 64, device=gpu).half()
+        cu = torch.tensor([0, ns[0], sum(ns)], dtype=torch.int32, device=gpu)
+        jobs.append(lambda q=q, k=k, v=v, t=table, n=lens, cu=cu, m=max(ns): ra.paged_attention(
+            q, k, v, t, n, cu_seqlens_q=cu, max_seqlen_q=m))
+    want = [job() for job in jobs]
+    torch.cuda.synchronize()
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream() if own_streams else torch.cuda.default_stream()):
+                got = [jobs[i]() for _ in range(30)]
+                torch.cuda.current_stream().synchronize()
+            assert all(torch.equal(x, want[i]) for x in got)
+        except BaseException as e:  # reported by the test's own thread
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, failed
+
+
 def test_same_bits_every_time(gpu):
     import rdnattention as ra
 
