@@ -10,19 +10,13 @@
 // (PagedWalk), which also splits the keys of a call of few row tiles over the chip.
 //
 // Step i of a wave: M(i), O += V(i - 1)^T P(i - 1) and S(i) = K(i) Q^T, one stream
-// of MFMAs; then X(i), the softmax of S(i) to P(i).  Up to D = 128 there are two groups
-// of four waves, A and B, one of each on every SIMD, half a step apart, so that one
-// feeds the matrix core while the other runs its softmax, barrier to barrier:
-//
-//   phase     0    1    2    3    4   ...
-//   group A  M(0) X(0) M(1) X(1) M(2)
-//   group B   -   M(0) X(0) M(1) X(1)
-//
-// K(i) and V(i - 1) are read in phases 2i and 2i + 1 and have two slots each.  A copies
-// the values, V(i) in its X(i) (phase 2i + 1; V(i - 2) was last read in 2i - 1), and
-// awaits them at that phase's end.  B copies the keys, K(i + 2) in its X(i) (2i + 2;
-// K(i) was last read in 2i + 1), and awaits them at the end of its M(i + 1).  Above
-// D = 128, where one wave fills a SIMD, a step is one phase of four waves.
+// of MFMAs; then the softmax of S(i) to P(i), and one barrier.  K(i + 1) and V(i) are
+// copied during step i, up to D = 128 (eight waves) the keys by waves 4-7 and the
+// values by waves 0-3, into the second of two slots each.  The two waves of a SIMD drift
+// apart by themselves, so that one feeds the matrix core while the other runs its
+// softmax.  (Two groups of waves held half a step apart by two barriers took 2 % less
+// time on B4 Hq32 Hkv8 S4096 D128 causal, 7 % more at D = 96 and on one sequence of 16
+// drafts, 15 % more on int8 pages.)
 //
 // Q goes through LDS too (up to D = 128, where there is room), in whole lines: loaded
 // straight into the MFMA layout every line was fetched several times over, 4 us of an
@@ -33,7 +27,10 @@ namespace rdna_amd {
 namespace {
 
 constexpr int kBN = 64;
-constexpr int kItemCost = 5; // key tiles that an item's begin and end take the time of: 8 us of 1.9 us each
+// Key tiles that an item's begin and end take the time of (about 8 us against 1.9 us).
+// us with 3 / 5 / 7: B4 Hq32 Hkv8 S4096 D128 causal 658 / 646 / 651, B2 Hq16 Hkv8 S2048
+// D96 74 / 76 / 77, 8 trees of 60 drafts 108 / 102 / 101.
+constexpr int kItemCost = 4;
 constexpr float kRescale = 8.0f;
 
 // for lambdas that are called more than once: called, they would keep what they
@@ -43,13 +40,13 @@ constexpr float kRescale = 8.0f;
 template <int D, bool I8>
 struct TileCfg {
     // eight waves; above D = 128 four, one per SIMD, whose O takes up to 128 registers
-    static constexpr bool PAIR = D <= 128;
-    static constexpr int WAVES = PAIR ? 8 : 4;
+    static constexpr int WAVES = D <= 128 ? 8 : 4;
+    static constexpr bool SPLIT = WAVES == 8; // waves 0-3 stage values, 4-7 keys
     static constexpr int THREADS = 64 * WAVES;
-    static constexpr int WAVES_PER_SIMD = PAIR ? 2 : 1;
+    static constexpr int WAVES_PER_SIMD = D <= 32 ? 4 : (SPLIT ? 2 : 1);
     static constexpr int ROWS = 32 * WAVES;
-    static constexpr bool KEEP = PAIR && !I8; // operand addresses in registers
-    static constexpr bool Q_LDS = PAIR;
+    static constexpr bool KEEP = SPLIT && !I8; // operand addresses in registers
+    static constexpr bool Q_LDS = SPLIT;
     static constexpr int DEPTH = D <= 224 ? 4 : 3; // MFMA operands in flight
     static constexpr int RB = 2 * D;
     static constexpr int KCH = D / 8;
@@ -87,7 +84,7 @@ __global__ __launch_bounds__((TileCfg<D, I8>::THREADS), (TileCfg<D, I8>::WAVES_P
     const int lane = tid & 63;
     const int l32 = lane & 31;
     const int g = lane >> 5;
-    const bool second = C::PAIR && wave >= 4; // group B
+    const bool second = C::SPLIT && wave >= 4; // stages keys
     constexpr int V_SLOTS = 2 * C::TILE_BYTES;
     const uint32_t lds0 = (uint32_t)reinterpret_cast<uintptr_t>(dsm);
     constexpr int TABS = 2 * V_SLOTS;
@@ -252,7 +249,7 @@ __global__ __launch_bounds__((TileCfg<D, I8>::THREADS), (TileCfg<D, I8>::WAVES_P
             if (t >= nt) {
                 return;
             }
-            if ((C::PAIR || !values) && t > 0 && (t & ((1 << log_b) - 1)) == 0) {
+            if ((C::SPLIT || !values) && t > 0 && (t & ((1 << log_b) - 1)) == 0) {
                 issue_tab(tab_rsrc(walk.b), odd, t0, (t >> log_b) + 1); // over entries of three batches ago
             }
             const char* const base = values ? vbase : kbase;
@@ -291,28 +288,34 @@ __global__ __launch_bounds__((TileCfg<D, I8>::THREADS), (TileCfg<D, I8>::WAVES_P
         // keys and values, which X(i) reads.
         constexpr int RCH = D / 16;
         float* const scales = reinterpret_cast<float*>(dsm + TABS); // [tile % 4][keys, values][kBN]
-        auto chunk_row = [&](int c) { return (256 * c + (tid & 255)) / RCH; };
+        auto fresh_tid = [&]() RDNA_INLINE { // no addresses kept in registers
+            int td = tid & 255;
+            asm volatile("" : "+v"(td));
+            return td;
+        };
         int32_t ent[C::NCH];
         i4 raw[C::NCH];
         float ksc[C::NCH], vsc[C::NCH];
         auto load_entries = [&](int t) RDNA_INLINE {
+            const int td = fresh_tid();
 #pragma unroll
             for (int c = 0; c < C::NCH; c++) {
-                const int e = ((t0 + t) * kBN + chunk_row(c)) >> p.c.lps;
+                const int e = ((t0 + t) * kBN + (256 * c + td) / RCH) >> p.c.lps;
                 ent[c] = p.c.table[walk.b * p.c.table_s + min(e, p.c.width - 1)];
             }
         };
         auto load_raw = [&](int t) RDNA_INLINE {
+            const int td = fresh_tid();
             const char* const base = second ? kbase : vbase;
             const int64_t sp = second ? p.c.k_sp : p.c.v_sp;
             const int64_t st = second ? p.c.k_st : p.c.v_st;
 #pragma unroll
             for (int c = 0; c < C::NCH; c++) {
-                const int key = (t0 + t) * kBN + chunk_row(c);
+                const int key = (t0 + t) * kBN + (256 * c + td) / RCH;
                 const bool seen = key >= item.lo && key <= item.hi;
                 const int64_t pg = (uint32_t)ent[c] < (uint32_t)p.c.pages ? ent[c] : 0;
                 const int64_t off = (uint32_t)key & page_mask;
-                raw[c] = *reinterpret_cast<const i4*>(base + pg * sp + off * st + 16 * (tid % RCH));
+                raw[c] = *reinterpret_cast<const i4*>(base + pg * sp + off * st + 16 * (td % RCH));
                 if (second) {
                     const float a = p.c.ks[pg * p.c.ks_sp + off * p.c.ks_st + h * p.c.ks_sh];
                     const float b = p.c.vs[pg * p.c.vs_sp + off * p.c.vs_st + h * p.c.vs_sh];
@@ -322,8 +325,7 @@ __global__ __launch_bounds__((TileCfg<D, I8>::THREADS), (TileCfg<D, I8>::WAVES_P
             }
         };
         auto stage_int8 = [&](int t) RDNA_INLINE {
-            int td = tid & 255;
-            asm volatile("" : "+v"(td)); // no addresses kept in registers
+            const int td = fresh_tid();
 #pragma unroll
             for (int c = 0; c < C::NCH; c++) {
                 const int r = (256 * c + td) / RCH;
@@ -348,7 +350,7 @@ __global__ __launch_bounds__((TileCfg<D, I8>::THREADS), (TileCfg<D, I8>::WAVES_P
             load_raw(t + 1);
             load_entries(t + 2);
         };
-        // keys or values of tile t: with two groups the wave's kind
+        // keys or values of tile t: of eight waves the wave's kind
         auto stage = [&](bool values, int t) RDNA_INLINE {
             if constexpr (I8) {
                 stage_int8(t);
@@ -368,7 +370,7 @@ __global__ __launch_bounds__((TileCfg<D, I8>::THREADS), (TileCfg<D, I8>::WAVES_P
                 load_raw(0);
                 load_entries(1);
             }
-            if (!C::PAIR || second) {
+            if (!C::SPLIT || second) {
                 stage(false, 0);
             }
         }
@@ -542,57 +544,35 @@ __global__ __launch_bounds__((TileCfg<D, I8>::THREADS), (TileCfg<D, I8>::WAVES_P
         }
         odd ^= 1;
         if (nt > 0) {
-            if constexpr (C::PAIR) {
-                // both groups pass 2 nt + 2 barriers from here on
-                if (second) {
-                    stage(false, 1);
-                    __syncthreads();
-                }
+            if (!C::SPLIT || second) {
+                stage(false, 1);
+            }
+            if (!C::SPLIT || !second) {
+                stage(true, 0);
+            }
+            if (active) {
+                mfmas(No{}, 0);
+            }
+            for (int i = 0; i < nt; i++) {
                 if (active) {
-                    mfmas(No{}, 0);
+                    softmax(i);
                 }
-                for (int i = 0; i < nt; i++) {
-                    if (!I8 && second) {
-                        __builtin_amdgcn_s_waitcnt(waitcnt_vm(0)); // its copies of K(i + 1)
-                    }
-                    __syncthreads();
-                    stage(!second, second ? i + 2 : i);
-                    if (active) {
-                        softmax(i);
-                    }
-                    if (!I8 && !second) {
-                        __builtin_amdgcn_s_waitcnt(waitcnt_vm(0)); // its copies of V(i)
-                    }
-                    __syncthreads();
-                    if (active) {
-                        mfmas(Yes{}, i + 1);
-                    }
+                if constexpr (!I8) {
+                    __builtin_amdgcn_s_waitcnt(waitcnt_vm(0)); // its copies of K(i + 1), V(i)
                 }
                 __syncthreads();
-                if (!second) {
-                    __syncthreads();
-                }
-            } else {
-                stage(false, 1);
-                stage(true, 0);
-                if (active) {
-                    mfmas(No{}, 0);
-                }
-                for (int i = 0; i < nt; i++) {
-                    if (active) {
-                        softmax(i);
-                    }
-                    __builtin_amdgcn_s_waitcnt(0); // its copies of K(i + 1), V(i)
-                    __syncthreads();
+                if (!C::SPLIT || second) {
                     stage(false, i + 2);
-                    stage(true, i + 1);
-                    if (active) {
-                        mfmas(Yes{}, i + 1);
-                    }
                 }
-                __builtin_amdgcn_s_waitcnt(0);
-                __syncthreads(); // the next item's copies overwrite the slots
+                if (!C::SPLIT || !second) {
+                    stage(true, i + 1);
+                }
+                if (active) {
+                    mfmas(Yes{}, i + 1);
+                }
             }
+            __builtin_amdgcn_s_waitcnt(0);
+            __syncthreads(); // the next item's copies overwrite the slots
         }
 
         const float l_tot = pair_sum(l_run);
