@@ -1,8 +1,8 @@
 /*
  * rdnattention_ext.h -- entry points of librdnattention.so that have no
- * counterpart in the reference's C ABI.  They exist for testing and
- * measurement; the four drop-in symbols in rdnattention.h do not depend on
- * them.  Same return-code and error-string conventions as rdnattention.h.
+ * counterpart in the reference's C ABI: paged key/value caches, quantisers,
+ * and what testing and measurement need; the four drop-in symbols in
+ * rdnattention.h do not depend on them.  Same return-code and error-string conventions as rdnattention.h.
  */
 #ifndef RDNATTENTION_EXT_H
 #define RDNATTENTION_EXT_H
@@ -30,8 +30,8 @@ RDNA_API int32_t rdna_attention_forward_path(
     int32_t path, void* hip_stream);
 
 /* Releases the device memory the library keeps for reuse: the scratch
- * buffers (RoPE-rotated K copies, split-K partials, quantiser partials, INT8
- * decode scores) it caches per (device, stream, use), grown to the largest
+ * buffers (RoPE-rotated K copies, split-K and paged partials, quantiser
+ * partials, INT8 decode scores) it caches per (device, stream, use), grown to the largest
  * call so far (at most 256 MiB each, at most 1 GiB per device over all
  * streams and uses), and the free blocks of the devices' default memory
  * pools.  A call never frees or
