@@ -24,11 +24,9 @@ struct PagedLaunch {
 // The merge of the items that several workgroups share (paged_merge.hip).
 int paged_merge(const PagedAttnArgs& a, const PagedAttnParams& p, hipStream_t stream, std::string& err);
 
-// Workgroups of `per_group` workers each for at most `units` units in shares of
-// min_units at least.
-inline int paged_workgroups(int64_t resident, int per_group, int64_t units, int min_units) {
-    const int64_t shares = (units + min_units - 1) / min_units;
-    int64_t n = std::min<int64_t>({resident, kPagedMaxWorkers / per_group, (shares + per_group - 1) / per_group});
+// Workers (workgroups) for at most `units` units in shares of min_units at least.
+inline int paged_workgroups(int64_t resident, int64_t units, int min_units) {
+    int64_t n = std::min<int64_t>({resident, kPagedMaxWorkers, (units + min_units - 1) / min_units});
     n = n >= 8 ? n / 8 * 8 : std::max<int64_t>(n, 1);
     return (int)n;
 }
@@ -45,7 +43,7 @@ constexpr size_t paged_scratch_bytes(int n_wg, int rows, int D) {
 }
 
 template <int ROWS, int BN, int EXTRA, class Go>
-int paged_launch(const PagedAttnArgs& a, const void* kernel, int threads, int per_group, int min_units, PagedAttnParams& p,
+int paged_launch(const PagedAttnArgs& a, const void* kernel, int threads, int min_units, PagedAttnParams& p,
                  const PagedLaunch& l, hipStream_t stream, std::string& err, Go&& go) {
     const int64_t units = paged_max_units<ROWS, BN, EXTRA>(p.work);
     if (units > INT32_MAX) {
@@ -59,8 +57,7 @@ int paged_launch(const PagedAttnArgs& a, const void* kernel, int threads, int pe
     p.work.min_rows = l.min_rows;
     p.work.max_rows = l.max_rows;
     p.work.min_units = min_units;
-    const int groups = paged_workgroups(resident, per_group, units, min_units);
-    p.work.n_wg = groups * per_group;
+    p.work.n_wg = paged_workgroups(resident, units, min_units);
     p.slot_rows = (int32_t)std::min<int64_t>(ROWS, (int64_t)p.work.seqs.total * p.work.G);
     const size_t bytes = paged_scratch_bytes(p.work.n_wg, p.slot_rows, a.D);
     StreamScratch ws(ScratchUse::PagedPartials);
@@ -72,7 +69,7 @@ int paged_launch(const PagedAttnArgs& a, const void* kernel, int threads, int pe
     p.records = reinterpret_cast<PagedRecord*>(p.part_ml + (size_t)2 * p.work.n_wg * p.slot_rows * 2);
     {
         KernelTimerGuard timer(stream);
-        go(dim3((uint32_t)groups));
+        go(dim3((uint32_t)p.work.n_wg));
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) {
             err = hipGetErrorString(e);

@@ -474,11 +474,10 @@ int paged_stream_attention(const PagedAttnArgs& a, PagedAttnParams& p, const Pag
         constexpr bool I8 = decltype(i8)::value;
         auto go = [&](auto waves) {
             constexpr int WV = decltype(waves)::value;
-            return paged_launch<kRows, kTile, 0>(a, reinterpret_cast<const void*>(&paged_stream<T, D, I8, WV>), 64 * WV, 1,
-                                              WV, p, l, stream, err, [&](dim3 grid) {
-                                                  hipLaunchKernelGGL((paged_stream<T, D, I8, WV>), grid, dim3(64 * WV),
-                                                                     0, stream, p);
-                                              });
+            const void* kernel = reinterpret_cast<const void*>(&paged_stream<T, D, I8, WV>);
+            return paged_launch<kRows, kTile, 0>(
+                a, kernel, 64 * WV, WV, p, l, stream, err,
+                [&](dim3 grid) { hipLaunchKernelGGL((paged_stream<T, D, I8, WV>), grid, dim3(64 * WV), 0, stream, p); });
         };
         // Eight waves on a CU where there are few heads: one workgroup, which streams
         // a head's keys in one front; where there are many, two of four waves, of

@@ -620,11 +620,10 @@ int paged_tile_attention(const PagedAttnArgs& a, PagedAttnParams& p, const Paged
         constexpr int D = decltype(d)::value;
         constexpr bool I8 = decltype(i8)::value;
         using C = TileCfg<D, I8>;
-        return paged_launch<C::ROWS, kBN, kItemCost>(a, reinterpret_cast<const void*>(&paged_tiles<T, D, I8>), C::THREADS, 1, 2, p, l,
-                                          stream, err, [&](dim3 grid) {
-                                              hipLaunchKernelGGL((paged_tiles<T, D, I8>), grid, dim3(C::THREADS), 0,
-                                                                 stream, p);
-                                          });
+        const void* kernel = reinterpret_cast<const void*>(&paged_tiles<T, D, I8>);
+        return paged_launch<C::ROWS, kBN, kItemCost>(
+            a, kernel, C::THREADS, 2, p, l, stream, err,
+            [&](dim3 grid) { hipLaunchKernelGGL((paged_tiles<T, D, I8>), grid, dim3(C::THREADS), 0, stream, p); });
     });
 }
 
