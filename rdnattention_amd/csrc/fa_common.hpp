@@ -257,6 +257,12 @@ __device__ __forceinline__ h8 buffer_load_h8(__amdgpu_buffer_rsrc_t r, uint32_t 
 // as a store to every LDS location (it would otherwise wait for all of them
 // before each LDS read); callers wait on vmcnt themselves.  The V# is built
 // by hand: base, stride 0, num_records, DATA_FORMAT 32.
+//
+// Nor does the compiler keep the wait states of what stands in inline asm, so
+// the asm has them itself: one between the write of M0 and the copy, five
+// between a vector instruction that writes a scalar register (v_readfirstlane;
+// v_readlane, which also reloads a spilled one) and a vector memory
+// instruction that reads it.  s_mov and s_nop 3 are five.
 typedef int i32x4_t __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ i32x4_t make_rsrc_v(const void* base, uint32_t num_records) {
     const uint64_t a = reinterpret_cast<uint64_t>(base);
@@ -268,7 +274,7 @@ __device__ __forceinline__ i32x4_t make_rsrc_v(const void* base, uint32_t num_re
     return r;
 }
 __device__ __forceinline__ void dma_load16(i32x4_t rsrc, uint32_t voff, uint32_t lds_byte_addr) {
-    asm volatile("s_mov_b32 m0, %2\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds"
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 3\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds"
                  :
                  : "v"(voff), "s"(rsrc), "s"(lds_byte_addr)
                  : "memory", "m0");
@@ -278,7 +284,7 @@ __device__ __forceinline__ void dma_load16(i32x4_t rsrc, uint32_t voff, uint32_t
 // Each lane's dword is range-checked on its own, so a vector of floats that
 // ends inside a 16-byte chunk is copied exactly.
 __device__ __forceinline__ void dma_load4(i32x4_t rsrc, uint32_t voff, uint32_t lds_byte_addr) {
-    asm volatile("s_mov_b32 m0, %2\n\tbuffer_load_dword %0, %1, 0 offen lds"
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 3\n\tbuffer_load_dword %0, %1, 0 offen lds"
                  :
                  : "v"(voff), "s"(rsrc), "s"(lds_byte_addr)
                  : "memory", "m0");
@@ -286,7 +292,7 @@ __device__ __forceinline__ void dma_load4(i32x4_t rsrc, uint32_t voff, uint32_t 
 // dma_load16 with a wave-uniform byte offset `soff` (the instruction's scalar
 // offset) added to voff: a loop over rows then keeps one vector offset.
 __device__ __forceinline__ void dma_load16_s(i32x4_t rsrc, uint32_t voff, uint32_t soff, uint32_t lds_byte_addr) {
-    asm volatile("s_mov_b32 m0, %3\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds"
+    asm volatile("s_mov_b32 m0, %3\n\ts_nop 3\n\tbuffer_load_dwordx4 %0, %1, %2 offen lds"
                  :
                  : "v"(voff), "s"(rsrc), "s"(soff), "s"(lds_byte_addr)
                  : "memory", "m0");
@@ -295,7 +301,7 @@ __device__ __forceinline__ void dma_load16_s(i32x4_t rsrc, uint32_t voff, uint32
 // (split-K decode streams K/V once): they then do not displace lines that are
 // reused. Kernels whose workgroups share K/V through the L2 use dma_load16.
 __device__ __forceinline__ void dma_load16_nt(i32x4_t rsrc, uint32_t voff, uint32_t lds_byte_addr) {
-    asm volatile("s_mov_b32 m0, %2\n\tbuffer_load_dwordx4 %0, %1, 0 offen nt lds"
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 3\n\tbuffer_load_dwordx4 %0, %1, 0 offen nt lds"
                  :
                  : "v"(voff), "s"(rsrc), "s"(lds_byte_addr)
                  : "memory", "m0");
@@ -303,7 +309,7 @@ __device__ __forceinline__ void dma_load16_nt(i32x4_t rsrc, uint32_t voff, uint3
 
 // dma_load16_nt with a wave-uniform byte offset (see dma_load16_s)
 __device__ __forceinline__ void dma_load16_nt_s(i32x4_t rsrc, uint32_t voff, uint32_t soff, uint32_t lds_byte_addr) {
-    asm volatile("s_mov_b32 m0, %3\n\tbuffer_load_dwordx4 %0, %1, %2 offen nt lds"
+    asm volatile("s_mov_b32 m0, %3\n\ts_nop 3\n\tbuffer_load_dwordx4 %0, %1, %2 offen nt lds"
                  :
                  : "v"(voff), "s"(rsrc), "s"(soff), "s"(lds_byte_addr)
                  : "memory", "m0");

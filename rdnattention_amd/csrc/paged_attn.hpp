@@ -90,29 +90,33 @@ __device__ __forceinline__ uint64_t readlane64(uint64_t v, int x) {
            (uint32_t)__builtin_amdgcn_readlane((int32_t)(uint32_t)v, x);
 }
 
-// HBM -> LDS copies with a 64-bit address per lane (see dma_load16)
+// HBM -> LDS copies with a 64-bit address per lane.  The wait states are those of
+// dma_load16: M0 is the only scalar register here.
 __device__ __forceinline__ void dma_gather16(uint64_t addr, uint32_t lds_byte_addr) {
-    asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off"
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off"
                  :
                  : "v"(addr), "s"(uniform((int32_t)lds_byte_addr))
                  : "memory", "m0");
 }
-// ... at a wave-uniform address and 32 bits per lane
+// ... at a wave-uniform address and 32 bits per lane.  The address usually comes straight
+// from v_readlane: copied by a scalar instruction, for which the hardware waits, it needs no
+// wait states before the load, and the copy is the one that M0 needs.
 __device__ __forceinline__ void dma_uniform16(uint64_t base, uint32_t off, uint32_t lds_byte_addr) {
-    asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1"
-                 :
+    uint64_t at;
+    asm volatile("s_mov_b32 m0, %3\n\ts_mov_b64 %0, %2\n\tglobal_load_lds_dwordx4 %1, %0"
+                 : "=&s"(at)
                  : "v"(off), "s"(uniform64(base)), "s"(uniform((int32_t)lds_byte_addr))
                  : "memory", "m0");
 }
 __device__ __forceinline__ void dma_gather16_nt(uint64_t addr, uint32_t lds_byte_addr) {
-    asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off nt"
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off nt"
                  :
                  : "v"(addr), "s"(uniform((int32_t)lds_byte_addr))
                  : "memory", "m0");
 }
 
 __device__ __forceinline__ void dma_gather4(uint64_t addr, uint32_t lds_byte_addr) {
-    asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dword %0, off"
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off"
                  :
                  : "v"(addr), "s"(uniform((int32_t)lds_byte_addr))
                  : "memory", "m0");
