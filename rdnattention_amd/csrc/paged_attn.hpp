@@ -298,16 +298,12 @@ __device__ __forceinline__ int32_t by_xcd(int32_t id, int32_t n) {
 template <int ROWS, int BN, bool MANY, int EXTRA>
 struct PagedWalk {
     const PagedWork& w;
-    int32_t wg;
-    int32_t left = 0;  // cost of the share not yet taken
-    int32_t at = 0;    // of the item's cost, what earlier shares have
-    int32_t start = 0; // of the call's cost, what lies before
-    int32_t share = 1;
+    PagedShare<EXTRA> part; // the worker's share, and of the current item
     int32_t b = 0, h = 0, rt = 0, n_rt = 0;
     PagedSeq seq;
     PagedTile tile;
 
-    __device__ __forceinline__ PagedWalk(const PagedWork& work, int32_t worker) : w(work), wg(uniform(worker)) {
+    __device__ __forceinline__ PagedWalk(const PagedWork& work, int32_t worker) : w(work), part(work, uniform(worker)) {
         const int lane = threadIdx.x & 63;
         const int32_t B = w.seqs.B;
         // sequence i and what one kv head of it costs
@@ -337,15 +333,14 @@ struct PagedWalk {
             PagedSeq s;
             total += __builtin_amdgcn_readlane(wave_prefix(cost_of(i + lane, s) * w.Hkv), 63);
         }
-        share = uniform(paged_share(w, total));
-        start = (int32_t)((int64_t)wg * share < total ? wg * share : total);
-        start = uniform(start);
-        left = uniform(mask_imin(share, total - start));
-        if (left <= 0) {
-            left = 0;
+        part.deal(w, total);
+        part.share = uniform(part.share);
+        part.start = uniform(part.start);
+        part.left = uniform(part.left);
+        if (!part.more()) {
             return;
         }
-        // the sequence that `start` is in
+        // the sequence that the share begins in
         int32_t before = 0, per_head = 0;
         for (int32_t i = 0; i < B; i += 64) {
             PagedSeq s = s0;
@@ -354,7 +349,7 @@ struct PagedWalk {
                 m = cost_of(i + lane, s);
                 sums = wave_prefix(m * w.Hkv);
             }
-            const uint64_t past = __builtin_amdgcn_ballot_w64(before + sums > start);
+            const uint64_t past = __builtin_amdgcn_ballot_w64(before + sums > part.start);
             if (past != 0) {
                 const int l = __builtin_ctzll(past);
                 b = i + l;
@@ -367,16 +362,15 @@ struct PagedWalk {
             before += __builtin_amdgcn_readlane(sums, 63);
         }
         b = uniform(b);
-        at = start - uniform(before);
         per_head = uniform(per_head);
-        if (per_head == 0) { // (lengths that change meanwhile)
-            left = 0;
+        if (per_head <= 0) { // (lengths that change meanwhile)
+            part.left = 0;
             return;
         }
         n_rt = uniform(paged_row_tiles<ROWS>(w, seq.n));
-        h = uniform(mask_imin(at / per_head, w.Hkv - 1));
-        at -= h * per_head;
+        h = uniform(part.enter(uniform(before), per_head, w.Hkv));
         rt = 0;
+        int32_t at = part.at;
         if constexpr (MANY) {
             // the row tile that `at` of the head is in
             for (int32_t first = 0; first < n_rt; first += 64) {
@@ -392,7 +386,6 @@ struct PagedWalk {
                 at -= __builtin_amdgcn_readlane(sum, 63);
             }
             rt = uniform(rt);
-            at = uniform(at);
             load_tile();
         } else {
             load_tile();
@@ -402,6 +395,8 @@ struct PagedWalk {
                 load_tile();
             }
         }
+        part.at = uniform(at);
+        part.item(tile.units);
     }
 
     static constexpr int32_t kFewTiles = 2;
@@ -446,59 +441,48 @@ struct PagedWalk {
         tile.hi = uniform(tile.hi);
         tile.first = uniform(tile.first);
         tile.units = uniform(tile.units);
-        if (at + left <= EXTRA) {
-            left = 0; // none of the item's units
-        }
     }
 
     // Every loop here ends by itself, whatever the lengths hold (a caller may, by
     // mistake, be changing them).
-    // The part of the current item that this share has: units [begin(), begin() +
-    // count()).
     __device__ __forceinline__ bool more() const {
-        return left > 0;
+        return part.more();
     }
     __device__ __forceinline__ int32_t begin() const {
-        return mask_imax(at - EXTRA, 0);
+        return part.begin();
     }
     __device__ __forceinline__ int32_t count() const {
-        return at + cost() - EXTRA - begin();
+        return part.count(tile.units);
     }
     __device__ __forceinline__ bool whole() const {
-        return begin() == 0 && at + cost() == tile.units + EXTRA;
+        return part.whole(tile.units);
     }
-    // Slot of a part that is not the whole item, and, of the first part, the last
-    // workgroup.
     __device__ __forceinline__ int32_t slot() const {
-        return begin() == 0 ? w.n_wg + wg : wg;
+        return part.slot();
     }
     __device__ __forceinline__ int32_t last_wg() const {
-        return (start - at + tile.units + EXTRA - 1) / share;
-    }
-    __device__ __forceinline__ int32_t cost() const {
-        return mask_imin(left, tile.units + EXTRA - at);
+        return part.last_wg(tile.units);
     }
     __device__ __forceinline__ void next() {
-        const int32_t n = cost();
-        left -= n;
-        start += n;
-        at = 0;
-        if (left > 0) {
-            if (++rt == n_rt) {
-                rt = 0;
-                if (++h == w.Hkv) {
-                    h = 0;
-                    do {
-                        if (++b >= w.seqs.B) {
-                            left = 0;
-                            return;
-                        }
-                        load_seq();
-                    } while (n_rt == 0);
-                }
-            }
-            load_tile();
+        part.take(tile.units);
+        if (!part.more()) {
+            return;
         }
+        if (++rt >= n_rt) {
+            rt = 0;
+            if (++h == w.Hkv) {
+                h = 0;
+                do {
+                    if (++b >= w.seqs.B) {
+                        part.left = 0;
+                        return;
+                    }
+                    load_seq();
+                } while (n_rt == 0);
+            }
+        }
+        load_tile();
+        part.item(tile.units);
     }
 };
 

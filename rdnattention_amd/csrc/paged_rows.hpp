@@ -7,13 +7,13 @@
 // and page tables are device memory that the host does not see, so every value
 // is bounded here and no access leaves a buffer, whatever they hold.
 //
-// The attention kernels deal a call's key tiles to their workers (workgroups, or
-// waves) in equal shares: the rows (n tokens of G query heads each) of every (sequence, kv
-// head) fall into row tiles of ROWS rows, a row tile is an item of as many
-// units as it sees key tiles of BN keys (one if none, for its zeros), and
-// worker w takes the units [w * per, (w + 1) * per) of the items in order
-// (sequence, kv head, row tile).  At most two of a worker's items are shared
-// with others: the first and the last.
+// The attention kernels deal a call's key tiles to their workers (workgroups): the
+// rows (n tokens of G query heads each) of every (sequence, kv head) fall into row
+// tiles of ROWS rows, and a row tile is an item of as many units as it sees key
+// tiles of BN keys (one if none, for its zeros).  An item costs its units and
+// EXTRA, what its begin and end take the time of, and worker w has the cost [w *
+// share, (w + 1) * share) of the items in order (sequence, kv head, row tile).
+// At most two of a worker's items are shared with others: the first and the last.
 #pragma once
 
 #include "fa_mask.hpp"
@@ -141,9 +141,78 @@ RDNA_MASK_FN int32_t paged_head_units(const PagedWork& w, const PagedSeq& s) {
     return u;
 }
 
-// Share of each worker of `total` units.
+// Cost of each worker's share of `total`.
 RDNA_MASK_FN int32_t paged_share(const PagedWork& w, int32_t total) {
-    return mask_imax((total + w.n_wg - 1) / w.n_wg, w.min_units);
+    return mask_imax(total / w.n_wg + (total % w.n_wg > 0 ? 1 : 0), w.min_units);
 }
+
+// Worker wg's share.  A caller that by mistake changes the lengths while a kernel
+// runs gets wrong rows, but no access outside a buffer: whatever the items'
+// units turn out to be, the parts lie inside their items, the slots and the last worker
+// inside their arrays, and the walk ends.
+template <int EXTRA>
+struct PagedShare {
+    int32_t n_wg, wg;
+    int32_t left = 0;  // cost not yet taken
+    int32_t at = 0;    // of the current item's cost, what earlier shares have
+    int32_t start = 0; // of the call's cost, what lies before
+    int32_t share = 1;
+
+    RDNA_MASK_FN PagedShare(const PagedWork& w, int32_t worker) : n_wg(w.n_wg), wg(worker) {}
+
+    RDNA_MASK_FN void deal(const PagedWork& w, int32_t total) {
+        share = paged_share(w, total);
+        start = (int64_t)wg * share < total ? wg * share : total;
+        left = mask_imax(mask_imin(share, total - start), 0);
+    }
+    // The share begins in a sequence with `before` in front of it, each of whose
+    // kv heads costs per_head > 0: that head.
+    RDNA_MASK_FN int32_t enter(int32_t before, int32_t per_head, int32_t Hkv) {
+        at = mask_imax(start - before, 0);
+        const int32_t h = mask_imin(at / per_head, Hkv - 1);
+        at -= h * per_head;
+        return h;
+    }
+    // The current item is one of `units`: nothing is left if none of them is in the
+    // share.
+    RDNA_MASK_FN void item(int32_t units) {
+        at = rows_clamp(at, 0, units + EXTRA - 1);
+        if (at + left <= EXTRA) {
+            left = 0;
+        }
+    }
+    RDNA_MASK_FN bool more() const {
+        return left > 0;
+    }
+    RDNA_MASK_FN int32_t cost(int32_t units) const {
+        return mask_imin(left, units + EXTRA - at);
+    }
+    // The part of the item in this share: units [begin, begin + count).
+    RDNA_MASK_FN int32_t begin() const {
+        return mask_imax(at - EXTRA, 0);
+    }
+    RDNA_MASK_FN int32_t count(int32_t units) const {
+        return at + cost(units) - EXTRA - begin();
+    }
+    RDNA_MASK_FN bool whole(int32_t units) const {
+        return begin() == 0 && at + cost(units) == units + EXTRA;
+    }
+    // Slot of a part that is not the whole item, and, of the first part, the last
+    // worker.
+    RDNA_MASK_FN int32_t slot() const {
+        return begin() == 0 ? n_wg + wg : wg;
+    }
+    RDNA_MASK_FN int32_t last_wg(int32_t units) const {
+        const uint32_t end = (uint32_t)(start - at) + (uint32_t)(units + EXTRA - 1);
+        return mask_imax((int32_t)(end / (uint32_t)share < (uint32_t)n_wg ? end / (uint32_t)share : n_wg - 1), wg);
+    }
+    // On to the next item, which is still to be given to item().
+    RDNA_MASK_FN void take(int32_t units) {
+        const int32_t n = cost(units);
+        left -= n;
+        start += n;
+        at = 0;
+    }
+};
 
 } // namespace rdna_amd

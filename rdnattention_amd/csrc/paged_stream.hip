@@ -459,7 +459,7 @@ __global__ __launch_bounds__((StreamCfg<D, I8, WV>::THREADS), (StreamCfg<D, I8, 
         walk.next();
     }
     if (tid == 0) {
-        p.records[walk.wg] = rec;
+        p.records[walk.part.wg] = rec;
     }
 }
 

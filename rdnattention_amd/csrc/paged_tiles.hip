@@ -606,7 +606,7 @@ __global__ __launch_bounds__((TileCfg<D, I8>::THREADS), (TileCfg<D, I8>::WAVES_P
         odd ^= 1;
     }
     if (tid == 0) {
-        p.records[walk.wg] = rec;
+        p.records[walk.part.wg] = rec;
     }
 }
 
