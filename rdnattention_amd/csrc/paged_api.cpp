@@ -19,17 +19,22 @@ bool aligned(const void* p, uintptr_t a) {
     return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0;
 }
 
-// Strides in elements of `size` bytes -> bytes; not negative, multiples of 16
-// bytes, small enough for a product with 31 bits.
-bool stride_bytes(int64_t stride, int64_t size, int64_t& out) {
-    if (stride < 0 || stride > (int64_t(1) << 40) || stride * size % 16 != 0) {
+// A stride in elements of `size` bytes over `count` of them: not negative, and all
+// within 2^56 bytes, so that sums of such offsets stay in 63 bits.
+bool stride_fits(int64_t stride, int64_t size, uint64_t count) {
+    return stride >= 0 && stride <= (int64_t(1) << 40) && (uint64_t)(stride * size) <= (uint64_t(1) << 56) / count;
+}
+
+// ... and a multiple of 16 bytes: in bytes.
+bool stride_bytes(int64_t stride, int64_t size, uint64_t count, int64_t& out) {
+    if (!stride_fits(stride, size, count) || stride * size % 16 != 0) {
         return false;
     }
     out = stride * size;
     return true;
 }
 
-constexpr const char* kStrides = "strides must be multiples of 16 bytes and not negative";
+constexpr const char* kStrides = "strides must be multiples of 16 bytes, not negative, and stay within 2^56 bytes";
 
 // The cache into `c` and `s`; "" or what is wrong.
 std::string check_cache(const rdna_paged_cache* in, rdna_amd::PagedPages& c, bool& i8) {
@@ -70,13 +75,18 @@ std::string check_cache(const rdna_paged_cache* in, rdna_amd::PagedPages& c, boo
     if (!aligned(in->key, 16) || !aligned(in->value, 16)) {
         return "cache base pointers must be 16-byte aligned";
     }
-    if (!aligned(in->block_tables, 4) || in->table_stride < 0 || in->table_stride > (int64_t(1) << 40)) {
-        return "block_tables must be an aligned int32 array with a row stride that is not negative";
+    if (!aligned(in->block_tables, 4) || !stride_fits(in->table_stride, 4, in->num_seqs)) {
+        return "block_tables must be an aligned int32 array with a row stride that is not negative and stays within "
+               "2^56 bytes";
     }
     const int64_t size = i8 ? 1 : 2;
-    if (!stride_bytes(in->key_stride[0], size, c.k_sp) || !stride_bytes(in->key_stride[1], size, c.k_st) ||
-        !stride_bytes(in->key_stride[2], size, c.k_sh) || !stride_bytes(in->value_stride[0], size, c.v_sp) ||
-        !stride_bytes(in->value_stride[1], size, c.v_st) || !stride_bytes(in->value_stride[2], size, c.v_sh)) {
+    const uint64_t counts[3] = {in->num_pages, in->page_size, in->num_kv_heads};
+    if (!stride_bytes(in->key_stride[0], size, counts[0], c.k_sp) ||
+        !stride_bytes(in->key_stride[1], size, counts[1], c.k_st) ||
+        !stride_bytes(in->key_stride[2], size, counts[2], c.k_sh) ||
+        !stride_bytes(in->value_stride[0], size, counts[0], c.v_sp) ||
+        !stride_bytes(in->value_stride[1], size, counts[1], c.v_st) ||
+        !stride_bytes(in->value_stride[2], size, counts[2], c.v_sh)) {
         return std::string("cache ") + kStrides;
     }
     if (i8) {
@@ -87,9 +97,9 @@ std::string check_cache(const rdna_paged_cache* in, rdna_amd::PagedPages& c, boo
             return "key_scale and value_scale must be aligned float arrays";
         }
         for (int i = 0; i < 3; i++) {
-            const int64_t a = in->key_scale_stride[i], b = in->value_scale_stride[i];
-            if (a < 0 || b < 0 || a > (int64_t(1) << 40) || b > (int64_t(1) << 40)) {
-                return "scale strides must not be negative";
+            if (!stride_fits(in->key_scale_stride[i], 4, counts[i]) ||
+                !stride_fits(in->value_scale_stride[i], 4, counts[i])) {
+                return "scale strides must not be negative, and stay within 2^56 bytes";
             }
         }
         c.ks = in->key_scale;
@@ -194,8 +204,10 @@ RDNA_API int32_t rdna_paged_append(const rdna_paged_cache* cache, const void* ke
             err = "null tensor pointer";
         } else if (!aligned(key, 16) || !aligned(value, 16) || !aligned(query, 16) || !aligned(query_out, 16)) {
             err = "tensor base pointers must be 16-byte aligned";
-        } else if (!stride_bytes(key_stride_row, 2, a.k_st) || !stride_bytes(key_stride_h, 2, a.k_sh) ||
-                   !stride_bytes(value_stride_row, 2, a.v_st) || !stride_bytes(value_stride_h, 2, a.v_sh)) {
+        } else if (!stride_bytes(key_stride_row, 2, num_rows, a.k_st) ||
+                   !stride_bytes(key_stride_h, 2, cache->num_kv_heads, a.k_sh) ||
+                   !stride_bytes(value_stride_row, 2, num_rows, a.v_st) ||
+                   !stride_bytes(value_stride_h, 2, cache->num_kv_heads, a.v_sh)) {
             err = std::string("row ") + kStrides;
         } else if ((rot_cos == nullptr) != (rot_sin == nullptr)) {
             err = "pass both rot_cos and rot_sin, or neither";
@@ -213,9 +225,10 @@ RDNA_API int32_t rdna_paged_append(const rdna_paged_cache* cache, const void* ke
                 err = "query without query_out";
             } else if (num_heads == 0 || num_heads > 65535) {
                 err = "num_heads must be 1 to 65535";
-            } else if (!stride_bytes(query_stride_row, 2, a.q_st) || !stride_bytes(query_stride_h, 2, a.q_sh) ||
-                       !stride_bytes(query_out_stride_row, 2, a.qo_st) ||
-                       !stride_bytes(query_out_stride_h, 2, a.qo_sh)) {
+            } else if (!stride_bytes(query_stride_row, 2, num_rows, a.q_st) ||
+                       !stride_bytes(query_stride_h, 2, num_heads, a.q_sh) ||
+                       !stride_bytes(query_out_stride_row, 2, num_rows, a.qo_st) ||
+                       !stride_bytes(query_out_stride_h, 2, num_heads, a.qo_sh)) {
                 err = std::string("query ") + kStrides;
             }
             a.Hq = (int32_t)num_heads;
@@ -272,16 +285,19 @@ RDNA_API int32_t rdna_paged_attention(const rdna_paged_cache* cache, const void*
             err = "null tensor pointer";
         } else if (!aligned(query, 16) || !aligned(output, 16)) {
             err = "tensor base pointers must be 16-byte aligned";
-        } else if (!stride_bytes(query_stride_row, 2, a.q_st) || !stride_bytes(query_stride_h, 2, a.q_sh) ||
-                   !stride_bytes(output_stride_row, 2, a.o_st) || !stride_bytes(output_stride_h, 2, a.o_sh)) {
+        } else if (!stride_bytes(query_stride_row, 2, num_rows, a.q_st) ||
+                   !stride_bytes(query_stride_h, 2, num_heads, a.q_sh) ||
+                   !stride_bytes(output_stride_row, 2, num_rows, a.o_st) ||
+                   !stride_bytes(output_stride_h, 2, num_heads, a.o_sh)) {
             err = std::string("query/output ") + kStrides;
         } else if (!std::isfinite(scale)) {
             err = "scale must be finite";
         } else if (tree_mask != nullptr && (causal != 0 || window_size > 0)) {
             err = "a tree mask goes with neither causal nor window_size";
         } else if (tree_mask != nullptr &&
-                   (tree_n == 0 || tree_n > (uint32_t)kPagedMaxLen || tree_stride_seq < 0 || tree_stride_row < 0)) {
-            err = "tree_n must be 1 to 2^28, the mask's strides not negative";
+                   (tree_n == 0 || tree_n > (uint32_t)kPagedMaxLen ||
+                    !stride_fits(tree_stride_seq, 1, cache->num_seqs) || !stride_fits(tree_stride_row, 1, tree_n))) {
+            err = "tree_n must be 1 to 2^28, the mask's strides not negative and within 2^56 bytes";
         }
         if (!err.empty()) {
             return -1;
@@ -326,8 +342,8 @@ RDNA_API int32_t rdna_paged_commit(const rdna_paged_cache* cache, const int32_t*
             err = "index arrays must be aligned int32 arrays";
         } else if (path_n == 0 || path_n > 1024) {
             err = "path_n must be 1 to 1024";
-        } else if (path_stride < 0 || path_stride > (int64_t(1) << 40)) {
-            err = "path_stride must not be negative";
+        } else if (!stride_fits(path_stride, 4, cache->num_seqs)) {
+            err = "path_stride must not be negative, and stay within 2^56 bytes";
         }
         if (!err.empty()) {
             return -1;
