@@ -248,8 +248,8 @@ typedef struct rdna_paged_cache {
  * first, by the angles of its index in the sequence or of positions[row]: channels
  * (2i, 2i + 1) by column i (rot_interleaved) or (i, i + rot_dim / 2); positions
  * outside the tables are taken as their first or last row.  With query, the query
- * rows [num_rows, num_heads, head_dim] are rotated likewise into query_out (which may
- * be query).  Rows without a place write nothing; their query rows come out as they
+ * rows [num_rows, num_heads, head_dim] are rotated likewise into query_out (query itself
+ * with its strides, or memory that does not overlap it).  Rows without a place write nothing; their query rows come out as they
  * are (rotated if positions are given, and the row is a sequence's).  rot_dim is a
  * multiple of 16. */
 RDNA_API int32_t rdna_paged_append(

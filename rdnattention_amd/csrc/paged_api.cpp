@@ -230,6 +230,8 @@ RDNA_API int32_t rdna_paged_append(const rdna_paged_cache* cache, const void* ke
                        !stride_bytes(query_out_stride_row, 2, num_rows, a.qo_st) ||
                        !stride_bytes(query_out_stride_h, 2, num_heads, a.qo_sh)) {
                 err = std::string("query ") + kStrides;
+            } else if (query == query_out && ((num_rows > 1 && a.q_st != a.qo_st) || (num_heads > 1 && a.q_sh != a.qo_sh))) {
+                err = "query_out in the place of query needs query's strides";
             }
             a.Hq = (int32_t)num_heads;
         }

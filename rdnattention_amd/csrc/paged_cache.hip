@@ -90,8 +90,9 @@ __global__ __launch_bounds__(kThreads) void paged_append_rows(AppendParams p) {
     V8 x = *reinterpret_cast<const V8*>(src + 16 * c);
     const bool rotated = which != 1 && 8 * c < a.rot;
     const int half = a.rot / 2;
+    const bool paired = rotated && !a.interleaved; // with the chunk half a rotation away
     V8 other = x;
-    if (rotated && !a.interleaved) {
+    if (paired) {
         other = *reinterpret_cast<const V8*>(src + 16 * c + (8 * c < half ? 2 * half : -2 * half));
     }
 
@@ -128,15 +129,26 @@ __global__ __launch_bounds__(kThreads) void paged_append_rows(AppendParams p) {
     if (rotated && b >= 0 && (a.positions != nullptr || key >= 0)) {
         const int32_t pos = rows_clamp(a.positions != nullptr ? a.positions[t] : key, 0, a.rot_rows - 1);
         const int64_t off = (int64_t)pos * half;
+        const V8 was = x;
         if (I8 && which == 0) {
             x = rotate8<T, double>(x, other, a.cos + off, a.sin + off, c, half, a.interleaved != 0);
         } else {
             x = rotate8<T, float>(x, other, a.cos + off, a.sin + off, c, half, a.interleaved != 0);
         }
+        if (which == 2 && paired) {
+            other = rotate8<T, float>(other, was, a.cos + off, a.sin + off, c + half / 8, half, false);
+        }
     }
     if (which == 2) {
-        if (active) {
-            *reinterpret_cast<V8*>((char*)a.q_out + t * a.qo_st + h * a.qo_sh + 16 * c) = x;
+        // The queries may be rotated in place: of two chunks that are rotated together the
+        // first one's thread, which has read both, writes both.  (A head's 12, 20, 24 or 28
+        // chunks straddle waves and workgroups, so the other thread may read them later.)
+        char* const dst = (char*)a.q_out + t * a.qo_st + h * a.qo_sh + 16 * c;
+        if (active && !(paired && 8 * c >= half)) {
+            *reinterpret_cast<V8*>(dst) = x;
+            if (paired) {
+                *reinterpret_cast<V8*>(dst + 2 * half) = other;
+            }
         }
         return;
     }

@@ -46,3 +46,11 @@ def test_no_offset_in_the_rows_leaves_63_bits(lib, kw):  # noqa: F811
 def test_no_offset_in_the_paths_leaves_63_bits(lib):  # noqa: F811
     rc, err = commit(lib, cache(num_seqs=65535), stride=2 ** 39)
     assert rc == -3 and "path_stride" in err and "2^56" in err, err
+
+
+@pytest.mark.parametrize("kw", [dict(os=320), dict(oh=128), dict(qs=512, qh=128)])
+def test_queries_in_place_need_their_own_strides(lib, kw):  # noqa: F811
+    """Rows that lie elsewhere in the same memory would be written over before
+    they are read."""
+    rc, err = append(lib, cache(), cos=_P, sin=_P, query=_P, out=_P, **kw)
+    assert rc == -3 and "query's strides" in err, err
