@@ -20,6 +20,12 @@ struct PagedLaunch {
     int32_t min_rows = 0;
     int32_t max_rows = INT32_MAX;
 };
+inline PagedWork paged_work(const PagedWork& call, const PagedLaunch& l) {
+    PagedWork w = call;
+    w.min_rows = l.min_rows;
+    w.max_rows = l.max_rows;
+    return w;
+}
 
 // The merge of the items that several workgroups share (paged_merge.hip).
 int paged_merge(const PagedAttnArgs& a, const PagedAttnParams& p, hipStream_t stream, std::string& err);
@@ -31,13 +37,6 @@ inline int paged_workgroups(int64_t resident, int64_t units, int min_units) {
     return (int)n;
 }
 
-// Cost of a call at most (see PagedWalk).
-template <int ROWS, int BN, int EXTRA>
-int64_t paged_max_units(const PagedWork& w) {
-    const int64_t tiles = (int64_t)w.seqs.total * w.G / ROWS + w.seqs.B;
-    return tiles * w.Hkv * (w.seqs.max_keys / BN + 1 + EXTRA);
-}
-
 constexpr size_t paged_scratch_bytes(int n_wg, int rows, int D) {
     return (size_t)n_wg * (2 * (size_t)rows * (D + 2) * sizeof(float) + sizeof(PagedRecord));
 }
@@ -45,19 +44,13 @@ constexpr size_t paged_scratch_bytes(int n_wg, int rows, int D) {
 template <int ROWS, int BN, int EXTRA, class Go>
 int paged_launch(const PagedAttnArgs& a, const void* kernel, int threads, int min_units, PagedAttnParams& p,
                  const PagedLaunch& l, hipStream_t stream, std::string& err, Go&& go) {
-    const int64_t units = paged_max_units<ROWS, BN, EXTRA>(p.work);
-    if (units > INT32_MAX) {
-        err = "the call has too many rows and page table entries (" + std::to_string(units) + " key tiles at most)";
-        return -1;
-    }
     const int64_t resident = resident_workgroups(kernel, threads, err);
     if (resident <= 0) {
         return -1;
     }
-    p.work.min_rows = l.min_rows;
-    p.work.max_rows = l.max_rows;
+    p.work = paged_work(p.work, l);
     p.work.min_units = min_units;
-    p.work.n_wg = paged_workgroups(resident, units, min_units);
+    p.work.n_wg = paged_workgroups(resident, paged_max_cost<ROWS, BN, EXTRA>(p.work), min_units);
     p.slot_rows = (int32_t)std::min<int64_t>(ROWS, (int64_t)p.work.seqs.total * p.work.G);
     const size_t bytes = paged_scratch_bytes(p.work.n_wg, p.slot_rows, a.D);
     StreamScratch ws(ScratchUse::PagedPartials);
@@ -113,5 +106,8 @@ int paged_stream_attention(const PagedAttnArgs& a, PagedAttnParams& p, const Pag
                            std::string& err);
 int paged_tile_attention(const PagedAttnArgs& a, PagedAttnParams& p, const PagedLaunch& l, hipStream_t stream,
                          std::string& err);
+// ... and what a launch of them may cost at most (paged_max_cost).
+int64_t paged_stream_cost(const PagedAttnArgs& a, const PagedWork& w);
+int64_t paged_tile_cost(const PagedAttnArgs& a, const PagedWork& w);
 
 } // namespace rdna_amd

@@ -2,7 +2,9 @@
 // several workgroups share.
 #include "paged_launch.hpp"
 
-#include <cmath>
+#include <algorithm>
+#include <cstdint>
+#include <string>
 
 namespace rdna_amd {
 
@@ -170,19 +172,24 @@ int paged_attention(const PagedAttnArgs& a, hipStream_t stream, std::string& err
     // Rows of a sequence and kv head: up to 32 stream the keys once; more share
     // them.  Ragged sequences may be of both kinds: each launch takes its own.
     constexpr int32_t kFew = 32;
-    const int64_t rows = (int64_t)a.max_rows_seq * p.work.G;
     PagedLaunch few, many;
-    if (rows <= kFew) {
-        return paged_stream_attention(a, p, few, stream, err);
+    const bool any_many = (int64_t)a.max_rows_seq * p.work.G > kFew;
+    const bool any_few = !any_many || a.seqs.cu != nullptr;
+    if (any_many && any_few) {
+        few.max_rows = many.min_rows = kFew;
     }
-    if (a.seqs.cu == nullptr) {
-        return paged_tile_attention(a, p, many, stream, err);
-    }
-    few.max_rows = many.min_rows = kFew;
-    if (paged_tile_attention(a, p, many, stream, err) != 0) {
+    // refused before the first of two launches has written anything
+    const int64_t cost = std::max(any_many ? paged_tile_cost(a, paged_work(p.work, many)) : 0,
+                                  any_few ? paged_stream_cost(a, paged_work(p.work, few)) : 0);
+    if (cost > INT32_MAX) {
+        err = "too many rows x heads x keys that the page table covers (up to " +
+              (cost == INT64_MAX ? std::string("2^63") : std::to_string(cost)) + " key tiles, at most 2^31 - 1)";
         return -1;
     }
-    return paged_stream_attention(a, p, few, stream, err);
+    if (any_many && paged_tile_attention(a, p, many, stream, err) != 0) {
+        return -1;
+    }
+    return any_few ? paged_stream_attention(a, p, few, stream, err) : 0;
 }
 
 } // namespace rdna_amd

@@ -141,6 +141,20 @@ RDNA_MASK_FN int32_t paged_head_units(const PagedWork& w, const PagedSeq& s) {
     return u;
 }
 
+// Most that the items of a call may cost (see PagedShare), whatever the lengths: the
+// sequences of a launch have more than min_rows and at most max_rows rows each, all of
+// them `total` tokens.  Past 32 bits the walk cannot count it.
+template <int ROWS, int BN, int EXTRA>
+inline int64_t paged_max_cost(const PagedWork& w) {
+    const int64_t rows = (int64_t)w.seqs.total * w.G;
+    const int64_t B = w.seqs.B;
+    const int64_t seqs = rows / ((int64_t)w.min_rows + 1) < B ? rows / ((int64_t)w.min_rows + 1) : B;
+    const int64_t each = ((int64_t)w.max_rows - 1) / ROWS + 1;
+    const int64_t tiles = rows / ROWS + seqs < seqs * each ? rows / ROWS + seqs : seqs * each;
+    const int64_t heads = tiles * w.Hkv;
+    return heads <= INT32_MAX ? heads * (w.seqs.max_keys / BN + 1 + EXTRA) : INT64_MAX;
+}
+
 // Cost of each worker's share of `total`.
 RDNA_MASK_FN int32_t paged_share(const PagedWork& w, int32_t total) {
     return mask_imax(total / w.n_wg + (total % w.n_wg > 0 ? 1 : 0), w.min_units);

@@ -465,6 +465,10 @@ __global__ __launch_bounds__((StreamCfg<D, I8, WV>::THREADS), (StreamCfg<D, I8, 
 
 } // namespace
 
+int64_t paged_stream_cost(const PagedAttnArgs&, const PagedWork& w) {
+    return paged_max_cost<kRows, kTile, 0>(w);
+}
+
 // Workers are workgroups; smallest share: a tile for every wave.
 int paged_stream_attention(const PagedAttnArgs& a, PagedAttnParams& p, const PagedLaunch& l, hipStream_t stream,
                            std::string& err) {

@@ -612,6 +612,11 @@ __global__ __launch_bounds__((TileCfg<D, I8>::THREADS), (TileCfg<D, I8>::WAVES_P
 
 } // namespace
 
+int64_t paged_tile_cost(const PagedAttnArgs& a, const PagedWork& w) {
+    return a.D <= 128 ? paged_max_cost<TileCfg<128, false>::ROWS, kBN, kItemCost>(w)
+                      : paged_max_cost<TileCfg<256, false>::ROWS, kBN, kItemCost>(w);
+}
+
 // Workers are workgroups; smallest share: two key tiles.
 int paged_tile_attention(const PagedAttnArgs& a, PagedAttnParams& p, const PagedLaunch& l, hipStream_t stream,
                          std::string& err) {

@@ -54,3 +54,14 @@ def test_queries_in_place_need_their_own_strides(lib, kw):  # noqa: F811
     they are read."""
     rc, err = append(lib, cache(), cos=_P, sin=_P, query=_P, out=_P, **kw)
     assert rc == -3 and "query's strides" in err, err
+
+
+@pytest.mark.parametrize("seqs,rows,heads,width,page", [
+    (65536, 65600, 32, 128, 1024),  # too many for the kernel of few rows only, which is launched second
+    (1, 2 ** 20, 64, 64, 2 ** 20), (2 ** 24, 2 ** 24 + 1, 32, 2 ** 10, 2 ** 18)])
+def test_calls_too_large_are_refused_whole(lib, seqs, rows, heads, width, page):  # noqa: F811
+    """Before the first launch: without a device any HIP call would give another
+    error."""
+    c = cache(num_seqs=seqs, num_kv_heads=8, table_width=width, page_size=page, cu_seqlens=_P, table_stride=width)
+    rc, err = attention(lib, c, rows=rows, heads=heads, most=rows)
+    assert rc == -3 and "key tiles" in err, err
