@@ -580,6 +580,12 @@ __global__ __launch_bounds__((TileCfg<D, I8>::THREADS), (TileCfg<D, I8>::WAVES_P
         const float unit = I8 ? vscale.factor() : 1.0f; // of O
         if (whole) {
             const float inv = l_tot > 0.0f ? unit / l_tot : 0.0f;
+            if (l_tot == 0.0f) { // no key seen: weights of zero, of values that need not be finite
+#pragma unroll
+                for (int dt = 0; dt < C::NDT; dt++) {
+                    oacc[dt] = f16x{};
+                }
+            }
             if (col_valid) {
                 char* const orow = p.o + (int64_t)(seq.q0 + tok) * p.o_st + head * p.o_sh;
 #pragma unroll
