@@ -99,7 +99,7 @@ __global__ __launch_bounds__(kThreads) void paged_append_rows(AppendParams p) {
     // the row's sequence and its place there
     int32_t b, key;
     if (a.seqs.cu == nullptr) {
-        b = t / a.seqs.rows;
+        b = paged_seq_of_row(a.seqs, t);
         key = rows_clamp(a.seqs.lens[b], 0, a.seqs.max_keys) - a.seqs.rows + (t - b * a.seqs.rows);
     } else {
         // the sequence of the wave's first row: how many end at or before it, 64 at a
@@ -111,15 +111,11 @@ __global__ __launch_bounds__(kThreads) void paged_append_rows(AppendParams p) {
             const bool ended = i + lane < a.seqs.B && a.seqs.cu[i + lane + 1] <= t0;
             b += __popcll(__builtin_amdgcn_ballot_w64(ended));
         }
-        while (b < a.seqs.B && a.seqs.cu[b + 1] <= t) {
-            b++;
-        }
-        if (b < a.seqs.B && a.seqs.cu[b] <= t) {
+        b = paged_seq_of_row(a.seqs, t, b);
+        key = -1;
+        if (b >= 0) {
             const PagedSeq s = paged_seq(a.seqs, b);
             key = s.len - s.n + (t - s.q0);
-        } else {
-            b = -1;
-            key = -1;
         }
     }
     int32_t page = -1;

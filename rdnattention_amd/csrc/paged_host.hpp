@@ -16,7 +16,7 @@ namespace rdna_amd {
 // and a window stay in 32 bits).
 constexpr int64_t kPagedMaxLen = int64_t(1) << 28;
 
-enum class PagedType : int32_t { F16 = 0, BF16 = 1, I8 = 2 };
+enum class PagedType : int32_t { F16 = 0, BF16 = 1 }; // of rows
 
 // Pages of keys and values: [pages, page_size, Hkv, D] with strides in bytes
 // (page, token, head), scales of int8 pages likewise in floats.

@@ -59,21 +59,16 @@ RDNA_MASK_FN PagedSeq paged_seq(const PagedSeqs& s, int32_t b) {
     return r;
 }
 
-// The sequence that row t belongs to, -1 for a row behind the last one.
-RDNA_MASK_FN int32_t paged_seq_of_row(const PagedSeqs& s, int32_t t) {
+// The sequence that row t of a ragged call belongs to, none before `from`: the first
+// that ends behind it.  -1 for a row behind the last one.
+RDNA_MASK_FN int32_t paged_seq_of_row(const PagedSeqs& s, int32_t t, int32_t from = 0) {
     if (s.cu == nullptr) {
         return t / s.rows;
     }
-    int32_t lo = 0, hi = s.B; // the first b with cu[b + 1] > t
-    while (lo < hi) {
-        const int32_t mid = (lo + hi) >> 1;
-        if (s.cu[mid + 1] > t) {
-            hi = mid;
-        } else {
-            lo = mid + 1;
-        }
+    while (from < s.B && s.cu[from + 1] <= t) {
+        from++;
     }
-    return lo < s.B && s.cu[lo] <= t ? lo : -1;
+    return from < s.B && s.cu[from] <= t ? from : -1;
 }
 
 // Visibility of a sequence's keys (see MaskSpec); a tree's prefix and drafts

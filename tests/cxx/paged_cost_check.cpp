@@ -57,6 +57,14 @@ static void one() {
         cost += w.Hkv * ((int64_t)paged_head_units<ROWS, BN>(w, s) + EXTRA * paged_row_tiles<ROWS>(w, s.n));
     }
     CHECK((cost <= paged_max_cost<ROWS, BN, EXTRA>(w)));
+    // a row's sequence, searched for from any sequence that is not behind it
+    for (int32_t t = 0; ragged && t < w.seqs.total; t += 1 + t / 8) {
+        const int32_t b = paged_seq_of_row(w.seqs, t);
+        for (int32_t from = 0; from <= b; from++) {
+            CHECK(paged_seq_of_row(w.seqs, t, from) == b);
+        }
+        CHECK(paged_seq_of_row(w.seqs, t, B) == -1);
+    }
 }
 
 // A ragged call: rows of Hq / Hkv heads of B sequences over tables of `keys`.
