@@ -213,7 +213,9 @@ RDNA_API int32_t rdna_kernel_timer_read(double* total_ms, int64_t* launches);
  * seq_lens, block_tables and cu_seqlens are device memory that the host does not
  * read.  The newest rows of sequence b are the rows cu_seqlens[b] .. cu_seqlens[b +
  * 1] - 1 of a call's row tensors [num_rows, heads, head_dim] (cu_seqlens null:
- * num_rows / num_seqs each), n of them its keys seq_lens[b] - n .. seq_lens[b] - 1.
+ * num_rows / num_seqs each), n of them its keys seq_lens[b] - n .. seq_lens[b] - 1;
+ * cu_seqlens begins with 0 and never falls (other values reach no row outside the
+ * tensors, and give no defined result).
  * Rows behind the last sequence belong to none.  A length beyond the page table is
  * taken as the table's, a negative one as 0; the entry of a page that does not exist
  * never leads outside the pages (nothing is written for it, and what a call that
@@ -263,7 +265,10 @@ RDNA_API int32_t rdna_paged_append(
  * up to 256, query and output fp16 or bf16 (dtype; the pages' own type, or any with
  * int8 pages).  causal and window_size as in rdna_attention_forward.  A row that sees
  * no key is zeros.  max_rows_per_seq: most rows of a sequence as far as the caller
- * knows (num_rows if not); it picks kernels and decides no result.
+ * knows (num_rows if not); it picks kernels, which round in other places, and decides
+ * nothing else.  Calls that could have 2^31 key tiles are refused, before anything is
+ * launched: about rows x num_heads x keys of the table beyond 2^45 (2^44 above head_dim
+ * 128), or num_seqs x num_kv_heads x keys of the table beyond 2^36.
  *
  * With tree_mask ([num_seqs, tree_n, tree_n] bytes, 0 or 1, strides of sequences and
  * rows in bytes) the newest rows are drafts: row i sees every key before the drafts

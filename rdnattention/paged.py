@@ -8,8 +8,8 @@ axis; transpose a cache kept as [num_pages, kv_heads, page_size, head_dim]).  ``
 ``seq_lens`` int32 [sequences] count the keys in the cache, a step's new rows
 among them.  Row tensors are [rows, heads, head_dim]: without ``cu_seqlens_q``
 every sequence has rows / sequences of them, with it (int32 [sequences + 1])
-rows cu_seqlens_q[b] .. cu_seqlens_q[b + 1] - 1 are sequence b's, and rows
-behind the last sequence are padding.  A sequence's n rows are its newest: row
+rows cu_seqlens_q[b] .. cu_seqlens_q[b + 1] - 1 are sequence b's - it begins with
+0 and never falls - and rows behind the last sequence are padding.  A sequence's n rows are its newest: row
 i has index seq_lens[b] - n + i in the sequence.
 
 All of these are tensors on one HIP device; none is read on the host, so calls
@@ -315,7 +315,9 @@ def paged_attention(query, key_cache, value_cache, block_tables, seq_lens, *, cu
     as in flash_attn, aligned to the end of the keys; a row that sees no key
     comes out as zeros.  scale defaults to 1/sqrt(head_dim).  max_seqlen_q: most
     rows of any sequence (with cu_seqlens_q; default: all rows) - it picks
-    kernels and decides no result.
+    kernels, which round in other places, and decides nothing else.  Keys and values
+    that some row of a sequence sees should be finite: weights of zero are
+    multiplied too, so others may reach rows that do not see them.
 
     out: optional tensor like query to write to, whose padding rows stay as they
     are; a new tensor's are zeros.  Returns the output."""

@@ -1,6 +1,7 @@
 // C ABI of the paged-cache operators.  Every argument that the host can see is
-// checked here, before any HIP call; lengths, page tables and row ranges are
-// device memory and bounded where they are read (paged_rows.hpp).
+// checked before any HIP call, here and, the work of a whole attention call, in
+// paged_merge.hip; lengths, page tables and row ranges are device memory and
+// bounded where they are read (paged_rows.hpp).
 #include "rdnattention_ext.h"
 
 #include "paged_host.hpp"

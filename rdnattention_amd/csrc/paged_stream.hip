@@ -486,9 +486,10 @@ int paged_stream_attention(const PagedAttnArgs& a, PagedAttnParams& p, const Pag
         // Eight waves on a CU where there are few heads: one workgroup, which streams
         // a head's keys in one front; where there are many, two of four waves, of
         // which one begins and ends heads while the other streams.  us of eight / four,
-        // D = 128: fp16 16 x 18432 keys of 8 heads 195 / 202, 64 x 375 to 3000 keys 93 /
-        // 87, 128 x 512 59 / 52; int8 32 x 8192 116 / 120, 64 ragged 85 / 67.  At D = 64
-        // 117 / 107, 59 / 55; int8 75 / 79, 67 / 56.
+        // 8 heads, 16 x 18432 keys, 64 x 375 to 3000 keys, 128 x 512: D = 128 192 / 200, 101 /
+        // 94, 57 / 52; D = 96 190 / 192, 96 / 92, 55 / 50; int8 at D = 128, 32 x 8192 keys 115 /
+        // 120, 64 x 375 to 3000 78 / 63.  At D = 64 four are faster with few heads too (16 x
+        // 18432 117 / 107), but for int8 (75 / 79).
         if constexpr (D == 96 || D == 128) {
             if ((int64_t)a.seqs.B * a.Hkv < kManyHeads) {
                 return go(std::integral_constant<int, 8>{});

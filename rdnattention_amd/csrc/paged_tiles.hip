@@ -27,9 +27,10 @@ namespace rdna_amd {
 namespace {
 
 constexpr int kBN = 64;
-// Key tiles that an item's begin and end take the time of (about 8 us against 1.9 us).
-// us with 3 / 5 / 7: B4 Hq32 Hkv8 S4096 D128 causal 658 / 646 / 651, B2 Hq16 Hkv8 S2048
-// D96 74 / 76 / 77, 8 trees of 60 drafts 108 / 102 / 101.
+// Key tiles that an item's begin and end take the time of (about 8 us against 2.2 us).
+// us with 3 / 4 / 5 / 7: B4 Hq32 Hkv8 S4096 D128 causal 681 / 666 / 675 / 676, B2 Hq16 Hkv8
+// S2048 D96 74 / 74 / 78 / 78 and D256 143 / 145 / 148 / 152, int8 B2 Hq32 Hkv8 S2048 D128
+// 169 / 174 / 173 / 178, 8 trees of 60 drafts 105 / 104 / 105 / 104.
 constexpr int kItemCost = 4;
 constexpr float kRescale = 8.0f;
 
@@ -453,7 +454,8 @@ __global__ __launch_bounds__((TileCfg<D, I8>::THREADS), (TileCfg<D, I8>::WAVES_P
                     }
                 });
             // (the priority is zero already) keeps the softmax's instructions behind the last
-            // product: above D = 128 1 to 4 % less time
+            // product.  us with / without, causal S2048: B2 Hq32 Hkv8 D64 67.7 / 68.7, B2 Hq16 Hkv8
+            // D256 144.7 / 142.7, D96 to D224 within 1 %
             __builtin_amdgcn_s_setprio(0);
         };
         auto softmax = [&](int i) RDNA_INLINE {
