@@ -206,7 +206,8 @@ RDNA_API int32_t rdna_kernel_timer_read(double* total_ms, int64_t* launches);
  * Keys and values live in pages of page_size tokens (a power of two): element
  * (page, token, head, channel) of the keys at key + page * key_stride[0] + token *
  * key_stride[1] + head * key_stride[2] + channel, strides in elements, multiples of
- * 16 bytes; the values likewise.  Key j of sequence b is token j % page_size of page
+ * 16 bytes; the values likewise (append and commit refuse values at the keys' own
+ * address).  Key j of sequence b is token j % page_size of page
  * block_tables[b * table_stride + j / page_size].  int8 pages have a float scale per
  * (page, token, head), strides in floats: the value is int8 * scale.
  *

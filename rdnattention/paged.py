@@ -3,8 +3,8 @@
 Keys and values of all sequences live in pages of page_size tokens, a power of
 two: ``key_cache`` and ``value_cache`` are [num_pages, page_size, kv_heads,
 head_dim] (any strides of a multiple of 16 bytes with a contiguous head_dim
-axis; transpose a cache kept as [num_pages, kv_heads, page_size, head_dim]).  ``block_tables`` int32
-[sequences, width] lists each sequence's pages in order.  The lengths
+axis; transpose a cache kept as [num_pages, kv_heads, page_size, head_dim]), for appends and commits in
+memory of their own each.  ``block_tables`` int32 [sequences, width] lists each sequence's pages in order.  The lengths
 ``seq_lens`` int32 [sequences] count the keys in the cache, a step's new rows
 among them.  Row tensors are [rows, heads, head_dim]: without ``cu_seqlens_q``
 every sequence has rows / sequences of them, with it (int32 [sequences + 1])

@@ -35,6 +35,8 @@ bool stride_bytes(int64_t stride, int64_t size, uint64_t count, int64_t& out) {
     return true;
 }
 
+// For the calls that write pages: workgroups move keys and values independently.
+constexpr const char* kShared = "the pages of keys and values must not be the same memory";
 constexpr const char* kStrides = "strides must be multiples of 16 bytes, not negative, and stay within 2^56 bytes";
 
 // The cache into `c` and `s`; "" or what is wrong.
@@ -239,6 +241,8 @@ RDNA_API int32_t rdna_paged_append(const rdna_paged_cache* cache, const void* ke
         if (err.empty() &&
             (uint64_t)num_rows * (uint64_t)(2 * a.Hkv + a.Hq) * (uint64_t)(a.D / 8) > (uint64_t)INT32_MAX) {
             err = "rows x heads x head_dim exceed 2^34 channels";
+        } else if (err.empty() && a.c.k == a.c.v) {
+            err = kShared;
         }
         if (!err.empty()) {
             return -1;
@@ -347,6 +351,8 @@ RDNA_API int32_t rdna_paged_commit(const rdna_paged_cache* cache, const int32_t*
             err = "path_n must be 1 to 1024";
         } else if (!stride_fits(path_stride, 4, cache->num_seqs)) {
             err = "path_stride must not be negative, and stay within 2^56 bytes";
+        } else if (a.c.k == a.c.v) {
+            err = kShared;
         }
         if (!err.empty()) {
             return -1;

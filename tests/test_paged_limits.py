@@ -65,3 +65,11 @@ def test_calls_too_large_are_refused_whole(lib, seqs, rows, heads, width, page):
     c = cache(num_seqs=seqs, num_kv_heads=8, table_width=width, page_size=page, cu_seqlens=_P, table_stride=width)
     rc, err = attention(lib, c, rows=rows, heads=heads, most=rows)
     assert rc == -3 and "key tiles" in err, err
+
+
+def test_keys_and_values_in_one_memory_are_not_written(lib):  # noqa: F811
+    """The workgroups that move keys and those that move values do not wait for
+    each other: in one memory a commit would read what it has already moved."""
+    for call in (append, commit):
+        rc, err = call(lib, cache())
+        assert rc == -3 and "same memory" in err, err
