@@ -225,6 +225,7 @@ RDNA_API int32_t rdna_kernel_timer_read(double* total_ms, int64_t* launches);
 #define RDNA_DTYPE_F16 0
 #define RDNA_DTYPE_BF16 1
 #define RDNA_DTYPE_INT8 2
+#define RDNA_DTYPE_F32 3 /* norm weights only */
 
 typedef struct rdna_paged_cache {
     void* key;
@@ -261,6 +262,32 @@ RDNA_API int32_t rdna_paged_append(
     void* query_out, int64_t query_stride_row, int64_t query_stride_h, int64_t query_out_stride_row,
     int64_t query_out_stride_h, uint32_t num_heads, const int32_t* positions, const void* rot_cos,
     const void* rot_sin, uint32_t rot_rows, uint32_t rot_dim, int32_t rot_interleaved, void* hip_stream);
+
+/* What rdna_paged_append_norm does to queries and keys before they are rotated, and by
+ * which positions. */
+typedef struct rdna_paged_norm {
+    const void* query_norm; /* [head_dim] weights, 16-byte aligned, or null */
+    const void* key_norm;
+    const int32_t* rot_axes;  /* [rot_dim / 2], or null: positions has one per row */
+    int64_t position_stride;  /* with rot_axes: of the rows of positions [num_rows, num_axes] */
+    uint32_t num_axes;
+    float eps;
+    int32_t dtype; /* RDNA_DTYPE_* of the weights: F32, or the rows' */
+} rdna_paged_norm;
+
+/* rdna_paged_append, where each head x of the queries (query_norm not null) and of the
+ * keys (key_norm) first becomes x w / sqrt(mean(x^2) + eps), eps at least 0, and column c
+ * of the tables turns by position rot_axes[c] of its row (outside 0 .. num_axes - 1: the
+ * first or last), all in fp32 (of keys that are quantised in fp64) and rounded once.
+ * query may be given without rot_cos and rot_sin where query_norm is.  Rows of no sequence
+ * are not normed.  `norm` is read by the host. */
+RDNA_API int32_t rdna_paged_append_norm(
+    const rdna_paged_cache* cache, const rdna_paged_norm* norm, const void* key, const void* value,
+    int64_t key_stride_row, int64_t key_stride_h, int64_t value_stride_row, int64_t value_stride_h, uint32_t num_rows,
+    int32_t dtype, const void* query, void* query_out, int64_t query_stride_row, int64_t query_stride_h,
+    int64_t query_out_stride_row, int64_t query_out_stride_h, uint32_t num_heads, const int32_t* positions,
+    const void* rot_cos, const void* rot_sin, uint32_t rot_rows, uint32_t rot_dim, int32_t rot_interleaved,
+    void* hip_stream);
 
 /* softmax(scale Q K^T) V of the newest rows over the pages, head_dim a multiple of 32
  * up to 256, query and output fp16 or bf16 (dtype; the pages' own type, or any with

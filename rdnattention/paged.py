@@ -37,6 +37,8 @@ _VP, _I64, _U32, _I32, _F32 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_uint32, 
 # rdna_paged_cache (include/rdnattention_ext.h): 7 pointers, 13 strides, pages,
 # page_size, table_width, num_seqs, num_kv_heads, head_dim, dtype
 _CACHE = struct.Struct("=7Q13q6Ii")
+# rdna_paged_norm: 3 pointers, the positions' row stride, axes, eps, dtype
+_NORM = struct.Struct("=3QqIfi")
 
 _torch = _lib = _device = _raw_stream = None
 _dtypes = None
@@ -67,7 +69,18 @@ def _handle():
     lib.rdna_paged_attention.restype = _I32
     lib.rdna_paged_commit.argtypes = [_VP, _VP, _VP, _I64, _U32, _VP, _VP]
     lib.rdna_paged_commit.restype = _I32
+    for name, args in {"rdna_paged_append_norm": [_VP] + lib.rdna_paged_append.argtypes}.items():
+        if hasattr(lib, name):  # absent from libraries built before it existed
+            getattr(lib, name).argtypes, getattr(lib, name).restype = args, _I32
     return lib
+
+
+def _newer(name):
+    """The library's function `name`, which an older one may lack."""
+    try:
+        return getattr(_lib, name)
+    except AttributeError:
+        raise _ra.RDNAttentionError(f"{_lib._name} has no {name}: rebuild it") from None
 
 
 def _index(name, t, dim, device):
@@ -187,9 +200,41 @@ def _call(device, what, fn, *args):
         raise _ra.RDNAttentionError(f"{what} failed: {_ra.last_error()}")
 
 
+def _norm(query_norm, key_norm, eps, head_dim, dtype, device, rot_axes, cols, axes, stride):
+    """The checked norms of an append and axes of its positions, packed."""
+    torch = _torch
+    code, at = 0, [0, 0]
+    for i, (name, t) in enumerate((("query_norm", query_norm), ("key_norm", key_norm))):
+        if t is None:
+            continue
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name} must be a torch.Tensor")
+        if t.shape != (head_dim,) or t.get_device() != device or t.dtype is not torch.float32 and t.dtype is not dtype:
+            raise ValueError(f"{name} must be a float32 or {dtype} tensor of shape ({head_dim},) on the device of "
+                             f"key_cache, got {t.dtype} {tuple(t.shape)}")
+        if t.stride(0) != 1:
+            raise ValueError(f"{name} must be contiguous")
+        if at[0] and t.dtype is not query_norm.dtype:
+            raise ValueError("query_norm and key_norm must have the same dtype")
+        code = 3 if t.dtype is torch.float32 else _dtypes[dtype]
+        at[i] = t.data_ptr()
+    if not 0.0 <= eps < float("inf"):
+        raise ValueError(f"norm_eps must be finite and not negative, got {eps}")
+    where = 0
+    if rot_axes is not None:
+        if axes is None:
+            raise ValueError("rot_axes needs rot_cos, rot_sin and positions")
+        where, shape, _ = _index("rot_axes", rot_axes, 1, device)
+        if shape[0] != cols:
+            raise ValueError(f"rot_axes must have one entry per column of the tables ({cols}), got {shape[0]}")
+        if not 0 < axes <= 1 << 16:
+            raise ValueError(f"positions must have 1 to 65536 axes, got {axes}")
+    return _NORM.pack(*at, where, stride, axes or 0, eps, code)
+
+
 def paged_append(key, value, key_cache, value_cache, block_tables, seq_lens, *, cu_seqlens_q=None, query=None,
                  positions=None, rot_cos=None, rot_sin=None, rot_interleaved: bool = True, key_scale=None,
-                 value_scale=None):
+                 value_scale=None, query_norm=None, key_norm=None, norm_eps: float = 1e-6, rot_axes=None):
     """Writes a step's keys and values to their places in the pages, in place.
 
     key/value: float16 or bfloat16 [rows, kv_heads, head_dim].  int8 pages get
@@ -204,6 +249,15 @@ def paged_append(key, value, key_cache, value_cache, block_tables, seq_lens, *, 
     (int32 [rows]: drafts of a tree stand side by side in the cache, not in the
     text); indices outside the tables are taken as their first or last row.
 
+    rot_axes: int32 [rot_dim // 2], with positions [rows, axes]: column c turns by
+    the row's position rot_axes[c] (time, height and width of image and video
+    tokens; a number outside the axes is taken as the first or last).
+
+    query_norm/key_norm: [head_dim] weights w (float32 or the rows' type): each
+    head x of the queries or keys first becomes x w / sqrt(mean(x^2) +
+    norm_eps), in the same pass and the same fp32, rounded once with the
+    rotation.  With query_norm, query needs no tables.
+
     query: optional [rows, heads, head_dim]; returned rotated likewise, as a new
     tensor.  Padding rows, and rows without a place (a sequence shorter than
     its rows, a page outside the cache), write nothing.  Returns None without
@@ -216,8 +270,9 @@ def paged_append(key, value, key_cache, value_cache, block_tables, seq_lens, *, 
         key_cache, value_cache, block_tables, seq_lens, "seq_lens", cu_seqlens_q, key_scale, value_scale, rows)
     k, _, ks, dtype = _rows("key", key, rows, kv_heads, head_dim, cache_dtype, None, device)
     v, _, vs, _ = _rows("value", value, rows, kv_heads, head_dim, cache_dtype, dtype, device)
-    cos = sin = pos = q = q_out = out = None
+    cos = sin = pos = q = q_out = out = norm = None
     rot_rows = rot_dim = heads = 0
+    axes, pos_stride = None, 1
     q_st = o_st = (0, 0)
     if rot_cos is not None and rot_sin is not None:
         for name, t in (("rot_cos", rot_cos), ("rot_sin", rot_sin)):
@@ -234,12 +289,14 @@ def paged_append(key, value, key_cache, value_cache, block_tables, seq_lens, *, 
                              f"got {tuple(table_shape)}")
         cos, sin = rot_cos.data_ptr(), rot_sin.data_ptr()
         if positions is not None:
-            pos, pos_shape, _ = _index("positions", positions, 1, device)
+            pos, pos_shape, pos_strides = _index("positions", positions, 1 if rot_axes is None else 2, device)
             if pos_shape[0] != rows:
                 raise ValueError(f"positions must have one entry per row ({rows}), got {pos_shape[0]}")
+            if rot_axes is not None:
+                axes, pos_stride = pos_shape[1], pos_strides[0]
     elif rot_cos is not None or rot_sin is not None:
         raise ValueError("pass both rot_cos and rot_sin, or neither")
-    elif query is not None or positions is not None:
+    elif query is not None and query_norm is None or positions is not None:
         raise ValueError("query and positions need rot_cos and rot_sin")
     if query is not None:
         q, (_, heads, _), q_st, _ = _rows("query", query, rows, None, head_dim, cache_dtype, dtype, device)
@@ -248,13 +305,21 @@ def paged_append(key, value, key_cache, value_cache, block_tables, seq_lens, *, 
             q = None
         else:
             q_out, o_st = out.data_ptr(), out.stride()
+    elif query_norm is not None:
+        raise ValueError("query_norm needs query")
+    if query_norm is not None or key_norm is not None or rot_axes is not None:
+        norm = _norm(query_norm if query is None or heads else None, key_norm, norm_eps, head_dim, dtype, device, rot_axes,
+                     rot_dim // 2, axes, pos_stride)
     if rows == 0:
         return out
     if seqs == 0:  # nothing but padding
         return out.copy_(query) if out is not None else None
-    _call(device, "paged_append", _lib.rdna_paged_append, c, k, v, ks[0], ks[1], vs[0], vs[1], rows, _dtypes[dtype], q,
-          q_out, q_st[0], q_st[1], o_st[0], o_st[1], heads, pos, cos, sin, rot_rows, rot_dim,
-          1 if rot_interleaved else 0)
+    rows_args = (k, v, ks[0], ks[1], vs[0], vs[1], rows, _dtypes[dtype], q, q_out, q_st[0], q_st[1], o_st[0], o_st[1],
+                 heads, pos, cos, sin, rot_rows, rot_dim, 1 if rot_interleaved else 0)
+    if norm is None:
+        _call(device, "paged_append", _lib.rdna_paged_append, c, *rows_args)
+    else:
+        _call(device, "paged_append", _newer("rdna_paged_append_norm"), c, norm, *rows_args)
     return out
 
 

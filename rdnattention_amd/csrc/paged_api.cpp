@@ -179,13 +179,59 @@ bool no_int8(const rdna_paged_cache* c, const char* fmt) {
 
 } // namespace
 
-RDNA_API int32_t rdna_paged_append(const rdna_paged_cache* cache, const void* key, const void* value,
-                                   int64_t key_stride_row, int64_t key_stride_h, int64_t value_stride_row,
-                                   int64_t value_stride_h, uint32_t num_rows, int32_t dtype, const void* query,
-                                   void* query_out, int64_t query_stride_row, int64_t query_stride_h,
-                                   int64_t query_out_stride_row, int64_t query_out_stride_h, uint32_t num_heads,
-                                   const int32_t* positions, const void* rot_cos, const void* rot_sin,
-                                   uint32_t rot_rows, uint32_t rot_dim, int32_t rot_interleaved, void* hip_stream) {
+namespace {
+
+// The norms of an append into `n`; "" or what is wrong.
+std::string check_norm(const rdna_paged_norm* in, const void* query, const int32_t* positions, const void* rot_cos,
+                       uint32_t num_rows, int32_t dtype, rdna_amd::PagedNorm& n) {
+    using rdna_amd::PagedNormType;
+    if (in->query_norm != nullptr && query == nullptr) {
+        return "query_norm without query";
+    }
+    if (in->query_norm != nullptr || in->key_norm != nullptr) {
+        if (in->dtype != RDNA_DTYPE_F32 && in->dtype != dtype) {
+            return "norm weights must be fp32 or of the rows' type";
+        }
+        if (!aligned(in->query_norm, 16) || !aligned(in->key_norm, 16)) {
+            return "norm weights must be 16-byte aligned";
+        }
+        if (!(in->eps >= 0.0f) || !std::isfinite(in->eps)) {
+            return "eps must be finite and not negative";
+        }
+    }
+    if (in->rot_axes != nullptr) {
+        if (positions == nullptr || rot_cos == nullptr) {
+            return "rot_axes needs positions, rot_cos and rot_sin";
+        }
+        if (!aligned(in->rot_axes, 4)) {
+            return "rot_axes must be an aligned int32 array";
+        }
+        if (in->num_axes == 0 || in->num_axes > (1u << 16)) {
+            return "num_axes must be 1 to 2^16";
+        }
+        if (!stride_fits(in->position_stride, 4, num_rows)) {
+            return "position_stride must not be negative, and stay within 2^56 bytes";
+        }
+        n.rot_axes = in->rot_axes;
+        n.position_s = in->position_stride;
+        n.axes = (int32_t)in->num_axes;
+    }
+    n.query = in->query_norm;
+    n.key = in->key_norm;
+    n.type = in->dtype == RDNA_DTYPE_F32 ? PagedNormType::F32
+             : dtype == RDNA_DTYPE_F16   ? PagedNormType::F16
+                                         : PagedNormType::BF16;
+    n.eps = in->eps;
+    return "";
+}
+
+// rdna_paged_append, with norms where `norm` is not null.
+int32_t append(const rdna_paged_norm* norm, const rdna_paged_cache* cache, const void* key, const void* value,
+               int64_t key_stride_row, int64_t key_stride_h, int64_t value_stride_row, int64_t value_stride_h,
+               uint32_t num_rows, int32_t dtype, const void* query, void* query_out, int64_t query_stride_row,
+               int64_t query_stride_h, int64_t query_out_stride_row, int64_t query_out_stride_h, uint32_t num_heads,
+               const int32_t* positions, const void* rot_cos, const void* rot_sin, uint32_t rot_rows, uint32_t rot_dim,
+               int32_t rot_interleaved, void* hip_stream) {
 #if defined(RDNATTENTION_NO_INT8)
     if (no_int8(cache, "Paged append unavailable: %s")) {
         return -4;
@@ -214,7 +260,8 @@ RDNA_API int32_t rdna_paged_append(const rdna_paged_cache* cache, const void* ke
             err = std::string("row ") + kStrides;
         } else if ((rot_cos == nullptr) != (rot_sin == nullptr)) {
             err = "pass both rot_cos and rot_sin, or neither";
-        } else if (rot_cos == nullptr && (query != nullptr || positions != nullptr)) {
+        } else if (rot_cos == nullptr &&
+                   ((query != nullptr && (norm == nullptr || norm->query_norm == nullptr)) || positions != nullptr)) {
             err = "query and positions need rot_cos and rot_sin";
         } else if (!aligned(rot_cos, 16) || !aligned(rot_sin, 16) || !aligned(positions, 4)) {
             err = "rot_cos and rot_sin must be 16-byte aligned, positions 4-byte aligned";
@@ -244,6 +291,10 @@ RDNA_API int32_t rdna_paged_append(const rdna_paged_cache* cache, const void* ke
         } else if (err.empty() && a.c.k == a.c.v) {
             err = kShared;
         }
+        rdna_amd::PagedNorm n;
+        if (err.empty() && norm != nullptr) {
+            err = check_norm(norm, query, positions, rot_cos, num_rows, dtype, n);
+        }
         if (!err.empty()) {
             return -1;
         }
@@ -257,9 +308,40 @@ RDNA_API int32_t rdna_paged_append(const rdna_paged_cache* cache, const void* ke
         a.rot = rot_cos != nullptr ? (int32_t)rot_dim : 0;
         a.rot_rows = (int32_t)rot_rows;
         a.interleaved = rot_interleaved != 0 ? 1 : 0;
-        return rdna_amd::paged_append(a, static_cast<hipStream_t>(hip_stream), err);
+        const hipStream_t stream = static_cast<hipStream_t>(hip_stream);
+        return norm != nullptr ? rdna_amd::paged_append_norm(a, n, stream, err)
+                               : rdna_amd::paged_append(a, stream, err);
     });
 }
+
+} // namespace
+
+RDNA_API int32_t rdna_paged_append(const rdna_paged_cache* cache, const void* key, const void* value,
+                                   int64_t key_stride_row, int64_t key_stride_h, int64_t value_stride_row,
+                                   int64_t value_stride_h, uint32_t num_rows, int32_t dtype, const void* query,
+                                   void* query_out, int64_t query_stride_row, int64_t query_stride_h,
+                                   int64_t query_out_stride_row, int64_t query_out_stride_h, uint32_t num_heads,
+                                   const int32_t* positions, const void* rot_cos, const void* rot_sin,
+                                   uint32_t rot_rows, uint32_t rot_dim, int32_t rot_interleaved, void* hip_stream) {
+    return append(nullptr, cache, key, value, key_stride_row, key_stride_h, value_stride_row, value_stride_h, num_rows,
+                  dtype, query, query_out, query_stride_row, query_stride_h, query_out_stride_row, query_out_stride_h,
+                  num_heads, positions, rot_cos, rot_sin, rot_rows, rot_dim, rot_interleaved, hip_stream);
+}
+
+RDNA_API int32_t rdna_paged_append_norm(
+    const rdna_paged_cache* cache, const rdna_paged_norm* norm, const void* key, const void* value,
+    int64_t key_stride_row, int64_t key_stride_h, int64_t value_stride_row, int64_t value_stride_h, uint32_t num_rows,
+    int32_t dtype, const void* query, void* query_out, int64_t query_stride_row, int64_t query_stride_h,
+    int64_t query_out_stride_row, int64_t query_out_stride_h, uint32_t num_heads, const int32_t* positions,
+    const void* rot_cos, const void* rot_sin, uint32_t rot_rows, uint32_t rot_dim, int32_t rot_interleaved,
+    void* hip_stream) {
+    static const rdna_paged_norm none = {};
+    return append(norm != nullptr ? norm : &none, cache, key, value, key_stride_row, key_stride_h, value_stride_row,
+                  value_stride_h, num_rows, dtype, query, query_out, query_stride_row, query_stride_h,
+                  query_out_stride_row, query_out_stride_h, num_heads, positions, rot_cos, rot_sin, rot_rows, rot_dim,
+                  rot_interleaved, hip_stream);
+}
+
 
 RDNA_API int32_t rdna_paged_attention(const rdna_paged_cache* cache, const void* query, void* output,
                                       int64_t query_stride_row, int64_t query_stride_h, int64_t output_stride_row,

@@ -61,6 +61,20 @@ struct PagedAppendArgs {
 };
 int paged_append(const PagedAppendArgs& a, hipStream_t stream, std::string& err);
 
+// Norms of an append's queries and keys (weights [D], either may be null), and
+// positions of several axes: column c of the tables turns by the row's position
+// rot_axes[c] of `axes`, position i of row t at positions[t * position_s + i].
+enum class PagedNormType : int32_t { F16 = 0, BF16 = 1, F32 = 2 };
+struct PagedNorm {
+    const void *query = nullptr, *key = nullptr;
+    PagedNormType type = PagedNormType::F32;
+    float eps = 0.0f;
+    const int32_t* rot_axes = nullptr;
+    int64_t position_s = 1;
+    int32_t axes = 1;
+};
+int paged_append_norm(const PagedAppendArgs& a, const PagedNorm& n, hipStream_t stream, std::string& err);
+
 struct PagedCommitArgs {
     PagedPages c;
     bool i8 = false;
