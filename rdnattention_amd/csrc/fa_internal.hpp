@@ -31,7 +31,7 @@ constexpr size_t region_bytes(size_t bytes) {
 
 // What a scratch buffer holds; calls keep one cached buffer per (device,
 // stream, purpose), so buffers of one call never alias.
-enum class ScratchUse : int { RotatedK = 0, SplitKPartials = 1, QuantPartials = 2, Int8Scores = 3, PagedPartials = 4 };
+enum class ScratchUse : int { RotatedK = 0, SplitKPartials = 1, QuantPartials = 2, Int8Scores = 3, PagedPartials = 4, PagedPrefix = 5 };
 
 // Scratch memory for one call (scratch.cpp).  Without a region: the buffer
 // cached for (device, stream, use); a call that finds it large enough makes
@@ -40,9 +40,10 @@ enum class ScratchUse : int { RotatedK = 0, SplitKPartials = 1, QuantPartials = 
 // use.  Growth replaces the buffer with hipMallocAsync after releasing the
 // old one with hipFreeAsync in the stream's order; the cached bytes of a
 // device are capped, with idle entries evicted least recently used first;
-// buffers above 256 MiB, calls under graph capture and a second host thread
-// that finds the buffer in use take a per-call default-pool block
-// (hipMallocAsync / hipFreeAsync).  No path here waits on the host.
+// buffers above 256 MiB and a second host thread that finds the buffer in use
+// take a per-call default-pool block (hipMallocAsync / hipFreeAsync).  No path
+// here waits on the host.  A call under graph capture takes a block that its graph
+// owns until it is destroyed, shared by the calls of that capture on that stream.
 // With a region: carved from it, nothing allocated or freed (the caller has
 // checked that it fits).
 // alloc: 0, or with `err` kScratchFull when the device has no memory left (a
@@ -55,6 +56,7 @@ struct StreamScratch {
     ScratchUse use;
     bool cached = false; // ptr is the (device, stream, use) cache entry's buffer
     bool pooled = false; // ptr is a per-call hipMallocAsync block
+    void* graph = nullptr; // the block of the graph that is being captured
     int device = 0;
     explicit StreamScratch(ScratchUse u, ScratchRegion* r = nullptr) : region(r), use(u) {}
     int alloc(size_t bytes, hipStream_t s, std::string& err);

@@ -16,7 +16,12 @@
 //     after their own last use (hipStreamWaitEvent on the event recorded
 //     after it), and a call that still does not fit takes a per-call
 //     default-pool block instead;
-//   * buffers above kEntryMax are never cached, only taken per call.
+//   * buffers above kEntryMax are never cached, only taken per call;
+//   * a captured call takes a block that its graph owns (GraphBlock) until the graph
+//     and its executables are destroyed.  A memory node (hipMallocAsync under
+//     capture) will not do: the runtime gives the nodes of one graph the
+//     addresses of another's, so that two graphs replayed side by side on two streams
+//     use one buffer, and the records read from it lead anywhere.
 // rdna_scratch_trim() (the one synchronising path) frees every idle entry and
 // returns the default pool's free blocks to the device.
 #include "fa_internal.hpp"
@@ -28,7 +33,9 @@
 #include <map>
 #include <mutex>
 #include <string>
+#include <tuple>
 #include <utility>
+#include <vector>
 
 namespace rdna_amd {
 namespace {
@@ -66,6 +73,116 @@ int alloc_failed(hipError_t e, std::string& err) {
     (void)hipGetLastError();
     err = hip_err("scratch allocation failed", e);
     return e == hipErrorOutOfMemory ? kScratchFull : -1;
+}
+
+// A captured call's scratch.  The calls that one capture makes on one stream run in turn
+// and share a block per use, as eager calls share the stream's; the graph holds it by a
+// user object, whose destructor hands it back for later captures.
+struct GraphBlock {
+    using Key = std::tuple<unsigned long long, hipStream_t, int>; // capture, stream, use
+    Key key;
+    void* ptr = nullptr;
+    size_t bytes = 0;
+    int device = 0;
+    bool busy = false; // a call of the capture holds it
+};
+struct GraphBlocks {
+    std::mutex mu;
+    std::map<GraphBlock::Key, GraphBlock*> held; // of each key the last
+    std::vector<GraphBlock*> free;
+};
+// Never destroyed: a graph may outlive the library's static objects.
+GraphBlocks& graph_blocks() {
+    static auto* const blocks = new GraphBlocks;
+    return *blocks;
+}
+
+// User object's destructor: no HIP calls here.
+void graph_block_released(void* p) {
+    GraphBlocks& g = graph_blocks();
+    auto* const b = static_cast<GraphBlock*>(p);
+    std::lock_guard<std::mutex> lock(g.mu);
+    const auto it = g.held.find(b->key);
+    if (it != g.held.end() && it->second == b) {
+        g.held.erase(it);
+    }
+    b->busy = false;
+    g.free.push_back(b);
+}
+
+// A block of at least `bytes` for a call that stream s captures.  0, or what
+// StreamScratch::alloc returns.
+int graph_block(size_t bytes, hipStream_t s, int use, int device, GraphBlock*& out, bool& allocated,
+                std::string& err) {
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    unsigned long long id = 0;
+    hipGraph_t graph = nullptr;
+    const hipGraphNode_t* deps = nullptr;
+    size_t n_deps = 0;
+    hipError_t e = hipStreamGetCaptureInfo_v2(s, &status, &id, &graph, &deps, &n_deps);
+    if (e != hipSuccess || graph == nullptr) {
+        err = hip_err("scratch allocation under capture failed", e != hipSuccess ? e : hipErrorStreamCaptureInvalidated);
+        return -1;
+    }
+    GraphBlocks& g = graph_blocks();
+    GraphBlock* b = nullptr;
+    {
+        std::lock_guard<std::mutex> lock(g.mu);
+        const auto it = g.held.find({id, s, use});
+        if (it != g.held.end() && !it->second->busy && it->second->bytes >= bytes && it->second->device == device) {
+            out = it->second;
+            out->busy = true;
+            return 0;
+        }
+        auto best = g.free.end();
+        for (auto f = g.free.begin(); f != g.free.end(); ++f) {
+            if ((*f)->device == device && (*f)->bytes >= bytes && (best == g.free.end() || (*f)->bytes < (*best)->bytes)) {
+                best = f;
+            }
+        }
+        if (best != g.free.end()) {
+            b = *best;
+            g.free.erase(best);
+        }
+    }
+    if (b == nullptr) {
+        void* ptr = nullptr;
+        const size_t want = (bytes + kGranule - 1) / kGranule * kGranule;
+        hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed; // hipMalloc is no part of the capture
+        e = hipThreadExchangeStreamCaptureMode(&mode);
+        if (e == hipSuccess) {
+            e = hipMalloc(&ptr, want);
+            (void)hipThreadExchangeStreamCaptureMode(&mode);
+        }
+        if (e != hipSuccess) {
+            return alloc_failed(e, err);
+        }
+        allocated = true;
+        b = new GraphBlock;
+        b->ptr = ptr;
+        b->bytes = want;
+        b->device = device;
+    }
+    b->key = {id, s, use};
+    b->busy = true;
+    hipUserObject_t owner = nullptr;
+    e = hipUserObjectCreate(&owner, b, graph_block_released, 1, hipUserObjectNoDestructorSync);
+    if (e != hipSuccess) {
+        graph_block_released(b);
+    } else {
+        e = hipGraphRetainUserObject(graph, owner, 1, hipGraphUserObjectMove);
+        if (e != hipSuccess) {
+            (void)hipUserObjectRelease(owner, 1); // hands the block back
+        }
+    }
+    if (e != hipSuccess) {
+        err = hip_err("scratch allocation under capture failed", e);
+        return -1;
+    }
+    std::lock_guard<std::mutex> lock(g.mu);
+    g.held[b->key] = b;
+    out = b;
+    return 0;
 }
 
 // Releases e's buffer in the order of stream s: after the work recorded in
@@ -109,14 +226,27 @@ int StreamScratch::alloc(size_t bytes, hipStream_t s, std::string& err) {
         err = hip_err("scratch allocation failed", e);
         return -1;
     }
-    // Under graph capture the allocation becomes a memory node the graph owns.
     hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
     e = hipStreamIsCapturing(s, &capture);
     if (e != hipSuccess) {
         err = hip_err("scratch allocation failed", e);
         return -1;
     }
-    bool per_call = capture != hipStreamCaptureStatusNone || bytes > kEntryMax;
+    if (capture != hipStreamCaptureStatusNone) {
+        GraphBlock* b = nullptr;
+        bool allocated = false;
+        const int rc = graph_block(bytes, s, static_cast<int>(use), device, b, allocated, err);
+        if (allocated) {
+            std::lock_guard<std::mutex> lock(g_mu);
+            g_devices[device].allocations++;
+        }
+        if (rc == 0) {
+            graph = b;
+            ptr = b->ptr;
+        }
+        return rc;
+    }
+    bool per_call = bytes > kEntryMax;
     if (!per_call) {
         std::lock_guard<std::mutex> lock(g_mu);
         DeviceCache& dc = g_devices[device];
@@ -219,10 +349,23 @@ StreamScratch::~StreamScratch() {
         ent.busy = false;
     } else if (pooled && ptr != nullptr) {
         (void)hipFreeAsync(ptr, stream);
+    } else if (graph != nullptr) {
+        std::lock_guard<std::mutex> lock(graph_blocks().mu);
+        static_cast<GraphBlock*>(graph)->busy = false;
     }
 }
 
 int scratch_trim(std::string& err) {
+    // blocks of graphs that are gone
+    std::vector<GraphBlock*> blocks;
+    {
+        std::lock_guard<std::mutex> lock(graph_blocks().mu);
+        blocks.swap(graph_blocks().free);
+    }
+    for (GraphBlock* b : blocks) {
+        (void)hipFree(b->ptr);
+        delete b;
+    }
     std::lock_guard<std::mutex> lock(g_mu);
     if (g_devices.empty()) {
         return 0; // nothing cached, no HIP call needed
