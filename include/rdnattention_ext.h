@@ -33,8 +33,8 @@ RDNA_API int32_t rdna_attention_forward_path(
  * buffers (RoPE-rotated K copies, split-K and paged partials, quantiser
  * partials, INT8 decode scores) it caches per (device, stream, use), grown to the largest
  * call so far (at most 256 MiB each, at most 1 GiB per device over all
- * streams and uses), and the free blocks of the devices' default memory
- * pools.  A call never frees or
+ * streams and uses), the scratch of captured graphs that have been destroyed,
+ * and the free blocks of the devices' default memory pools.  A call never frees or
  * allocates scratch on the host's time: a cached buffer large enough is
  * reused with no allocator call; growth and eviction are stream-ordered
  * (hipFreeAsync / hipMallocAsync).  This trim is the one synchronising path:
@@ -309,6 +309,31 @@ RDNA_API int32_t rdna_paged_attention(
     int64_t output_stride_row, int64_t output_stride_h, uint32_t num_rows, uint32_t num_heads, int32_t dtype,
     uint32_t max_rows_per_seq, float scale, int32_t causal, int32_t window_size, const uint8_t* tree_mask,
     int64_t tree_stride_seq, int64_t tree_stride_row, uint32_t tree_n, int32_t zero_tail, void* hip_stream);
+
+/* Prefixes that sequences share, in the pages of the same cache: the first lens[i] keys
+ * of table row i come before the own keys of sequences seqs[i] .. seqs[i + 1] - 1 (seqs
+ * [num_prefixes + 1], from 0 to the number of sequences and never falling; null: one
+ * prefix, of all of them).  All of it device memory that the host does not read; a
+ * length of 0 is no prefix. */
+typedef struct rdna_paged_prefix {
+    const int32_t* block_tables; /* [num_prefixes, table_width] */
+    const int32_t* lens;         /* [num_prefixes] */
+    const int32_t* seqs;
+    int64_t table_stride;
+    uint32_t table_width, num_prefixes;
+} rdna_paged_prefix;
+
+/* rdna_paged_attention of rows that see their sequence's prefix too (prefix not null):
+ * all of it, whatever causal hides of the sequence's own keys; without window_size.  A
+ * prefix is read once for all of its sequences.  lse, if not null: float [num_rows,
+ * num_heads], the logarithm of the sum of exp(score) over the keys that a row sees, -inf
+ * where there is none; of the rows behind the last sequence (where cu_seqlens is given)
+ * -inf whether or not zero_tail is set. */
+RDNA_API int32_t rdna_paged_attention_lse(
+    const rdna_paged_cache* cache, const rdna_paged_prefix* prefix, const void* query, void* output,
+    int64_t query_stride_row, int64_t query_stride_h, int64_t output_stride_row, int64_t output_stride_h,
+    uint32_t num_rows, uint32_t num_heads, int32_t dtype, uint32_t max_rows_per_seq, float scale, int32_t causal,
+    int32_t window_size, int32_t zero_tail, float* lse, void* hip_stream);
 
 /* Keeps accepted drafts: for every sequence, key and value prefix_lens[b] + i become
  * those of prefix_lens[b] + path[b * path_stride + i], i < path_lens[b] (at most

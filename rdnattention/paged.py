@@ -39,6 +39,8 @@ _VP, _I64, _U32, _I32, _F32 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_uint32, 
 _CACHE = struct.Struct("=7Q13q6Ii")
 # rdna_paged_norm: 3 pointers, the positions' row stride, axes, eps, dtype
 _NORM = struct.Struct("=3QqIfi")
+# rdna_paged_prefix: 3 pointers, the table's row stride, its width, prefixes
+_PREFIX = struct.Struct("=3Qq2I")
 
 _torch = _lib = _device = _raw_stream = None
 _dtypes = None
@@ -69,7 +71,10 @@ def _handle():
     lib.rdna_paged_attention.restype = _I32
     lib.rdna_paged_commit.argtypes = [_VP, _VP, _VP, _I64, _U32, _VP, _VP]
     lib.rdna_paged_commit.restype = _I32
-    for name, args in {"rdna_paged_append_norm": [_VP] + lib.rdna_paged_append.argtypes}.items():
+    newer = {"rdna_paged_append_norm": [_VP] + lib.rdna_paged_append.argtypes,
+             "rdna_paged_attention_lse": ([_VP] * 4 + [_I64] * 4 + [_U32, _U32, _I32, _U32, _F32, _I32, _I32, _I32, _VP,
+                                                                    _VP])}
+    for name, args in newer.items():
         if hasattr(lib, name):  # absent from libraries built before it existed
             getattr(lib, name).argtypes, getattr(lib, name).restype = args, _I32
     return lib
@@ -323,8 +328,24 @@ def paged_append(key, value, key_cache, value_cache, block_tables, seq_lens, *, 
     return out
 
 
+def _prefix(tables, lens, seqs, device):
+    """The checked prefixes, packed."""
+    table, (n, width), stride = _index("prefix_tables", tables, 2, device)
+    at, shape, _ = _index("prefix_lens", lens, 1, device)
+    if n == 0 or shape[0] != n:
+        raise ValueError(f"prefix_lens must have one entry per row of prefix_tables ({n}, at least one), got {shape[0]}")
+    of = 0
+    if seqs is not None:
+        of, shape, _ = _index("prefix_seqs", seqs, 1, device)
+        if shape[0] != n + 1:
+            raise ValueError(f"prefix_seqs must have {n + 1} entries, got {shape[0]}")
+    elif n != 1:
+        raise ValueError(f"{n} prefixes need prefix_seqs")
+    return _PREFIX.pack(table, at, of, stride[0], width, n)
+
+
 def _attend(what, query, key_cache, value_cache, block_tables, seq_lens, cu_seqlens_q, max_seqlen_q, is_causal,
-            window_size, scale, tree_mask, key_scale, value_scale, out):
+            window_size, scale, tree_mask, key_scale, value_scale, out, return_lse=False, prefix=None):
     torch = _torch or _init()
     if not isinstance(query, torch.Tensor):
         raise TypeError("query must be a torch.Tensor")
@@ -358,20 +379,29 @@ def _attend(what, query, key_cache, value_cache, block_tables, seq_lens, cu_seql
     else:
         zero_tail = 0
         o, _, os_, _ = _rows("out", out, rows, heads, head_dim, cache_dtype, dtype, device)
+    if prefix is not None:
+        prefix = _prefix(*prefix, device)
+    lse = torch.empty(rows, heads, dtype=torch.float32, device=query.device) if return_lse else None
     if rows == 0 or heads == 0:
-        return out
+        return (out, lse) if return_lse else out
     if seqs == 0:  # nothing but padding
-        return out.zero_() if zero_tail else out
+        out = out.zero_() if zero_tail else out
+        return (out, lse.fill_(float("-inf"))) if return_lse else out
     most = rows if max_seqlen_q is None else max(0, min(rows, int(max_seqlen_q)))
-    _call(device, what, _lib.rdna_paged_attention, c, q, o, qs[0], qs[1], os_[0], os_[1], rows, heads, _dtypes[dtype],
-          most, head_dim ** -0.5 if scale is None else float(scale), 1 if is_causal else 0,
-          max(-1, min(int(window_size), 2 ** 31 - 1)), tree, t_sb, t_sr, t_n, zero_tail)
+    args = (q, o, qs[0], qs[1], os_[0], os_[1], rows, heads, _dtypes[dtype], most,
+            head_dim ** -0.5 if scale is None else float(scale), 1 if is_causal else 0,
+            max(-1, min(int(window_size), 2 ** 31 - 1)))
+    if return_lse or prefix is not None:
+        _call(device, what, _newer("rdna_paged_attention_lse"), c, prefix, *args, zero_tail,
+              lse.data_ptr() if return_lse else None)
+        return (out, lse) if return_lse else out
+    _call(device, what, _lib.rdna_paged_attention, c, *args, tree, t_sb, t_sr, t_n, zero_tail)
     return out
 
 
 def paged_attention(query, key_cache, value_cache, block_tables, seq_lens, *, cu_seqlens_q=None, max_seqlen_q=None,
                     is_causal: bool = True, window_size: int = -1, scale=None, key_scale=None, value_scale=None,
-                    out=None):
+                    out=None, return_lse: bool = False):
     """Attention of each sequence's newest rows over its pages: single tokens,
     chunks of a prompt, whole prompts, or all of them in one ragged batch.
 
@@ -385,9 +415,31 @@ def paged_attention(query, key_cache, value_cache, block_tables, seq_lens, *, cu
     multiplied too, so others may reach rows that do not see them.
 
     out: optional tensor like query to write to, whose padding rows stay as they
-    are; a new tensor's are zeros.  Returns the output."""
+    are; a new tensor's are zeros.  Returns the output, with return_lse (output,
+    lse): float32 [rows, heads], the logarithm of the sum of exp(score) over the
+    keys that the row sees, -inf where it sees none and of padding rows."""
     return _attend("paged_attention", query, key_cache, value_cache, block_tables, seq_lens, cu_seqlens_q, max_seqlen_q,
-                   is_causal, window_size, scale, None, key_scale, value_scale, out)
+                   is_causal, window_size, scale, None, key_scale, value_scale, out, return_lse)
+
+
+def paged_prefix_attention(query, key_cache, value_cache, prefix_tables, prefix_lens, block_tables, seq_lens, *,
+                           prefix_seqs=None, cu_seqlens_q=None, max_seqlen_q=None, is_causal: bool = True, scale=None,
+                           key_scale=None, value_scale=None, out=None, return_lse: bool = False):
+    """Attention of sequences that share prefixes: an instruction text, a document,
+    the prompt of several samples.
+
+    Row i of prefix_tables (int32 [prefixes, width]) lists the pages of a prefix,
+    prefix_lens (int32 [prefixes]) counts its keys, and sequences prefix_seqs[i] ..
+    prefix_seqs[i + 1] - 1 follow it: prefix_seqs (int32 [prefixes + 1]) begins with
+    0, never falls and ends with the number of sequences; without it there is one
+    prefix, of all of them.  block_tables and seq_lens are of the sequences' own
+    keys alone, all else as in paged_attention: every row sees the whole prefix,
+    and its own keys as is_causal says.  Each prefix is read once for all of its
+    sequences.  A length of 0 is no prefix.  (A position in the text is the
+    prefix's length more than the row's index: paged_append's positions.)"""
+    return _attend("paged_prefix_attention", query, key_cache, value_cache, block_tables, seq_lens, cu_seqlens_q,
+                   max_seqlen_q, is_causal, -1, scale, None, key_scale, value_scale, out, return_lse,
+                   (prefix_tables, prefix_lens, prefix_seqs))
 
 
 def paged_tree_attention(query, key_cache, value_cache, block_tables, seq_lens, tree_mask, *, cu_seqlens_q=None,

@@ -343,12 +343,41 @@ RDNA_API int32_t rdna_paged_append_norm(
 }
 
 
-RDNA_API int32_t rdna_paged_attention(const rdna_paged_cache* cache, const void* query, void* output,
-                                      int64_t query_stride_row, int64_t query_stride_h, int64_t output_stride_row,
-                                      int64_t output_stride_h, uint32_t num_rows, uint32_t num_heads, int32_t dtype,
-                                      uint32_t max_rows_per_seq, float scale, int32_t causal, int32_t window_size,
-                                      const uint8_t* tree_mask, int64_t tree_stride_seq, int64_t tree_stride_row,
-                                      uint32_t tree_n, int32_t zero_tail, void* hip_stream) {
+namespace {
+
+// The prefixes into `p`; "" or what is wrong.
+std::string check_prefix(const rdna_paged_prefix* in, const rdna_paged_cache* cache, rdna_amd::PagedPrefix& p) {
+    if (in->num_prefixes == 0 || in->num_prefixes > (1u << 24)) {
+        return "num_prefixes must be 1 to 2^24";
+    }
+    if (in->seqs == nullptr && in->num_prefixes != 1) {
+        return "several prefixes need seqs";
+    }
+    if ((uint64_t)in->table_width * cache->page_size > (uint64_t)kPagedMaxLen) {
+        return "the prefixes' page table covers more than 2^28 keys";
+    }
+    if (in->lens == nullptr || (in->block_tables == nullptr && in->table_width != 0)) {
+        return "null prefix pointer";
+    }
+    if (!aligned(in->lens, 4) || !aligned(in->seqs, 4) || !aligned(in->block_tables, 4) ||
+        !stride_fits(in->table_stride, 4, in->num_prefixes)) {
+        return "the prefixes' lens, seqs and block_tables must be aligned int32 arrays, with a row stride that is not "
+               "negative and stays within 2^56 bytes";
+    }
+    p.table = in->block_tables;
+    p.lens = in->lens;
+    p.seqs = in->seqs;
+    p.table_s = in->table_stride;
+    p.width = (int32_t)in->table_width;
+    p.n = (int32_t)in->num_prefixes;
+    return "";
+}
+
+int32_t attention(const rdna_paged_cache* cache, const rdna_paged_prefix* prefix, const void* query, void* output,
+                  int64_t query_stride_row, int64_t query_stride_h, int64_t output_stride_row, int64_t output_stride_h,
+                  uint32_t num_rows, uint32_t num_heads, int32_t dtype, uint32_t max_rows_per_seq, float scale,
+                  int32_t causal, int32_t window_size, const uint8_t* tree_mask, int64_t tree_stride_seq,
+                  int64_t tree_stride_row, uint32_t tree_n, int32_t zero_tail, float* lse, void* hip_stream) {
 #if defined(RDNATTENTION_NO_INT8)
     if (no_int8(cache, "Paged attention unavailable: %s")) {
         return -4;
@@ -387,6 +416,13 @@ RDNA_API int32_t rdna_paged_attention(const rdna_paged_cache* cache, const void*
                    (tree_n == 0 || tree_n > (uint32_t)kPagedMaxLen ||
                     !stride_fits(tree_stride_seq, 1, cache->num_seqs) || !stride_fits(tree_stride_row, 1, tree_n))) {
             err = "tree_n must be 1 to 2^28, the mask's strides not negative and within 2^56 bytes";
+        } else if (!aligned(lse, 4)) {
+            err = "lse must be an aligned float array";
+        } else if (prefix != nullptr && window_size > 0) {
+            err = "a prefix goes without window_size";
+        }
+        if (err.empty() && prefix != nullptr) {
+            err = check_prefix(prefix, cache, a.prefix);
         }
         if (!err.empty()) {
             return -1;
@@ -405,9 +441,35 @@ RDNA_API int32_t rdna_paged_attention(const rdna_paged_cache* cache, const void*
         a.tree_sb = tree_stride_seq;
         a.tree_sr = tree_stride_row;
         a.tree_n = (int32_t)tree_n;
+        a.lse = lse;
         return rdna_amd::paged_attention(a, static_cast<hipStream_t>(hip_stream), err);
     });
 }
+
+} // namespace
+
+RDNA_API int32_t rdna_paged_attention(const rdna_paged_cache* cache, const void* query, void* output,
+                                      int64_t query_stride_row, int64_t query_stride_h, int64_t output_stride_row,
+                                      int64_t output_stride_h, uint32_t num_rows, uint32_t num_heads, int32_t dtype,
+                                      uint32_t max_rows_per_seq, float scale, int32_t causal, int32_t window_size,
+                                      const uint8_t* tree_mask, int64_t tree_stride_seq, int64_t tree_stride_row,
+                                      uint32_t tree_n, int32_t zero_tail, void* hip_stream) {
+    return attention(cache, nullptr, query, output, query_stride_row, query_stride_h, output_stride_row,
+                     output_stride_h, num_rows, num_heads, dtype, max_rows_per_seq, scale, causal, window_size,
+                     tree_mask, tree_stride_seq, tree_stride_row, tree_n, zero_tail, nullptr, hip_stream);
+}
+
+RDNA_API int32_t rdna_paged_attention_lse(const rdna_paged_cache* cache, const rdna_paged_prefix* prefix,
+                                          const void* query, void* output, int64_t query_stride_row,
+                                          int64_t query_stride_h, int64_t output_stride_row, int64_t output_stride_h,
+                                          uint32_t num_rows, uint32_t num_heads, int32_t dtype,
+                                          uint32_t max_rows_per_seq, float scale, int32_t causal, int32_t window_size,
+                                          int32_t zero_tail, float* lse, void* hip_stream) {
+    return attention(cache, prefix, query, output, query_stride_row, query_stride_h, output_stride_row,
+                     output_stride_h, num_rows, num_heads, dtype, max_rows_per_seq, scale, causal, window_size, nullptr,
+                     0, 0, 0, zero_tail, lse, hip_stream);
+}
+
 
 RDNA_API int32_t rdna_paged_commit(const rdna_paged_cache* cache, const int32_t* prefix_lens, const int32_t* path,
                                    int64_t path_stride, uint32_t path_n, const int32_t* path_lens,

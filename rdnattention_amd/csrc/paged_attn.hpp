@@ -38,6 +38,21 @@ struct PagedRecord {
     int32_t unused[3];
 };
 
+// Rows whose keys are in two parts, and log-sum-exps; rows of D channels by row * Hq +
+// head.
+struct PagedJoin {
+    float* raw_o;       // not null: O in fp32 and the log-sum-exp in log2 units go here,
+    float* raw_l;       // -inf of a row that sees no key, and no output is written
+    const float* pre_o; // not null: the other part as such, joined with this one
+    const float* pre_l;
+    float* lse; // not null: the log-sum-exp
+    int32_t Hq, D;
+
+    __host__ __device__ __forceinline__ bool any() const {
+        return raw_o != nullptr || pre_o != nullptr || lse != nullptr;
+    }
+};
+
 struct PagedAttnParams {
     PagedPages c;
     PagedWork work;
@@ -46,7 +61,6 @@ struct PagedAttnParams {
     int64_t q_st, q_sh, o_st, o_sh; // bytes
     float scale_log2e;              // |scale| log2(e)
     float q_sign;
-    int32_t zero_tail;
     int32_t Hq;
     const uint8_t* tree; // null: no tree
     int64_t tree_sb, tree_sr;
@@ -55,7 +69,50 @@ struct PagedAttnParams {
     float* part_o;
     float* part_ml;
     PagedRecord* records;
+    PagedJoin join;
+    int32_t zero_tail; // kTailOut, kTailLse
 };
+
+// zero_tail
+constexpr int kTailOut = 1, kTailLse = 2;
+
+// How a row whose keys here sum to l (relative to 2^m) comes out: its unnormalised O
+// times `own`, plus the other part's times `pre`.
+struct PagedRowOut {
+    float own, pre, lse2;
+};
+__device__ __forceinline__ PagedRowOut paged_row_out(const PagedJoin& p, int64_t row, float m, float l) {
+    const float other = p.pre_l != nullptr ? p.pre_l[row] : -INFINITY;
+    const float top = fmaxf(l == 0.0f ? -INFINITY : m, other);
+    const float a = l == 0.0f ? 0.0f : part_weight(m, top);
+    const float b = other == -INFINITY ? 0.0f : part_weight(other, top);
+    const float sum = l * a + b;
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    return PagedRowOut{a * inv, b * inv, sum == 0.0f ? -INFINITY : top + __builtin_amdgcn_logf(sum)};
+}
+// Four channels of a row, from `d` on: to the output, or as one part.
+template <class T>
+__device__ __forceinline__ void paged_store(const PagedJoin& p, const PagedRowOut& r, int64_t row, int d, f4 x,
+                                            char* out) {
+    using V4 = typename PagedVec<T>::v4;
+    x *= r.own;
+    if (p.pre_o != nullptr && r.pre != 0.0f) {
+        x += *reinterpret_cast<const f4*>(p.pre_o + row * p.D + d) * r.pre;
+    }
+    if (p.raw_o != nullptr) {
+        *reinterpret_cast<f4*>(p.raw_o + row * p.D + d) = x;
+    } else {
+        *reinterpret_cast<V4*>(out + 2 * d) = __builtin_convertvector(x, V4);
+    }
+}
+__device__ __forceinline__ void paged_store_lse(const PagedJoin& p, const PagedRowOut& r, int64_t row) {
+    if (p.raw_l != nullptr) {
+        p.raw_l[row] = r.lse2;
+    }
+    if (p.lse != nullptr) {
+        p.lse[row] = r.lse2 * 0.6931471805599453f;
+    }
+}
 
 // 16-byte chunk swizzle of row r of a tile of unpadded rows (see dec_swz of the
 // split-K kernel: rows that start in the same bank differ in it, so 16-row
@@ -514,15 +571,22 @@ __device__ __forceinline__ void tree_mask_scores(f16x (&s)[N], const uint8_t* ro
     }
 }
 
-// Zeros for the rows behind the last sequence, dealt to the workgroups.
+// Zeros (log-sum-exp: -inf) for the rows behind the last sequence, dealt to the workgroups.
 template <int D>
 __device__ __forceinline__ void zero_tail_rows(const PagedAttnParams& p) {
     constexpr int CH = D / 8;
     const int32_t per_row = p.Hq * CH;
     for (int32_t t = paged_rows_end(p.work.seqs) + blockIdx.x; t < p.work.seqs.total; t += gridDim.x) {
-        for (int32_t i = threadIdx.x; i < per_row; i += blockDim.x) {
-            const int32_t h = i / CH;
-            *reinterpret_cast<i4*>(p.o + t * p.o_st + h * p.o_sh + 16 * (i - h * CH)) = i4{0, 0, 0, 0};
+        if ((p.zero_tail & kTailOut) != 0) {
+            for (int32_t i = threadIdx.x; i < per_row; i += blockDim.x) {
+                const int32_t h = i / CH;
+                *reinterpret_cast<i4*>(p.o + t * p.o_st + h * p.o_sh + 16 * (i - h * CH)) = i4{0, 0, 0, 0};
+            }
+        }
+        if ((p.zero_tail & kTailLse) != 0) {
+            for (int32_t h = threadIdx.x; h < p.Hq; h += blockDim.x) {
+                p.join.lse[(int64_t)t * p.Hq + h] = -INFINITY;
+            }
         }
     }
 }

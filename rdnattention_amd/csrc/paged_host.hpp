@@ -84,9 +84,21 @@ struct PagedCommitArgs {
 };
 int paged_commit(const PagedCommitArgs& a, hipStream_t stream, std::string& err);
 
+// Prefixes of the sequences, in the same pages: tables [n, width], lengths [n], and
+// which sequences follow each (see PagedSeqs::group).
+struct PagedPrefix {
+    const int32_t* table = nullptr;
+    const int32_t* lens = nullptr;
+    const int32_t* seqs = nullptr;
+    int64_t table_s = 0;
+    int32_t width = 0, n = 0; // n 0: none
+};
+
 struct PagedAttnArgs {
     PagedPages c;
     PagedSeqs seqs;
+    PagedPrefix prefix;
+    float* lse = nullptr; // [rows, Hq] log-sum-exp of the scores, or null
     PagedMask mask;
     PagedType type = PagedType::F16;
     bool i8 = false;

@@ -106,6 +106,8 @@ int paged_stream_attention(const PagedAttnArgs& a, PagedAttnParams& p, const Pag
                            std::string& err);
 int paged_tile_attention(const PagedAttnArgs& a, PagedAttnParams& p, const PagedLaunch& l, hipStream_t stream,
                          std::string& err);
+int paged_join_tile_attention(const PagedAttnArgs& a, PagedAttnParams& p, const PagedLaunch& l, hipStream_t stream,
+                              std::string& err);
 // ... and what a launch of them may cost at most (paged_max_cost).
 int64_t paged_stream_cost(const PagedAttnArgs& a, const PagedWork& w);
 int64_t paged_tile_cost(const PagedAttnArgs& a, const PagedWork& w);

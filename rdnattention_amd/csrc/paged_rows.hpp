@@ -29,6 +29,10 @@ struct PagedSeqs {
     int32_t rows;
     int32_t total;    // rows of the query tensor
     int32_t max_keys; // keys that a row of the page table covers
+    // > 0: entry b stands for sequences group[b] .. group[b + 1] - 1 of so many (group
+    // null: for all of them), whose rows cu and `rows` give: those that share a prefix
+    int32_t members = 0;
+    const int32_t* group = nullptr;
 };
 
 struct PagedSeq {
@@ -49,7 +53,17 @@ RDNA_MASK_FN int32_t paged_rows_end(const PagedSeqs& s) {
 RDNA_MASK_FN PagedSeq paged_seq(const PagedSeqs& s, int32_t b) {
     PagedSeq r;
     r.len = rows_clamp(s.lens[b], 0, s.max_keys);
-    if (s.cu != nullptr) {
+    if (s.members > 0) {
+        const int32_t first = s.group != nullptr ? rows_clamp(s.group[b], 0, s.members) : 0;
+        const int32_t end = s.group != nullptr ? rows_clamp(s.group[b + 1], first, s.members) : s.members;
+        if (s.cu != nullptr) {
+            r.q0 = rows_clamp(s.cu[first], 0, s.total);
+            r.n = rows_clamp(s.cu[end], r.q0, s.total) - r.q0;
+        } else {
+            r.q0 = first * s.rows;
+            r.n = (end - first) * s.rows;
+        }
+    } else if (s.cu != nullptr) {
         r.q0 = rows_clamp(s.cu[b], 0, s.total);
         r.n = rows_clamp(s.cu[b + 1], r.q0, s.total) - r.q0;
     } else {

@@ -442,7 +442,15 @@ __global__ __launch_bounds__((StreamCfg<D, I8, WV>::THREADS), (StreamCfg<D, I8, 
                     const f4 x = *reinterpret_cast<const f4*>(&sm_o[(w * n_rows + col) * LDM + d]);
                     acc += ml[w].y != 0.0f ? x * wt : f4{0.0f, 0.0f, 0.0f, 0.0f};
                 }
-                if (whole) {
+                if (whole && p.join.any()) {
+                    const int tk = (r0 + col) / G, hd = h * G + r0 + col - tk * G;
+                    const int64_t row = (int64_t)(seq.q0 + tk) * p.Hq + hd;
+                    const PagedRowOut out = paged_row_out(p.join, row, mref, lsum);
+                    paged_store<T>(p.join, out, row, d, acc, p.o + (int64_t)(seq.q0 + tk) * p.o_st + hd * p.o_sh);
+                    if (d == 0) {
+                        paged_store_lse(p.join, out, row);
+                    }
+                } else if (whole) {
                     const int tk = (r0 + col) / G;
                     acc *= lsum > 0.0f ? 1.0f / lsum : 0.0f;
                     *reinterpret_cast<V4*>(p.o + (int64_t)(seq.q0 + tk) * p.o_st + (h * G + r0 + col - tk * G) * p.o_sh +
