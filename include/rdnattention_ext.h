@@ -344,6 +344,34 @@ RDNA_API int32_t rdna_paged_commit(const rdna_paged_cache* cache, const int32_t*
                                    int64_t path_stride, uint32_t path_n, const int32_t* path_lens,
                                    void* hip_stream);
 
+/* Adds the attention that each key has received from the newest rows to its weight:
+ *   w = (decay w, or 0 where the key is one of the newest rows' own)
+ *       + sum over the rows and the heads of the key's kv head of exp(score - lse)
+ * with lse [num_rows, num_heads] as rdna_paged_attention_lse gives it (a row of -inf adds
+ * nothing) and scores, causal and window_size as there; over the cache's own keys alone
+ * where the rows saw a prefix too.  key_weights: float (page, token, head) with
+ * key_weights_stride in floats.  decay at least 0; with 0 the old weights are not read.
+ * Sequences without rows, and places without a key, are left as they are.  The values of
+ * the cache are not looked at.  The same bits every time. */
+RDNA_API int32_t rdna_paged_key_weights(
+    const rdna_paged_cache* cache, const void* query, int64_t query_stride_row, int64_t query_stride_h,
+    uint32_t num_rows, uint32_t num_heads, int32_t dtype, uint32_t max_rows_per_seq, const float* lse, float scale,
+    int32_t causal, int32_t window_size, float decay, float* key_weights, const int64_t* key_weights_stride,
+    void* hip_stream);
+
+/* Keeps `budget` keys of every sequence that has more, for each kv head its own: the
+ * `first` first ones, the `recent` newest ones and, of those between, the ones of the
+ * largest weights (of equal ones those in front; a weight that is not a number is below
+ * all).  In their order they move up to the front of the sequence, with their values,
+ * scales and weights; what is behind them then is unspecified.  new_lens [num_seqs]
+ * (not seq_lens itself): the lengths after it, min(length, budget); kept [num_seqs,
+ * num_kv_heads, budget]: which keys they were, -1 behind the last.  No page may belong to
+ * two sequences.  Where a table names a page that does not exist, the weight counts as
+ * below all and nothing moves.  At most 65535 sequences. */
+RDNA_API int32_t rdna_paged_evict(const rdna_paged_cache* cache, float* key_weights,
+                                  const int64_t* key_weights_stride, uint32_t budget, uint32_t first, uint32_t recent,
+                                  int32_t* new_lens, int32_t* kept, void* hip_stream);
+
 /* Library version string ("0.1.0-gfx950"). */
 RDNA_API const char* rdna_version(void);
 

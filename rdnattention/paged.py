@@ -1,4 +1,5 @@
-"""Paged key/value caches: appending, attention, trees of drafts, commits.
+"""Paged key/value caches: appending, attention, trees of drafts, commits, shared
+prefixes, eviction.
 
 Keys and values of all sequences live in pages of page_size tokens, a power of
 two: ``key_cache`` and ``value_cache`` are [num_pages, page_size, kv_heads,
@@ -39,6 +40,7 @@ _VP, _I64, _U32, _I32, _F32 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_uint32, 
 _CACHE = struct.Struct("=7Q13q6Ii")
 # rdna_paged_norm: 3 pointers, the positions' row stride, axes, eps, dtype
 _NORM = struct.Struct("=3QqIfi")
+_STRIDES = struct.Struct("=3q")
 # rdna_paged_prefix: 3 pointers, the table's row stride, its width, prefixes
 _PREFIX = struct.Struct("=3Qq2I")
 
@@ -73,7 +75,10 @@ def _handle():
     lib.rdna_paged_commit.restype = _I32
     newer = {"rdna_paged_append_norm": [_VP] + lib.rdna_paged_append.argtypes,
              "rdna_paged_attention_lse": ([_VP] * 4 + [_I64] * 4 + [_U32, _U32, _I32, _U32, _F32, _I32, _I32, _I32, _VP,
-                                                                    _VP])}
+                                                                    _VP]),
+             "rdna_paged_key_weights": ([_VP, _VP, _I64, _I64, _U32, _U32, _I32, _U32, _VP, _F32, _I32, _I32, _F32, _VP,
+                                         _VP, _VP]),
+             "rdna_paged_evict": [_VP, _VP, _VP, _U32, _U32, _U32, _VP, _VP, _VP]}
     for name, args in newer.items():
         if hasattr(lib, name):  # absent from libraries built before it existed
             getattr(lib, name).argtypes, getattr(lib, name).restype = args, _I32
@@ -481,3 +486,87 @@ def paged_commit(key_cache, value_cache, block_tables, prefix_lens, path, path_l
     if path_shape[1] == 0 or seqs == 0:
         return
     _call(device, "paged_commit", _lib.rdna_paged_commit, c, prefix, p, path_stride[0], path_shape[1], n)
+
+
+def _key_weights(t, shape, device):
+    """The checked weights' address and packed strides."""
+    if not isinstance(t, _torch.Tensor):
+        raise TypeError("key_weights must be a torch.Tensor")
+    if t.dtype is not _torch.float32 or t.shape != shape or t.get_device() != device:
+        raise ValueError(f"key_weights must be a float32 tensor of shape {tuple(shape)} on the device of key_cache, got "
+                         f"{t.dtype} {tuple(t.shape)}")
+    return t.data_ptr(), _STRIDES.pack(*t.stride())
+
+
+def paged_key_weights(query, lse, key_cache, block_tables, seq_lens, key_weights, *, cu_seqlens_q=None,
+                      max_seqlen_q=None, is_causal: bool = True, window_size: int = -1, scale=None, key_scale=None,
+                      decay: float = 1.0) -> None:
+    """Adds the attention that each cached key has received from a step's rows to
+    its weight, in place:
+
+        w = (decay * w, or 0 for the rows' own keys) + sum of exp(score - lse)
+
+    over the rows and the heads that share the key's kv head.  query, is_causal,
+    window_size and scale as the step's paged_attention or paged_prefix_attention
+    had them, lse (float32 [rows, heads]) as it returned it; behind a prefix the
+    weights are of the sequences' own keys.  key_weights: float32 [num_pages,
+    page_size, kv_heads], any strides.  The rows' own keys begin at 0, so weights
+    of pages that are handed out again need no clearing.  decay: at least 0; with
+    0 old weights are not read.  Sequences without rows are left as they are.
+    Returns None."""
+    torch = _torch or _init()
+    if not isinstance(query, torch.Tensor):
+        raise TypeError("query must be a torch.Tensor")
+    rows = query.shape[0] if query.dim() else 0
+    c, cache_dtype, device, seqs, kv_heads, head_dim, _ = _cache(
+        key_cache, key_cache, block_tables, seq_lens, "seq_lens", cu_seqlens_q, key_scale, key_scale, rows)
+    q, (_, heads, _), qs, dtype = _rows("query", query, rows, None, head_dim, cache_dtype, None, device)
+    if heads % kv_heads:
+        raise ValueError(f"query heads ({heads}) must be a multiple of kv heads ({kv_heads})")
+    if not isinstance(lse, torch.Tensor):
+        raise TypeError("lse must be a torch.Tensor")
+    if lse.dtype is not torch.float32 or lse.shape != (rows, heads) or lse.get_device() != device:
+        raise ValueError(f"lse must be a float32 tensor of shape ({rows}, {heads}) on the device of key_cache, got "
+                         f"{lse.dtype} {tuple(lse.shape)}")
+    if not lse.is_contiguous():
+        raise ValueError("lse must be contiguous")
+    w, w_stride = _key_weights(key_weights, key_cache.shape[:3], device)
+    if not 0.0 <= decay < float("inf"):
+        raise ValueError(f"decay must be finite and not negative, got {decay}")
+    if rows == 0 or heads == 0 or seqs == 0:
+        return
+    most = rows if max_seqlen_q is None else max(0, min(rows, int(max_seqlen_q)))
+    _call(device, "paged_key_weights", _newer("rdna_paged_key_weights"), c, q, qs[0], qs[1], rows, heads, _dtypes[dtype],
+          most, lse.data_ptr(), head_dim ** -0.5 if scale is None else float(scale), 1 if is_causal else 0,
+          max(-1, min(int(window_size), 2 ** 31 - 1)), decay, w, w_stride)
+
+
+def paged_evict(key_cache, value_cache, block_tables, seq_lens, key_weights, budget, *, first: int = 0,
+                recent: int = 0, key_scale=None, value_scale=None):
+    """Keeps `budget` keys of every sequence that has more, in place, each kv head
+    its own: the `first` first keys, the `recent` newest ones, and of those
+    between the ones of the largest key_weights (of equal ones those in front; NaN
+    is below all).  They move up to the front of the sequence in their order, with
+    their values, scales and weights; pages behind the new lengths are free.  No page may
+    belong to two sequences (a shared prefix is no part of these tables).
+
+    Returns (lens, kept): int32 [sequences], the lengths after it, min(length,
+    budget) - seq_lens itself is left as it is; and int32 [sequences, kv_heads,
+    budget], which keys they were, -1 behind the last.  Later rows are appended
+    behind the new lengths with the positions of the text (paged_append's
+    positions).  At most 65535 sequences."""
+    torch = _torch or _init()
+    c, _, device, seqs, kv_heads, _, _ = _cache(key_cache, value_cache, block_tables, seq_lens, "seq_lens", None,
+                                                key_scale, value_scale, None)
+    w, w_stride = _key_weights(key_weights, key_cache.shape[:3], device)
+    budget, first, recent = int(budget), int(first), int(recent)
+    if not 0 < budget <= 1 << 28:
+        raise ValueError(f"budget must be 1 to 2^28, got {budget}")
+    if first < 0 or recent < 0 or first + recent > budget:
+        raise ValueError(f"first ({first}) and recent ({recent}) must not be negative, nor exceed budget ({budget}) together")
+    lens = torch.empty(seqs, dtype=torch.int32, device=key_cache.device)
+    kept = torch.empty(seqs, kv_heads, budget, dtype=torch.int32, device=key_cache.device)
+    if seqs:
+        _call(device, "paged_evict", _newer("rdna_paged_evict"), c, w, w_stride, budget, first, recent, lens.data_ptr(),
+              kept.data_ptr())
+    return lens, kept

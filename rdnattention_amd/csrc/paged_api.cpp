@@ -512,3 +512,141 @@ RDNA_API int32_t rdna_paged_commit(const rdna_paged_cache* cache, const int32_t*
         return rdna_amd::paged_commit(a, static_cast<hipStream_t>(hip_stream), err);
     });
 }
+
+namespace {
+
+// Weights of keys [pages, page, heads]; "" or what is wrong.
+std::string check_weights(const rdna_paged_cache* in, const float* w, const int64_t* stride) {
+    if (w == nullptr || stride == nullptr) {
+        return "null key_weights";
+    }
+    if (!aligned(w, 4)) {
+        return "key_weights must be an aligned float array";
+    }
+    if (!stride_fits(stride[0], 4, in->num_pages) || !stride_fits(stride[1], 4, in->page_size) ||
+        !stride_fits(stride[2], 4, in->num_kv_heads)) {
+        return "the strides of key_weights must not be negative, and stay within 2^56 bytes";
+    }
+    return "";
+}
+
+} // namespace
+
+RDNA_API int32_t rdna_paged_key_weights(const rdna_paged_cache* cache, const void* query, int64_t query_stride_row,
+                                        int64_t query_stride_h, uint32_t num_rows, uint32_t num_heads, int32_t dtype,
+                                        uint32_t max_rows_per_seq, const float* lse, float scale, int32_t causal,
+                                        int32_t window_size, float decay, float* key_weights,
+                                        const int64_t* key_weights_stride, void* hip_stream) {
+#if defined(RDNATTENTION_NO_INT8)
+    if (no_int8(cache, "Paged key weights unavailable: %s")) {
+        return -4;
+    }
+#endif
+    return guarded("Paged key weights failed: %s", [&](std::string& err) {
+        rdna_amd::PagedWeightsArgs a;
+        rdna_paged_cache keys = {};
+        if (cache != nullptr) { // values are not looked at
+            keys = *cache;
+            keys.value = keys.key;
+            keys.value_scale = keys.key_scale;
+            for (int i = 0; i < 3; i++) {
+                keys.value_stride[i] = keys.key_stride[i];
+                keys.value_scale_stride[i] = keys.key_scale_stride[i];
+            }
+        }
+        err = check_cache(cache != nullptr ? &keys : nullptr, a.c, a.i8);
+        if (err.empty()) {
+            err = check_rows(cache, num_rows, dtype, a.i8, a.seqs);
+        }
+        if (err.empty()) {
+            err = check_weights(cache, key_weights, key_weights_stride);
+        }
+        if (!err.empty()) {
+            return -1;
+        }
+        a.type = dtype == RDNA_DTYPE_F16 ? PagedType::F16 : PagedType::BF16;
+        a.Hkv = (int32_t)cache->num_kv_heads;
+        a.D = (int32_t)cache->head_dim;
+        if (num_heads == 0 || num_heads > 65535 || num_heads % cache->num_kv_heads != 0) {
+            err = "num_heads must be a positive multiple of num_kv_heads, at most 65535";
+        } else if ((uint64_t)num_rows * (num_heads / cache->num_kv_heads) > (uint64_t(1) << 30)) {
+            err = "rows x heads per kv head exceed 2^30";
+        } else if (query == nullptr || lse == nullptr) {
+            err = "null tensor pointer";
+        } else if (!aligned(query, 16) || !aligned(lse, 4)) {
+            err = "query must be 16-byte aligned, lse 4-byte aligned";
+        } else if (!stride_bytes(query_stride_row, 2, num_rows, a.q_st) ||
+                   !stride_bytes(query_stride_h, 2, num_heads, a.q_sh)) {
+            err = std::string("query ") + kStrides;
+        } else if (!std::isfinite(scale)) {
+            err = "scale must be finite";
+        } else if (!std::isfinite(decay) || decay < 0.0f) {
+            err = "decay must be finite and not negative";
+        }
+        if (!err.empty()) {
+            return -1;
+        }
+        a.Hq = (int32_t)num_heads;
+        a.max_rows_seq = cache->cu_seqlens == nullptr ? a.seqs.rows
+                                                      : (int32_t)(max_rows_per_seq < num_rows ? max_rows_per_seq : num_rows);
+        a.q = query;
+        a.lse = lse;
+        a.scale = scale;
+        a.decay = decay;
+        a.mask.causal = causal != 0 ? 1 : 0;
+        a.mask.window = window_size > 0 && window_size < (1 << 30) ? window_size : 0;
+        a.w = key_weights;
+        a.w_sp = key_weights_stride[0], a.w_st = key_weights_stride[1], a.w_sh = key_weights_stride[2];
+        return rdna_amd::paged_key_weights(a, static_cast<hipStream_t>(hip_stream), err);
+    });
+}
+
+RDNA_API int32_t rdna_paged_evict(const rdna_paged_cache* cache, float* key_weights, const int64_t* key_weights_stride,
+                                  uint32_t budget, uint32_t first, uint32_t recent, int32_t* new_lens, int32_t* kept,
+                                  void* hip_stream) {
+#if defined(RDNATTENTION_NO_INT8)
+    if (no_int8(cache, "Paged evict unavailable: %s")) {
+        return -4;
+    }
+#endif
+    return guarded("Paged evict failed: %s", [&](std::string& err) {
+        rdna_amd::PagedEvictArgs a;
+        err = check_cache(cache, a.c, a.i8);
+        if (err.empty()) {
+            err = check_weights(cache, key_weights, key_weights_stride);
+        }
+        if (!err.empty()) {
+            return -1;
+        }
+        if (cache->num_seqs > 65535) {
+            err = "num_seqs exceeds 65535";
+        } else if (cache->seq_lens == nullptr || new_lens == nullptr || kept == nullptr) {
+            err = "null index pointer";
+        } else if (!aligned(cache->seq_lens, 4) || !aligned(new_lens, 4) || !aligned(kept, 4)) {
+            err = "index arrays must be aligned int32 arrays";
+        } else if (cache->seq_lens == new_lens) {
+            err = "new_lens must not be seq_lens";
+        } else if (budget == 0 || budget > (uint32_t)kPagedMaxLen) {
+            err = "budget must be 1 to 2^28";
+        } else if ((uint64_t)first + recent > budget) {
+            err = "first and recent must not exceed budget together";
+        } else if (a.c.k == a.c.v) {
+            err = kShared;
+        }
+        if (!err.empty()) {
+            return -1;
+        }
+        a.B = (int32_t)cache->num_seqs;
+        a.Hkv = (int32_t)cache->num_kv_heads;
+        a.row_bytes = (int32_t)cache->head_dim * (a.i8 ? 1 : 2);
+        a.lens = cache->seq_lens;
+        a.budget = (int32_t)budget;
+        a.first = (int32_t)first;
+        a.recent = (int32_t)recent;
+        a.w = key_weights;
+        a.w_sp = key_weights_stride[0], a.w_st = key_weights_stride[1], a.w_sh = key_weights_stride[2];
+        a.new_lens = new_lens;
+        a.kept = kept;
+        return rdna_amd::paged_evict(a, static_cast<hipStream_t>(hip_stream), err);
+    });
+}

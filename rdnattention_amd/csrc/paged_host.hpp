@@ -115,6 +115,39 @@ struct PagedAttnArgs {
 };
 int paged_attention(const PagedAttnArgs& a, hipStream_t stream, std::string& err);
 
+// The attention that keys have received (paged_weights.hip): only the keys of c and seqs,
+// weights [pages, page, Hkv] with strides in floats.
+struct PagedWeightsArgs {
+    PagedPages c;
+    PagedSeqs seqs;
+    PagedMask mask;
+    PagedType type = PagedType::F16;
+    bool i8 = false;
+    int32_t Hq = 0, Hkv = 0, D = 0;
+    int32_t max_rows_seq = 0;
+    const void* q = nullptr;
+    int64_t q_st = 0, q_sh = 0; // bytes
+    const float* lse = nullptr; // [rows, Hq]
+    float scale = 1.0f, decay = 1.0f;
+    float* w = nullptr;
+    int64_t w_sp = 0, w_st = 0, w_sh = 0;
+};
+int paged_key_weights(const PagedWeightsArgs& a, hipStream_t stream, std::string& err);
+
+// The keys of the largest weights to the front (paged_evict.hip).
+struct PagedEvictArgs {
+    PagedPages c;
+    bool i8 = false;
+    int32_t B = 0, Hkv = 0, row_bytes = 0;
+    const int32_t* lens = nullptr;
+    int32_t budget = 0, first = 0, recent = 0;
+    float* w = nullptr;
+    int64_t w_sp = 0, w_st = 0, w_sh = 0;
+    int32_t* new_lens = nullptr; // [B]
+    int32_t* kept = nullptr;     // [B, Hkv, budget]
+};
+int paged_evict(const PagedEvictArgs& a, hipStream_t stream, std::string& err);
+
 // Sets the library's thread-local error message (c_api.cpp).
 void set_api_error(const char* fmt, const std::string& detail);
 

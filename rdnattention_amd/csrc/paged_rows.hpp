@@ -96,6 +96,29 @@ RDNA_MASK_FN MaskSpec paged_mask(const PagedMask& m, const PagedSeq& s) {
     return MaskSpec{s.len, s.len - s.n, m.causal, m.window};
 }
 
+// Rows lo .. hi (tokens times G and heads, none where hi < lo) of a sequence that see
+// key `key`: neither falls as the key grows.
+struct PagedKeyRows {
+    int32_t lo, hi;
+};
+RDNA_MASK_FN PagedKeyRows paged_key_rows(const PagedMask& m, const PagedSeq& s, int32_t G, int32_t key) {
+    // the first and the last token that sees it
+    const int32_t at = key - (s.len - s.n);
+    int32_t first = 0, last = s.n - 1;
+    if (m.causal != 0) {
+        first = at;
+        if (m.window > 0) {
+            last = at + m.window - 1;
+        }
+    } else if (m.window > 0) {
+        first = at - (m.window >> 1);
+        last = at + (m.window >> 1);
+    }
+    first = rows_clamp(first, 0, s.n);
+    last = mask_imin(mask_imax(last, -1), s.n - 1);
+    return key >= 0 && key < s.len ? PagedKeyRows{first * G, (last + 1) * G - 1} : PagedKeyRows{s.n * G, -1};
+}
+
 // Work of a call: sequences with more than min_rows and at most max_rows rows
 // (tokens times G) are dealt to n_wg workers.
 struct PagedWork {

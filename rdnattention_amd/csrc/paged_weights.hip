@@ -1,0 +1,444 @@
+// The attention that each cached key has received from a call's rows, added to its
+// weight: w_j = (decay w_j, or 0 where the key is one of the newest rows) + the sum over
+// the rows i and the G heads of the key's kv head of exp(c q_i k_j - lse_i).
+//
+// The keys are the lanes of the matrix products (S = Q K^T, a row of Q to a register),
+// so that a key's sum stays in its lane, whatever its page holds reaches no other key,
+// and no two workgroups share a key: no atomics, no scratch, the same bits every time.
+//   * few rows (up to 32 of a kv head): bound by HBM, K is read once.  The waves take 32-key
+//     tiles, straight into the MFMA layout, one tile ahead
+//   * more rows: bound by the exponentials beside the products.  A workgroup keeps a block of
+//     keys in registers and its waves take the row tiles in turn, Q through LDS one tile
+//     ahead
+#include "fa_common.hpp"
+#include "paged_attn.hpp"
+#include "paged_launch.hpp"
+
+#include <algorithm>
+
+namespace rdna_amd {
+
+float softmax_log2_scale(float scale);
+
+namespace {
+
+constexpr int kTile = 32;    // keys and rows of a product
+constexpr int kFewRows = 32; // one row tile
+// one item per kv head of a sequence, its units blocks of keys
+constexpr int kAllRows = 1 << 30;
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct WeightsParams {
+    PagedPages c;
+    PagedWork work; // its mask hides nothing: every key has a weight
+    PagedMask mask;
+    const char* q;
+    int64_t q_st, q_sh; // bytes
+    const float* lse;
+    int32_t Hq;
+    float scale_log2e; // |scale| log2(e)
+    float q_sign;
+    float decay;
+    float* w;
+    int64_t w_sp, w_st, w_sh;
+};
+
+// A row's log-sum-exp in log2 units, as what is subtracted in the exponent and a factor
+// for the rest of the product lse log2(e), which 32 bits do not hold: the weights of a row
+// would all be off by 2^-24 of the exponent.  A row that sees nothing has no weights.
+struct RowLse {
+    float sub, factor;
+};
+__device__ __forceinline__ RowLse row_lse(float lse) {
+    const float hi = lse * kLog2e;
+    float lo = fmaf(lse, kLog2e, -hi) + lse * 1.925963033500000e-08f; // log2(e) - kLog2e
+    lo = fabsf(lo) < 1.0f ? lo : 0.0f;                                // infinities
+    return lse == -INFINITY ? RowLse{INFINITY, 1.0f} : RowLse{hi, fast_exp2(-lo)};
+}
+
+// What a lane needs of key `key`: where its row and weight are, and which rows see it.
+struct LaneKey {
+    const char* k;
+    float* w;      // null: no key, or no page
+    float k_scale; // int8 pages
+    PagedKeyRows rows;
+    bool old;
+};
+
+template <bool I8>
+__device__ __forceinline__ LaneKey lane_key(const WeightsParams& p, const PagedSeq& seq, const int32_t* table, int h,
+                                            int key) {
+    LaneKey r;
+    const int32_t pg = key < seq.len ? paged_page(p.c, table, key >> p.c.lps) : -1;
+    const int64_t page = pg >= 0 ? pg : 0;
+    const int64_t off = key & ((1 << p.c.lps) - 1);
+    r.k = pg >= 0 ? p.c.k + page * p.c.k_sp + off * p.c.k_st + h * p.c.k_sh
+                  : reinterpret_cast<const char*>(kPagedZeroRow);
+    r.w = pg >= 0 ? p.w + page * p.w_sp + off * p.w_st + h * p.w_sh : nullptr;
+    r.k_scale = 1.0f;
+    if constexpr (I8) {
+        r.k_scale = pg >= 0 ? p.c.ks[page * p.c.ks_sp + off * p.c.ks_st + h * p.c.ks_sh] : 0.0f;
+    }
+    r.rows = paged_key_rows(p.mask, seq, p.work.G, key);
+    r.old = key < seq.len - seq.n;
+    return r;
+}
+
+// A key's row in the MFMA layout: lane (l32, g) holds chunk x of row l32, a chunk being 16
+// bytes of it.
+template <int D, bool I8>
+struct KeyRegs {
+    static constexpr int N = I8 ? D / 32 : D / 16;
+    i4 x[N];
+    __device__ __forceinline__ void load(const char* row, int g) {
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            x[i] = *reinterpret_cast<const i4*>(row + 32 * i + 16 * g);
+        }
+    }
+    // operand s of the product over D, which chunk_of_q(s) of the row of Q meets
+    template <class T>
+    __device__ __forceinline__ typename PagedVec<T>::v8 operand(int s) const {
+        if constexpr (I8) {
+            return widen_int8<T>(i2v{x[s >> 1][2 * (s & 1)], x[s >> 1][2 * (s & 1) + 1]});
+        } else {
+            return __builtin_bit_cast(typename PagedVec<T>::v8, x[s]);
+        }
+    }
+};
+template <bool I8>
+__device__ __forceinline__ int chunk_of_q(int s, int g) {
+    return I8 ? 4 * (s >> 1) + 2 * g + (s & 1) : 2 * s + g;
+}
+
+// Sum over the lane's 16 rows (base + 8 (e / 4) + 4 g + e % 4) of their weights on its key.
+template <bool MASK>
+__device__ __forceinline__ float sum_weights(const f16x& s, float c, const f4 (&sub)[4], const f4 (&factor)[4], int lo,
+                                             int hi, float sum) {
+    float part[4] = {sum, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int e = 0; e < 16; e++) {
+        float p = fast_exp2(fmaf(s[e], c, -sub[e >> 2][e & 3]));
+        if constexpr (MASK) {
+            const int off = 8 * (e >> 2) + (e & 3);
+            p = off < lo || off > hi ? 0.0f : p;
+        }
+        part[e & 3] = fmaf(p, factor[e >> 2][e & 3], part[e & 3]);
+    }
+    return (part[0] + part[1]) + (part[2] + part[3]);
+}
+
+__device__ __forceinline__ float new_weight(const WeightsParams& p, const LaneKey& k, float sum, float old) {
+    return k.old && p.decay != 0.0f ? fmaf(p.decay, old, sum) : sum;
+}
+
+template <class T, int D, bool I8>
+__global__ __launch_bounds__(256) void paged_weights_few(WeightsParams p) {
+    using V8 = typename PagedVec<T>::v8;
+    constexpr int NS = D / 16;
+    __shared__ __attribute__((aligned(16))) float rows_lse[4][2][kTile];
+    const int wave = uniform(threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63;
+    const int l32 = lane & 31, g = lane >> 5;
+    PagedWalk<kAllRows, kTile, false, 0> walk(p.work, I8 ? by_xcd(blockIdx.x, p.work.n_wg) : (int32_t)blockIdx.x);
+    while (walk.more()) {
+        const PagedSeq seq = walk.seq;
+        const int h = uniform(walk.h), G = p.work.G;
+        const int rows = uniform(seq.n * G);
+        const int t0 = uniform(walk.tile.first + walk.begin());
+        const int nt = uniform(walk.tile.hi >= walk.tile.lo ? walk.count() : 0);
+        const int32_t* const table = p.c.table + walk.b * p.c.table_s;
+
+        // one row tile (more only where the caller has said that there were fewer rows)
+        for (int base = 0; base < rows; base += kTile) {
+            const bool valid = base + l32 < rows;
+            const int tok = valid ? (base + l32) / G : 0;
+            const int head = h * G + (valid ? base + l32 - tok * G : 0);
+            V8 q[NS];
+            {
+                const char* const row = p.q + (int64_t)(seq.q0 + tok) * p.q_st + head * p.q_sh;
+#pragma unroll
+                for (int s = 0; s < NS; s++) {
+                    const V8 x = *reinterpret_cast<const V8*>(row + 16 * chunk_of_q<I8>(s, g));
+                    q[s] = valid ? (p.q_sign < 0.0f ? -x : x) : V8{};
+                }
+                const RowLse r = row_lse(valid ? p.lse[(int64_t)(seq.q0 + tok) * p.Hq + head] : -INFINITY);
+                rows_lse[wave][0][l32] = r.sub;
+                rows_lse[wave][1][l32] = r.factor;
+            }
+            f4 sub[4], factor[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                sub[i] = *reinterpret_cast<const f4*>(&rows_lse[wave][0][8 * i + 4 * g]);
+                factor[i] = *reinterpret_cast<const f4*>(&rows_lse[wave][1][8 * i + 4 * g]);
+            }
+            auto key_of = [&](int j) { return (t0 + wave + 4 * j) * kTile + l32; };
+            const int mine = nt > wave ? (nt - wave + 3) / 4 : 0;
+            KeyRegs<D, I8> k0, k1;
+            LaneKey a, b;
+            auto tile = [&](const LaneKey& key, const KeyRegs<D, I8>& k) __attribute__((always_inline)) {
+                const bool later = base > 0;
+                const float old = g == 0 && key.w != nullptr && (key.old || later) ? *key.w : 0.0f;
+                f16x s = f16x{};
+#pragma unroll
+                for (int i = 0; i < NS; i++) {
+                    s = paged_mfma<T>(q[i], k.template operand<T>(i), s);
+                }
+                const float c = p.scale_log2e * key.k_scale;
+                const int lo = key.rows.lo - base - 4 * g, hi = key.rows.hi - base - 4 * g;
+                float sum;
+                if (wave_any(key.rows.lo > base || key.rows.hi < base + kTile - 1)) {
+                    sum = sum_weights<true>(s, c, sub, factor, lo, hi, 0.0f);
+                } else {
+                    sum = sum_weights<false>(s, c, sub, factor, lo, hi, 0.0f);
+                }
+                sum = pair_sum(sum);
+                if (g == 0 && key.w != nullptr) {
+                    *key.w = later ? old + sum : new_weight(p, key, sum, old);
+                }
+            };
+            if (mine > 0) {
+                a = lane_key<I8>(p, seq, table, h, key_of(0));
+                k0.load(a.k, g);
+            }
+            for (int j = 0; j < mine; j += 2) {
+                if (j + 1 < mine) {
+                    b = lane_key<I8>(p, seq, table, h, key_of(j + 1));
+                    k1.load(b.k, g);
+                }
+                tile(a, k0);
+                if (j + 2 < mine) {
+                    a = lane_key<I8>(p, seq, table, h, key_of(j + 2));
+                    k0.load(a.k, g);
+                }
+                if (j + 1 < mine) {
+                    tile(b, k1);
+                }
+            }
+        }
+        walk.next();
+    }
+}
+
+template <int D>
+struct ManyCfg {
+    static constexpr int WAVES = 4;
+    static constexpr int THREADS = 64 * WAVES;
+    static constexpr int KT = D <= 96 ? 4 : D <= 128 ? 3 : 2; // 32-key tiles in registers
+    static constexpr int BLOCK = kTile * KT;
+    static constexpr int WAVES_PER_SIMD = D <= 128 ? 2 : 1;
+    static constexpr int RB = 2 * D;
+    static constexpr int KCH = D / 8;
+    static constexpr int Q_BYTES = kTile * RB;
+    static constexpr int NS = D / 16;
+    static constexpr int LDS_BYTES = WAVES * (2 * Q_BYTES + 2 * kTile * 4);
+    static_assert(LDS_BYTES + WAVES * BLOCK * 4 <= 160 * 1024 / (D <= 128 ? 2 : 1), "workgroups fit the LDS");
+};
+
+template <class T, int D, bool I8>
+__global__ __launch_bounds__((ManyCfg<D>::THREADS), (ManyCfg<D>::WAVES_PER_SIMD)) void paged_weights_many(
+    WeightsParams p) {
+    using C = ManyCfg<D>;
+    using V8 = typename PagedVec<T>::v8;
+    __shared__ __attribute__((aligned(16))) char dsm[C::LDS_BYTES];
+    __shared__ float sums[C::WAVES][C::BLOCK];
+    const int tid = threadIdx.x;
+    const int wave = uniform(tid >> 6);
+    const int lane = tid & 63;
+    const int l32 = lane & 31, g = lane >> 5;
+    const uint32_t lds_w = (uint32_t)reinterpret_cast<uintptr_t>(dsm) + wave * 2 * C::Q_BYTES;
+    char* const qsm = dsm + wave * 2 * C::Q_BYTES;
+    float* const lsm = reinterpret_cast<float*>(dsm + C::WAVES * 2 * C::Q_BYTES) + wave * 2 * kTile;
+
+    PagedWalk<kAllRows, C::BLOCK, false, 0> walk(p.work, by_xcd(blockIdx.x, p.work.n_wg));
+    while (walk.more()) {
+        const PagedSeq seq = walk.seq;
+        const int h = uniform(walk.h), G = p.work.G;
+        const int rows = uniform(seq.n * G);
+        const int nt = uniform(walk.tile.hi >= walk.tile.lo ? walk.count() : 0);
+        const int32_t* const table = p.c.table + walk.b * p.c.table_s;
+        for (int u = 0; u < nt; u++) {
+            const int key0 = uniform(walk.tile.first + walk.begin() + u) * C::BLOCK;
+            const int last = min(key0 + C::BLOCK, seq.len) - 1;
+            // row tiles that some key of the block is seen by
+            const int r_lo = uniform(paged_key_rows(p.mask, seq, G, key0).lo);
+            const int r_hi = uniform(paged_key_rows(p.mask, seq, G, last).hi);
+            const int rt0 = r_lo / kTile, rt1 = r_hi < 0 ? -1 : r_hi / kTile;
+
+            // row of a tile that this lane loads
+            float lse_next = 0.0f;
+            auto prefetch = [&](int rt, int slot) __attribute__((always_inline)) {
+                const int r = min(rt * kTile + l32, rows - 1);
+                const int tok = r / G;
+                const int head = h * G + r - tok * G;
+                const char* const at = p.q + (int64_t)(seq.q0 + tok) * p.q_st + head * p.q_sh;
+                const uint64_t mine = reinterpret_cast<uint64_t>(at);
+                lse_next = p.lse[(int64_t)(seq.q0 + tok) * p.Hq + head];
+                const uint32_t lo = (uint32_t)mine, hi = (uint32_t)(mine >> 32);
+                int ln = lane;
+                asm volatile("" : "+v"(ln));
+#pragma unroll
+                for (int n = 0; n < C::NS; n++) {
+                    const int c = 64 * n + ln;
+                    const int x = c / C::KCH;
+                    const uint64_t row = (uint64_t)(uint32_t)__builtin_amdgcn_ds_bpermute(4 * x, (int)hi) << 32 |
+                                         (uint32_t)__builtin_amdgcn_ds_bpermute(4 * x, (int)lo);
+                    dma_gather16(row + (uint32_t)((c - x * C::KCH) ^ paged_swz<D>(x)) * 16u,
+                                 (uint32_t)uniform((int)lds_w + slot * C::Q_BYTES + 1024 * n));
+                }
+            };
+            int rt = rt0 + wave;
+            if (rt <= rt1) {
+                prefetch(rt, 0);
+            }
+            KeyRegs<D, I8> k[C::KT];
+            float scale[C::KT], sum[C::KT];
+            int lo[C::KT], hi[C::KT];
+#pragma unroll
+            for (int t = 0; t < C::KT; t++) {
+                const LaneKey key = lane_key<I8>(p, seq, table, h, key0 + kTile * t + l32);
+                k[t].load(key.k, g);
+                scale[t] = p.scale_log2e * key.k_scale * p.q_sign;
+                lo[t] = key.rows.lo - 4 * g;
+                hi[t] = key.rows.hi - 4 * g;
+                sum[t] = 0.0f;
+            }
+            for (int slot = 0; rt <= rt1; rt += C::WAVES, slot ^= 1) {
+                const RowLse r = row_lse(lse_next);
+                lsm[l32] = r.sub;
+                lsm[kTile + l32] = r.factor;
+                // this tile's Q has landed, and what the next one overwrites has been read
+                __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
+                __builtin_amdgcn_s_waitcnt(waitcnt_lgkm(0));
+                asm volatile("" ::: "memory");
+                if (rt + C::WAVES <= rt1) {
+                    prefetch(rt + C::WAVES, slot ^ 1);
+                }
+                f4 sub[4], factor[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    sub[i] = *reinterpret_cast<const f4*>(lsm + 8 * i + 4 * g);
+                    factor[i] = *reinterpret_cast<const f4*>(lsm + kTile + 8 * i + 4 * g);
+                }
+                V8 q[C::NS];
+#pragma unroll
+                for (int s = 0; s < C::NS; s++) {
+                    q[s] = *reinterpret_cast<const V8*>(qsm + slot * C::Q_BYTES + l32 * C::RB +
+                                                        ((chunk_of_q<I8>(s, g) ^ paged_swz<D>(l32)) << 4));
+                }
+                const int base = rt * kTile;
+#pragma unroll
+                for (int t = 0; t < C::KT; t++) {
+                    f16x s = f16x{};
+#pragma unroll
+                    for (int i = 0; i < C::NS; i++) {
+                        s = paged_mfma<T>(q[i], k[t].template operand<T>(i), s);
+                    }
+                    if (wave_any(lo[t] + 4 * g > base || hi[t] + 4 * g < base + kTile - 1)) {
+                        sum[t] = sum_weights<true>(s, scale[t], sub, factor, lo[t] - base, hi[t] - base, sum[t]);
+                    } else {
+                        sum[t] = sum_weights<false>(s, scale[t], sub, factor, 0, 0, sum[t]);
+                    }
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < C::KT; t++) {
+                const float x = pair_sum(sum[t]);
+                if (g == 0) {
+                    sums[wave][kTile * t + l32] = x;
+                }
+            }
+            __syncthreads();
+            if (tid < C::BLOCK) {
+                const LaneKey key = lane_key<false>(p, seq, table, h, key0 + tid);
+                float x = 0.0f;
+#pragma unroll
+                for (int w = 0; w < C::WAVES; w++) {
+                    x += sums[w][tid];
+                }
+                if (key.w != nullptr) {
+                    *key.w = new_weight(p, key, x, key.old ? *key.w : 0.0f);
+                }
+            }
+            __syncthreads(); // before the sums of the next block
+        }
+        walk.next();
+    }
+}
+
+template <class T, int D, bool I8>
+int launch_weights(const PagedWeightsArgs& a, WeightsParams& p, hipStream_t stream, std::string& err) {
+    auto go = [&](auto* kernel, int threads, int64_t units, int min_units) {
+        const int64_t resident = resident_workgroups(reinterpret_cast<const void*>(kernel), threads, err);
+        if (resident <= 0) {
+            return -1;
+        }
+        p.work.min_units = min_units;
+        p.work.n_wg = paged_workgroups(resident, units, min_units);
+        hipLaunchKernelGGL(kernel, dim3((uint32_t)p.work.n_wg), dim3(threads), 0, stream, p);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) {
+            err = hipGetErrorString(e);
+            return -1;
+        }
+        return 0;
+    };
+    // as in paged_attention: each launch takes the sequences of its kind
+    const bool any_many = (int64_t)a.max_rows_seq * p.work.G > kFewRows;
+    const bool any_few = !any_many || a.seqs.cu != nullptr;
+    PagedLaunch few, many;
+    if (any_many && any_few) {
+        few.max_rows = many.min_rows = kFewRows;
+    }
+    const PagedWork wf = paged_work(p.work, few), wm = paged_work(p.work, many);
+    const int64_t cf = any_few ? paged_max_cost<kAllRows, kTile, 0>(wf) : 0;
+    const int64_t cm = any_many ? paged_max_cost<kAllRows, ManyCfg<D>::BLOCK, 0>(wm) : 0;
+    if (std::max(cf, cm) > INT32_MAX) {
+        err = "too many sequences x heads x keys that the page table covers (at most 2^31 - 1 key tiles)";
+        return -1;
+    }
+    if (any_many) {
+        p.work = wm;
+        if (go(&paged_weights_many<T, D, I8>, ManyCfg<D>::THREADS, cm, 1) != 0) {
+            return -1;
+        }
+    }
+    if (any_few) {
+        p.work = wf;
+        return go(&paged_weights_few<T, D, I8>, 256, cf, 4);
+    }
+    return 0;
+}
+
+} // namespace
+
+int paged_key_weights(const PagedWeightsArgs& a, hipStream_t stream, std::string& err) {
+    WeightsParams p{};
+    p.c = a.c;
+    p.work.seqs = a.seqs;
+    p.work.mask = PagedMask{0, 0};
+    p.work.Hkv = a.Hkv;
+    p.work.G = a.Hq / a.Hkv;
+    p.mask = a.mask;
+    p.q = static_cast<const char*>(a.q);
+    p.q_st = a.q_st;
+    p.q_sh = a.q_sh;
+    p.lse = a.lse;
+    p.Hq = a.Hq;
+    p.scale_log2e = softmax_log2_scale(a.scale);
+    p.q_sign = a.scale < 0.0f ? -1.0f : 1.0f;
+    p.decay = a.decay;
+    p.w = a.w;
+    p.w_sp = a.w_sp;
+    p.w_st = a.w_st;
+    p.w_sh = a.w_sh;
+    PagedAttnArgs types; // of the kernels
+    types.type = a.type;
+    types.i8 = a.i8;
+    types.D = a.D;
+    return paged_for_type(types, [&](auto t, auto d, auto i8) {
+        return launch_weights<decltype(t), decltype(d)::value, decltype(i8)::value>(a, p, stream, err);
+    });
+}
+
+} // namespace rdna_amd
