@@ -47,10 +47,26 @@ struct PagedJoin {
     const float* pre_l;
     float* lse; // not null: the log-sum-exp
     int32_t Hq, D;
+    // Of the kernel that has prefixes and sequences in one launch (paged_join_stream), by kind (0
+    // prefix, 1 own keys) and row: what a whole item leaves, O as in a slot and (m, l), and
+    // where the parts of the others are.
+    float* whole_o;
+    float* whole_ml;
+    struct PagedParts* parts;
+    const int32_t* prefix_table;
+    int64_t prefix_table_s;
+    int32_t prefix_width;
+    int32_t rows; // rows x heads of the call
 
     __host__ __device__ __forceinline__ bool any() const {
         return raw_o != nullptr || pre_o != nullptr || lse != nullptr;
     }
+};
+
+// The parts of a row: of workers w (slot n_wg + w) and w + 1 .. w_last (slots of their
+// number), in row `col` of each slot; w < 0: one, whole.
+struct PagedParts {
+    int32_t w, w_last, col, unused;
 };
 
 struct PagedAttnParams {
@@ -352,7 +368,9 @@ __device__ __forceinline__ int32_t by_xcd(int32_t id, int32_t n) {
 // tile, longer ones are only slower.)  An item costs its units and EXTRA, the time
 // before its first and after its last key tile in key tiles, and the shares are of equal
 // cost: a worker with the many short row tiles at a prompt's begin has fewer key tiles.
-template <int ROWS, int BN, bool MANY, int EXTRA>
+// PREFIXES: the first entries are prefixes (PagedSeqs), all keys of which all their rows see,
+// so that their row tiles are alike.
+template <int ROWS, int BN, bool MANY, int EXTRA, bool PREFIXES = false>
 struct PagedWalk {
     const PagedWork& w;
     PagedShare<EXTRA> part; // the worker's share, and of the current item
@@ -365,10 +383,12 @@ struct PagedWalk {
         const int32_t B = w.seqs.B;
         // sequence i and what one kv head of it costs
         auto cost_of = [&](int32_t i, PagedSeq& s) {
-            s = i < B ? paged_seq(w.seqs, i) : PagedSeq{0, 0, 0};
+            s = i < B ? entry(i) : PagedSeq{0, 0, 0};
             const int32_t n = paged_row_tiles<ROWS>(w, s.n);
             int32_t u = 0;
-            if (!MANY || n <= kFewTiles) {
+            if (PREFIXES && i < w.seqs.prefixes) {
+                u = n * (prefix_tile(s).units + EXTRA);
+            } else if (!MANY || n <= kFewTiles) {
                 u = paged_head_units<ROWS, BN>(w, s) + n * EXTRA;
             }
             if constexpr (MANY) {
@@ -446,6 +466,10 @@ struct PagedWalk {
             load_tile();
         } else {
             load_tile();
+            if (PREFIXES && b < w.seqs.prefixes) {
+                rt = uniform(min(at / (tile.units + EXTRA), n_rt - 1));
+                at -= rt * (tile.units + EXTRA);
+            }
             while (at >= tile.units + EXTRA && rt + 1 < n_rt) {
                 at -= tile.units + EXTRA;
                 rt++;
@@ -486,14 +510,21 @@ struct PagedWalk {
     }
 
     __device__ __forceinline__ void load_seq() {
-        seq = paged_seq(w.seqs, b);
+        seq = entry(b);
         seq.q0 = uniform(seq.q0);
         seq.n = uniform(seq.n);
         seq.len = uniform(seq.len);
         n_rt = uniform(paged_row_tiles<ROWS>(w, seq.n));
     }
+    __device__ __forceinline__ PagedSeq entry(int32_t i) const {
+        return PREFIXES ? paged_entry(w.seqs, i) : paged_seq(w.seqs, i);
+    }
+    // Any row tile of a prefix.
+    __device__ __forceinline__ PagedTile prefix_tile(const PagedSeq& s) const {
+        return s.len > 0 ? PagedTile{0, s.len - 1, 0, (s.len + BN - 1) / BN} : PagedTile{0, -1, 0, 1};
+    }
     __device__ __forceinline__ void load_tile() {
-        tile = paged_tile<ROWS, BN>(w, seq, rt);
+        tile = PREFIXES && b < w.seqs.prefixes ? prefix_tile(seq) : paged_tile<ROWS, BN>(w, seq, rt);
         tile.lo = uniform(tile.lo);
         tile.hi = uniform(tile.hi);
         tile.first = uniform(tile.first);

@@ -27,7 +27,8 @@ inline PagedWork paged_work(const PagedWork& call, const PagedLaunch& l) {
     return w;
 }
 
-// The merge of the items that several workgroups share (paged_merge.hip).
+// The merge of the items that several workgroups share (paged_merge.hip), or of every row's
+// parts where p.join.parts says where they are.
 int paged_merge(const PagedAttnArgs& a, const PagedAttnParams& p, hipStream_t stream, std::string& err);
 
 // Workers (workgroups) for at most `units` units in shares of min_units at least.
@@ -108,6 +109,9 @@ int paged_tile_attention(const PagedAttnArgs& a, PagedAttnParams& p, const Paged
                          std::string& err);
 int paged_join_tile_attention(const PagedAttnArgs& a, PagedAttnParams& p, const PagedLaunch& l, hipStream_t stream,
                               std::string& err);
+// ... of few rows with their prefixes, in one launch
+int paged_join_stream_attention(const PagedAttnArgs& a, PagedAttnParams& p, hipStream_t stream, std::string& err);
+int64_t paged_join_cost(const PagedWork& w);
 // ... and what a launch of them may cost at most (paged_max_cost).
 int64_t paged_stream_cost(const PagedAttnArgs& a, const PagedWork& w);
 int64_t paged_tile_cost(const PagedAttnArgs& a, const PagedWork& w);

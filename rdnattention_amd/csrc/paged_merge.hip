@@ -129,6 +129,96 @@ __global__ __launch_bounds__(kMergeThreads) void paged_merge_rows(MergeParams p)
     }
 }
 
+// Workgroup x: row x % heads x of the call, all its parts (PagedParts), the prefix's and its
+// own, joined as above.  Garbage in `parts` (rows that no prefix's sequences have) leads to
+// no access outside the scratch.
+template <class T>
+__global__ __launch_bounds__(kMergeThreads) void paged_merge_parts(MergeParams p) {
+    using V4 = typename PagedVec<T>::v4;
+    __shared__ float wgt[2 * (kPagedMaxWorkers + 1)];
+    __shared__ __attribute__((aligned(16))) f4 red[kMergeThreads];
+    const PagedJoin& join = p.p.join;
+    const int row = blockIdx.x;
+    const int t = row / join.Hq, head = row - t * join.Hq;
+    if (t >= paged_rows_end(p.p.work.seqs)) {
+        return;
+    }
+    int32_t w[2], n[2], col[2];
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+        const PagedParts x = join.parts[k * join.rows + row];
+        w[k] = uniform(min(max(x.w, -1), p.n_wg - 1));
+        n[k] = uniform(w[k] < 0 ? 1 : min(max(x.w_last, w[k]), p.n_wg - 1) - w[k] + 1);
+        col[k] = uniform(min(max(x.col, 0), p.rows - 1));
+    }
+    const int parts = n[0] + n[1];
+    // part s: its O and (m, l)
+    auto at = [&](int s, const float*& o, const float2*& ml) {
+        const int k = s < n[0] ? 0 : 1;
+        s -= k == 0 ? 0 : n[0];
+        const int64_t r = w[k] < 0 ? (int64_t)k * join.rows + row
+                                   : (int64_t)(s == 0 ? p.n_wg + w[k] : w[k] + s) * p.rows + col[k];
+        o = (w[k] < 0 ? join.whole_o : p.p.part_o) + r * p.D;
+        ml = reinterpret_cast<const float2*>(w[k] < 0 ? join.whole_ml : p.p.part_ml) + r;
+    };
+    const int tid = threadIdx.x;
+    if (tid < 64) {
+        const float* o;
+        const float2* ml;
+        float mx = -INFINITY;
+        for (int s = tid; s < parts; s += 64) {
+            at(s, o, ml);
+            mx = fmaxf(mx, ml->y != 0.0f ? ml->x : -INFINITY);
+        }
+#pragma unroll
+        for (int off = 32; off > 0; off >>= 1) {
+            mx = fmaxf(mx, __shfl_xor(mx, off));
+        }
+        float sum = 0.0f;
+        for (int s = tid; s < parts; s += 64) {
+            at(s, o, ml);
+            const float2 v = *ml;
+            const float e = v.y != 0.0f ? part_weight(v.x, mx) : -1.0f;
+            sum += v.y != 0.0f ? v.y * e : 0.0f;
+            wgt[s] = e;
+        }
+#pragma unroll
+        for (int off = 32; off > 0; off >>= 1) {
+            sum += __shfl_xor(sum, off);
+        }
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        for (int s = tid; s < parts; s += 64) {
+            wgt[s] = wgt[s] < 0.0f ? -1.0f : wgt[s] * inv;
+        }
+        if (tid == 0 && join.lse != nullptr) {
+            join.lse[row] = sum == 0.0f ? -INFINITY : (mx + __builtin_amdgcn_logf(sum)) * 0.6931471805599453f;
+        }
+    }
+    __syncthreads();
+    const int E = p.D / 4;
+    const int per = kMergeThreads / E; // parts side by side
+    const int e = tid % E, sg = tid / E;
+    f4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (sg < per) {
+        for (int s = sg; s < parts; s += per) {
+            const float* o;
+            const float2* ml;
+            at(s, o, ml);
+            const f4 x = *reinterpret_cast<const f4*>(o + 4 * e);
+            acc += wgt[s] < 0.0f ? f4{0.0f, 0.0f, 0.0f, 0.0f} : x * wgt[s];
+        }
+    }
+    red[tid] = acc;
+    __syncthreads();
+    if (sg == 0) {
+        for (int i = 1; i < per && i < parts; i++) {
+            acc += red[i * E + e];
+        }
+        *reinterpret_cast<V4*>(p.p.o + (int64_t)t * p.p.o_st + head * p.p.o_sh + 8 * e) =
+            __builtin_convertvector(acc, V4);
+    }
+}
+
 } // namespace
 
 int paged_merge(const PagedAttnArgs& a, const PagedAttnParams& p, hipStream_t stream, std::string& err) {
@@ -141,6 +231,16 @@ int paged_merge(const PagedAttnArgs& a, const PagedAttnParams& p, hipStream_t st
     // few rows with many parts: a row per workgroup
     m.rpb = p.slot_rows <= 32 ? 1 : std::min({kMergeRows, kMergeThreads / (a.D / 4), kPagedMaxWorkers / m.n_wg});
     m.weights = kPagedMaxWorkers / m.rpb;
+    if (p.join.parts != nullptr) {
+        auto* const kernel = a.type == PagedType::F16 ? &paged_merge_parts<_Float16> : &paged_merge_parts<__bf16>;
+        hipLaunchKernelGGL(kernel, dim3((uint32_t)p.join.rows), dim3(kMergeThreads), 0, stream, m);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) {
+            err = hipGetErrorString(e);
+            return -1;
+        }
+        return 0;
+    }
     const dim3 grid((uint32_t)m.n_wg, (uint32_t)((m.rows + m.rpb - 1) / m.rpb));
     const bool join = p.join.any();
     auto* const kernel = a.type == PagedType::F16
@@ -189,28 +289,41 @@ int paged_attention(const PagedAttnArgs& a, hipStream_t stream, std::string& err
     if (any_many && any_few) {
         few.max_rows = many.min_rows = kFew;
     }
-    // The prefixes' rows are those of all their sequences: one launch, for all of them.
+    // The prefixes' rows are those of all their sequences.  Up to kShared of them per kv head (a
+    // row tile is 32, each of which reads the prefix again) and with few of every sequence, one
+    // launch has the prefixes and the sequences; else the prefixes have one, by tiles, of
+    // their own before the sequences'.
     PagedAttnParams shared = p;
-    const bool shared_many = (int64_t)a.seqs.total * p.work.G > kFew;
+    bool together = false;
     if (a.prefix.n > 0) {
-        shared.c.table = a.prefix.table;
-        shared.c.table_s = a.prefix.table_s;
-        shared.c.width = a.prefix.width;
-        shared.work.seqs.lens = a.prefix.lens;
-        shared.work.seqs.B = a.prefix.n;
-        shared.work.seqs.max_keys = (int32_t)((int64_t)a.prefix.width << a.c.lps);
-        shared.work.seqs.members = a.seqs.B;
-        shared.work.seqs.group = a.prefix.seqs;
-        shared.work.mask = PagedMask{0, 0};
-        shared.zero_tail = 0;
-        shared.join.lse = nullptr;
+        constexpr int64_t kShared = 512;
+        together = !any_many && (int64_t)a.seqs.total * p.work.G <= kShared;
+        PagedSeqs& s = shared.work.seqs;
+        s.prefixes = a.prefix.n;
+        s.members = a.seqs.B;
+        s.prefix_lens = a.prefix.lens;
+        s.prefix_keys = (int32_t)((int64_t)a.prefix.width << a.c.lps);
+        s.group = a.prefix.seqs;
+        s.B = a.prefix.n + (together ? a.seqs.B : 0);
+        if (!together) {
+            shared.c.table = a.prefix.table;
+            shared.c.table_s = a.prefix.table_s;
+            shared.c.width = a.prefix.width;
+            shared.work.mask = PagedMask{0, 0};
+            shared.zero_tail = 0;
+            shared.join.lse = nullptr;
+        }
     }
     // refused before the first of the launches has written anything
-    int64_t cost = std::max(any_many ? paged_tile_cost(a, paged_work(p.work, many)) : 0,
-                            any_few ? paged_stream_cost(a, paged_work(p.work, few)) : 0);
-    if (a.prefix.n > 0) {
-        const PagedWork w = paged_work(shared.work, PagedLaunch{});
-        cost = std::max(cost, shared_many ? paged_tile_cost(a, w) : paged_stream_cost(a, w));
+    int64_t cost;
+    if (together) {
+        cost = paged_join_cost(paged_work(shared.work, PagedLaunch{}));
+    } else {
+        cost = std::max(any_many ? paged_tile_cost(a, paged_work(p.work, many)) : 0,
+                        any_few ? paged_stream_cost(a, paged_work(p.work, few)) : 0);
+        if (a.prefix.n > 0) {
+            cost = std::max(cost, paged_tile_cost(a, paged_work(shared.work, PagedLaunch{})));
+        }
     }
     if (cost > INT32_MAX) {
         err = "too many rows x heads x keys that the page table covers (up to " +
@@ -218,8 +331,21 @@ int paged_attention(const PagedAttnArgs& a, hipStream_t stream, std::string& err
         return -1;
     }
     StreamScratch ws(ScratchUse::PagedPrefix);
+    const size_t rows = (size_t)a.seqs.total * a.Hq;
+    if (together) {
+        if (ws.alloc(2 * rows * ((a.D + 2) * sizeof(float) + sizeof(PagedParts)), stream, err) != 0) {
+            return -1;
+        }
+        shared.join.parts = static_cast<PagedParts*>(ws.ptr);
+        shared.join.whole_o = reinterpret_cast<float*>(shared.join.parts + 2 * rows);
+        shared.join.whole_ml = shared.join.whole_o + 2 * rows * a.D;
+        shared.join.prefix_table = a.prefix.table;
+        shared.join.prefix_table_s = a.prefix.table_s;
+        shared.join.prefix_width = a.prefix.width;
+        shared.join.rows = (int32_t)rows;
+        return paged_join_stream_attention(a, shared, stream, err);
+    }
     if (a.prefix.n > 0) {
-        const size_t rows = (size_t)a.seqs.total * a.Hq;
         if (ws.alloc(rows * (a.D + 1) * sizeof(float), stream, err) != 0) {
             return -1;
         }
@@ -227,7 +353,7 @@ int paged_attention(const PagedAttnArgs& a, hipStream_t stream, std::string& err
         shared.join.raw_l = shared.join.raw_o + rows * a.D;
         p.join.pre_o = shared.join.raw_o;
         p.join.pre_l = shared.join.raw_l;
-        if ((shared_many ? paged_tile_attention : paged_stream_attention)(a, shared, PagedLaunch{}, stream, err) != 0) {
+        if (paged_tile_attention(a, shared, PagedLaunch{}, stream, err) != 0) {
             return -1;
         }
     }

@@ -29,9 +29,13 @@ struct PagedSeqs {
     int32_t rows;
     int32_t total;    // rows of the query tensor
     int32_t max_keys; // keys that a row of the page table covers
-    // > 0: entry b stands for sequences group[b] .. group[b + 1] - 1 of so many (group
-    // null: for all of them), whose rows cu and `rows` give: those that share a prefix
+    // The first `prefixes` of the B entries are prefixes: entry b has prefix_lens[b] keys and the
+    // rows of sequences group[b] .. group[b + 1] - 1 of `members` (group null: of all of
+    // them), and the entries behind them are the sequences themselves.
+    int32_t prefixes = 0;
     int32_t members = 0;
+    int32_t prefix_keys = 0; // keys that a row of the prefixes' page table covers
+    const int32_t* prefix_lens = nullptr;
     const int32_t* group = nullptr;
 };
 
@@ -47,28 +51,37 @@ RDNA_MASK_FN int32_t rows_clamp(int32_t x, int32_t lo, int32_t hi) {
 
 // Rows that belong to a sequence: [0, paged_rows_end).
 RDNA_MASK_FN int32_t paged_rows_end(const PagedSeqs& s) {
-    return s.cu != nullptr ? rows_clamp(s.cu[s.B], 0, s.total) : s.total;
+    return s.cu != nullptr ? rows_clamp(s.cu[s.prefixes > 0 ? s.members : s.B], 0, s.total) : s.total;
 }
 
 RDNA_MASK_FN PagedSeq paged_seq(const PagedSeqs& s, int32_t b) {
     PagedSeq r;
     r.len = rows_clamp(s.lens[b], 0, s.max_keys);
-    if (s.members > 0) {
-        const int32_t first = s.group != nullptr ? rows_clamp(s.group[b], 0, s.members) : 0;
-        const int32_t end = s.group != nullptr ? rows_clamp(s.group[b + 1], first, s.members) : s.members;
-        if (s.cu != nullptr) {
-            r.q0 = rows_clamp(s.cu[first], 0, s.total);
-            r.n = rows_clamp(s.cu[end], r.q0, s.total) - r.q0;
-        } else {
-            r.q0 = first * s.rows;
-            r.n = (end - first) * s.rows;
-        }
-    } else if (s.cu != nullptr) {
+    if (s.cu != nullptr) {
         r.q0 = rows_clamp(s.cu[b], 0, s.total);
         r.n = rows_clamp(s.cu[b + 1], r.q0, s.total) - r.q0;
     } else {
         r.q0 = b * s.rows;
         r.n = s.rows;
+    }
+    return r;
+}
+
+// Entry b of those that prefixes begin.
+RDNA_MASK_FN PagedSeq paged_entry(const PagedSeqs& s, int32_t b) {
+    if (b >= s.prefixes) {
+        return paged_seq(s, b - s.prefixes);
+    }
+    PagedSeq r;
+    r.len = rows_clamp(s.prefix_lens[b], 0, s.prefix_keys);
+    const int32_t first = s.group != nullptr ? rows_clamp(s.group[b], 0, s.members) : 0;
+    const int32_t end = s.group != nullptr ? rows_clamp(s.group[b + 1], first, s.members) : s.members;
+    if (s.cu != nullptr) {
+        r.q0 = rows_clamp(s.cu[first], 0, s.total);
+        r.n = rows_clamp(s.cu[end], r.q0, s.total) - r.q0;
+    } else {
+        r.q0 = first * s.rows;
+        r.n = (end - first) * s.rows;
     }
     return r;
 }
@@ -178,6 +191,17 @@ RDNA_MASK_FN int32_t paged_head_units(const PagedWork& w, const PagedSeq& s) {
 // them `total` tokens.  Past 32 bits the walk cannot count it.
 template <int ROWS, int BN, int EXTRA>
 inline int64_t paged_max_cost(const PagedWork& w) {
+    if (w.seqs.prefixes > 0) { // the prefixes' entries have all rows too
+        PagedWork part = w;
+        part.seqs.prefixes = 0;
+        part.seqs.B = w.seqs.prefixes;
+        part.seqs.max_keys = w.seqs.prefix_keys;
+        const int64_t shared = paged_max_cost<ROWS, BN, EXTRA>(part);
+        part.seqs.B = w.seqs.B - w.seqs.prefixes;
+        part.seqs.max_keys = w.seqs.max_keys;
+        const int64_t own = paged_max_cost<ROWS, BN, EXTRA>(part);
+        return shared > INT32_MAX || own > INT32_MAX ? INT64_MAX : shared + own;
+    }
     const int64_t rows = (int64_t)w.seqs.total * w.G;
     const int64_t B = w.seqs.B;
     const int64_t seqs = rows / ((int64_t)w.min_rows + 1) < B ? rows / ((int64_t)w.min_rows + 1) : B;

@@ -1,0 +1,23 @@
+// Paged attention of few rows behind prefixes that sequences share.
+#include "paged_stream.hpp"
+
+namespace rdna_amd {
+
+int64_t paged_join_cost(const PagedWork& w) {
+    return paged_max_cost<kRows, kTile, kJoinCost>(w);
+}
+
+int paged_join_stream_attention(const PagedAttnArgs& a, PagedAttnParams& p, hipStream_t stream, std::string& err) {
+    return paged_for_type(a, [&](auto t, auto d, auto i8) {
+        using T = decltype(t);
+        constexpr int D = decltype(d)::value;
+        constexpr bool I8 = decltype(i8)::value;
+        constexpr int WV = D == 96 || D == 128 ? 8 : 4;
+        auto* const kernel = &paged_join_stream<T, D, I8, WV>;
+        return paged_launch<kRows, kTile, kJoinCost>(
+            a, reinterpret_cast<const void*>(kernel), 64 * WV, WV, p, PagedLaunch{}, stream, err,
+            [&](dim3 grid) { hipLaunchKernelGGL(kernel, grid, dim3(64 * WV), 0, stream, p); });
+    });
+}
+
+} // namespace rdna_amd

@@ -47,7 +47,7 @@
     }
     PagedRecord rec = {};
     // row tiles of one head, which read the same keys, through one L2
-    PagedWalk<C::ROWS, kBN, true, kItemCost> walk(p.work, by_xcd(blockIdx.x, p.work.n_wg));
+    PagedWalk<C::ROWS, kBN, true, kItemCost, JOIN> walk(p.work, by_xcd(blockIdx.x, p.work.n_wg));
 
     const int log_n = max(0, 6 - p.c.lps); // table entries of a tile
     const int log_b = 6 - log_n;           // tiles of a batch of 64

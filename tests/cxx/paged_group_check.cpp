@@ -1,4 +1,4 @@
-// paged_seq of entries that stand for groups of sequences: the rows of the group where
+// paged_entry of prefixes, which stand for groups of sequences, and of the sequences behind them: the rows of the group where
 // the arrays make sense, rows inside the tensors whatever they hold.
 #include "paged_rows.hpp"
 
@@ -48,12 +48,19 @@ int main() {
                 x = odd[pick(0, 6)];
             }
         }
-        PagedSeqs s{lens.data(), ragged ? cu.data() : nullptr, groups, rows, total, 80};
+        std::vector<int> own(seqs);
+        for (int& n : own) {
+            n = sane ? pick(0, 60) : pick(0, 1) != 0 ? INT_MAX : INT_MIN;
+        }
+        PagedSeqs s{own.data(), ragged ? cu.data() : nullptr, groups + seqs, rows, total, 50};
+        s.prefixes = groups;
         s.members = seqs;
+        s.prefix_keys = 80;
+        s.prefix_lens = lens.data();
         s.group = groups == 1 && pick(0, 1) != 0 ? nullptr : group.data();
         int next = 0;
         for (int g = 0; g < groups; g++) {
-            const PagedSeq r = paged_seq(s, g);
+            const PagedSeq r = paged_entry(s, g);
             CHECK(r.q0 >= 0 && r.n >= 0 && r.n <= total && r.q0 <= total - r.n);
             CHECK(r.len >= 0 && r.len <= 80);
             if (sane) {
@@ -62,6 +69,13 @@ int main() {
             }
             checked++;
         }
+        for (int b = 0; b < seqs; b++) {
+            const PagedSeq r = paged_entry(s, groups + b);
+            CHECK(r.q0 >= 0 && r.n >= 0 && r.n <= total && r.q0 <= total - r.n && r.len >= 0 && r.len <= 50);
+            CHECK(!sane || (r.q0 == cu[b] && r.n == cu[b + 1] - cu[b] && r.len == (own[b] < 50 ? own[b] : 50)));
+            checked++;
+        }
+        CHECK(!sane || paged_rows_end(s) == (ragged ? cu[seqs] : total));
         CHECK(!sane || next == (ragged ? cu[seqs] : total));
     }
     std::printf("ok %ld\n", checked);
