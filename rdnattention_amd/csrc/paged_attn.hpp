@@ -370,26 +370,31 @@ __device__ __forceinline__ int32_t by_xcd(int32_t id, int32_t n) {
 // cost: a worker with the many short row tiles at a prompt's begin has fewer key tiles.
 // PREFIXES: the first entries are prefixes (PagedSeqs), all keys of which all their rows see,
 // so that their row tiles are alike.
-template <int ROWS, int BN, bool MANY, int EXTRA, bool PREFIXES = false>
-struct PagedWalk {
+template <class Items, bool MANY, int EXTRA, bool PREFIXES>
+struct PagedItemWalk {
     const PagedWork& w;
     PagedShare<EXTRA> part; // the worker's share, and of the current item
     int32_t b = 0, h = 0, rt = 0, n_rt = 0;
     PagedSeq seq;
     PagedTile tile;
 
-    __device__ __forceinline__ PagedWalk(const PagedWork& work, int32_t worker) : w(work), part(work, uniform(worker)) {
+    __device__ __forceinline__ PagedItemWalk(const PagedWork& work, int32_t worker) : w(work), part(work, uniform(worker)) {
         const int lane = threadIdx.x & 63;
         const int32_t B = w.seqs.B;
         // sequence i and what one kv head of it costs
         auto cost_of = [&](int32_t i, PagedSeq& s) {
             s = i < B ? entry(i) : PagedSeq{0, 0, 0};
-            const int32_t n = paged_row_tiles<ROWS>(w, s.n);
+            const int32_t n = Items::count(w, s);
             int32_t u = 0;
             if (PREFIXES && i < w.seqs.prefixes) {
-                u = n * (prefix_tile(s).units + EXTRA);
+                if constexpr (PREFIXES) {
+                    u = n * (Items::all(s).units + EXTRA);
+                }
             } else if (!MANY || n <= kFewTiles) {
-                u = paged_head_units<ROWS, BN>(w, s) + n * EXTRA;
+                for (int32_t x = 0; x < n; x++) {
+                    u += Items::tile(w, s, x).units;
+                }
+                u += n * EXTRA;
             }
             if constexpr (MANY) {
                 for (uint64_t more = __builtin_amdgcn_ballot_w64(n > kFewTiles); more != 0; more &= more - 1) {
@@ -444,7 +449,7 @@ struct PagedWalk {
             part.left = 0;
             return;
         }
-        n_rt = uniform(paged_row_tiles<ROWS>(w, seq.n));
+        n_rt = uniform(Items::count(w, seq));
         h = uniform(part.enter(uniform(before), per_head, w.Hkv));
         rt = 0;
         int32_t at = part.at;
@@ -484,11 +489,11 @@ struct PagedWalk {
 
     // Cost of row tile i of n.
     __device__ __forceinline__ int32_t tile_cost(const PagedSeq& s, int32_t n, int32_t i) const {
-        return i < n ? paged_tile<ROWS, BN>(w, s, i).units + EXTRA : 0;
+        return i < n ? Items::tile(w, s, i).units + EXTRA : 0;
     }
     // Cost of one kv head of a sequence that is the same in every lane.
     __device__ __forceinline__ int32_t head_cost(const PagedSeq& s) const {
-        const int32_t n = paged_row_tiles<ROWS>(w, s.n);
+        const int32_t n = Items::count(w, s);
         int32_t u = 0;
         for (int32_t first = 0; first < n; first += 64) {
             u += tile_cost(s, n, first + (int)(threadIdx.x & 63));
@@ -514,17 +519,16 @@ struct PagedWalk {
         seq.q0 = uniform(seq.q0);
         seq.n = uniform(seq.n);
         seq.len = uniform(seq.len);
-        n_rt = uniform(paged_row_tiles<ROWS>(w, seq.n));
+        n_rt = uniform(Items::count(w, seq));
     }
     __device__ __forceinline__ PagedSeq entry(int32_t i) const {
         return PREFIXES ? paged_entry(w.seqs, i) : paged_seq(w.seqs, i);
     }
-    // Any row tile of a prefix.
-    __device__ __forceinline__ PagedTile prefix_tile(const PagedSeq& s) const {
-        return s.len > 0 ? PagedTile{0, s.len - 1, 0, (s.len + BN - 1) / BN} : PagedTile{0, -1, 0, 1};
-    }
     __device__ __forceinline__ void load_tile() {
-        tile = PREFIXES && b < w.seqs.prefixes ? prefix_tile(seq) : paged_tile<ROWS, BN>(w, seq, rt);
+        tile = Items::tile(w, seq, rt);
+        if constexpr (PREFIXES) {
+            tile = b < w.seqs.prefixes ? Items::all(seq) : tile;
+        }
         tile.lo = uniform(tile.lo);
         tile.hi = uniform(tile.hi);
         tile.first = uniform(tile.first);
@@ -573,6 +577,8 @@ struct PagedWalk {
         part.item(tile.units);
     }
 };
+template <int ROWS, int BN, bool MANY, int EXTRA, bool PREFIXES = false>
+using PagedWalk = PagedItemWalk<PagedRowItems<ROWS, BN>, MANY, EXTRA, PREFIXES>;
 
 // Masks the scores s[0 .. 16 N - 1] of keys key0 + 32 (e / 16) + 8 (e % 16 / 4) + e
 // % 4 that row `row` of the mask (n columns, drafts from `prefix` on) does not see.

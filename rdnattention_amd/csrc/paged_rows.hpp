@@ -186,6 +186,36 @@ RDNA_MASK_FN int32_t paged_head_units(const PagedWork& w, const PagedSeq& s) {
     return u;
 }
 
+// Items of a call: of a sequence and kv head its row tiles, whose units are key tiles.
+template <int ROWS, int BN>
+struct PagedRowItems {
+    static RDNA_MASK_FN int32_t count(const PagedWork& w, const PagedSeq& s) {
+        return paged_row_tiles<ROWS>(w, s.n);
+    }
+    static RDNA_MASK_FN PagedTile tile(const PagedWork& w, const PagedSeq& s, int32_t i) {
+        return paged_tile<ROWS, BN>(w, s, i);
+    }
+    // any of those whose rows see all keys
+    static RDNA_MASK_FN PagedTile all(const PagedSeq& s) {
+        return s.len > 0 ? PagedTile{0, s.len - 1, 0, (s.len + BN - 1) / BN} : PagedTile{0, -1, 0, 1};
+    }
+};
+
+// ... or its blocks of BLOCK keys, whose units are the tiles of ROWS rows that see some key
+// of theirs; lo .. hi are rows.
+template <int BLOCK, int ROWS>
+struct PagedKeyItems {
+    static RDNA_MASK_FN int32_t count(const PagedWork& w, const PagedSeq& s) {
+        const int32_t rows = s.n * w.G;
+        return rows > w.min_rows && rows <= w.max_rows ? (s.len + BLOCK - 1) / BLOCK : 0;
+    }
+    static RDNA_MASK_FN PagedTile tile(const PagedWork& w, const PagedSeq& s, int32_t i) {
+        const int32_t lo = paged_key_rows(w.mask, s, w.G, i * BLOCK).lo;
+        const int32_t hi = paged_key_rows(w.mask, s, w.G, mask_imin((i + 1) * BLOCK, s.len) - 1).hi;
+        return lo <= hi ? PagedTile{lo, hi, lo / ROWS, hi / ROWS + 1 - lo / ROWS} : PagedTile{0, -1, 0, 1};
+    }
+};
+
 // Most that the items of a call may cost (see PagedShare), whatever the lengths: the
 // sequences of a launch have more than min_rows and at most max_rows rows each, all of
 // them `total` tokens.  Past 32 bits the walk cannot count it.
@@ -209,6 +239,16 @@ inline int64_t paged_max_cost(const PagedWork& w) {
     const int64_t tiles = rows / ROWS + seqs < seqs * each ? rows / ROWS + seqs : seqs * each;
     const int64_t heads = tiles * w.Hkv;
     return heads <= INT32_MAX ? heads * (w.seqs.max_keys / BN + 1 + EXTRA) : INT64_MAX;
+}
+
+// ... and those of blocks of keys.
+template <int BLOCK, int ROWS, int EXTRA>
+inline int64_t paged_max_key_cost(const PagedWork& w) {
+    const int64_t rows = (int64_t)w.seqs.total * w.G;
+    const int64_t B = w.seqs.B;
+    const int64_t seqs = rows / ((int64_t)w.min_rows + 1) < B ? rows / ((int64_t)w.min_rows + 1) : B;
+    const int64_t heads = (rows / ROWS + seqs * (2 + EXTRA)) * w.Hkv; // row tiles, whole or cut, and EXTRA
+    return heads <= INT32_MAX ? heads * (w.seqs.max_keys / BLOCK + 1) : INT64_MAX;
 }
 
 // Cost of each worker's share of `total`.

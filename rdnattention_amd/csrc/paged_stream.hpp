@@ -34,7 +34,7 @@ constexpr int kManyHeads = 512; // kv heads of all sequences: two per CU
 constexpr float kRescale = 8.0f;
 constexpr int kDepth = 4; // MFMA operands in flight
 // paged_join_stream: what an item's begin and end cost, in key tiles of the workgroup
-constexpr int kJoinCost = 16;
+constexpr int kJoinCost = 24;
 
 template <int D, bool I8, int WV>
 struct StreamCfg {

@@ -4,7 +4,8 @@
 //
 // The keys are the lanes of the matrix products (S = Q K^T, a row of Q to a register),
 // so that a key's sum stays in its lane, whatever its page holds reaches no other key,
-// and no two workgroups share a key: no atomics, no scratch, the same bits every time.
+// and two workgroups that share a key leave their sums in order: no atomics, the same bits
+// every time.
 //   * few rows (up to 32 of a kv head): bound by HBM, K is read once.  The waves take 32-key
 //     tiles, straight into the MFMA layout, one tile ahead
 //   * more rows: bound by the exponentials beside the products.  A workgroup keeps a block of
@@ -30,7 +31,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 
 struct WeightsParams {
     PagedPages c;
-    PagedWork work; // its mask hides nothing: every key has a weight
+    PagedWork work; // of few rows without a mask: every key has a weight
     PagedMask mask;
     const char* q;
     int64_t q_st, q_sh; // bytes
@@ -41,6 +42,10 @@ struct WeightsParams {
     float decay;
     float* w;
     int64_t w_sp, w_st, w_sh;
+    // blocks of keys that several workers share: sums by slot, as in PagedRecord, whose q0 is
+    // the sequence and r0 the first key
+    float* parts;
+    PagedRecord* records;
 };
 
 // A row's log-sum-exp in log2 units, as what is subtracted in the exponent and a factor
@@ -220,13 +225,14 @@ __global__ __launch_bounds__(256) void paged_weights_few(WeightsParams p) {
     }
 }
 
-template <int D>
+template <int D, bool I8>
 struct ManyCfg {
     static constexpr int WAVES = 4;
     static constexpr int THREADS = 64 * WAVES;
-    static constexpr int KT = D <= 96 ? 4 : D <= 128 ? 3 : 2; // 32-key tiles in registers
+    static constexpr int KT = D <= 96 ? 4 : D <= 128 && !I8 ? 3 : 2; // 32-key tiles in registers
     static constexpr int BLOCK = kTile * KT;
     static constexpr int WAVES_PER_SIMD = D <= 128 ? 2 : 1;
+    static constexpr int COST = 8; // of an item beside its row tiles
     static constexpr int RB = 2 * D;
     static constexpr int KCH = D / 8;
     static constexpr int Q_BYTES = kTile * RB;
@@ -236,9 +242,9 @@ struct ManyCfg {
 };
 
 template <class T, int D, bool I8>
-__global__ __launch_bounds__((ManyCfg<D>::THREADS), (ManyCfg<D>::WAVES_PER_SIMD)) void paged_weights_many(
+__global__ __launch_bounds__((ManyCfg<D, I8>::THREADS), (ManyCfg<D, I8>::WAVES_PER_SIMD)) void paged_weights_many(
     WeightsParams p) {
-    using C = ManyCfg<D>;
+    using C = ManyCfg<D, I8>;
     using V8 = typename PagedVec<T>::v8;
     __shared__ __attribute__((aligned(16))) char dsm[C::LDS_BYTES];
     __shared__ float sums[C::WAVES][C::BLOCK];
@@ -250,20 +256,18 @@ __global__ __launch_bounds__((ManyCfg<D>::THREADS), (ManyCfg<D>::WAVES_PER_SIMD)
     char* const qsm = dsm + wave * 2 * C::Q_BYTES;
     float* const lsm = reinterpret_cast<float*>(dsm + C::WAVES * 2 * C::Q_BYTES) + wave * 2 * kTile;
 
-    PagedWalk<kAllRows, C::BLOCK, false, 0> walk(p.work, by_xcd(blockIdx.x, p.work.n_wg));
+    PagedItemWalk<PagedKeyItems<C::BLOCK, kTile>, true, C::COST, false> walk(p.work, by_xcd(blockIdx.x, p.work.n_wg));
+    PagedRecord rec = {};
     while (walk.more()) {
         const PagedSeq seq = walk.seq;
         const int h = uniform(walk.h), G = p.work.G;
         const int rows = uniform(seq.n * G);
-        const int nt = uniform(walk.tile.hi >= walk.tile.lo ? walk.count() : 0);
         const int32_t* const table = p.c.table + walk.b * p.c.table_s;
-        for (int u = 0; u < nt; u++) {
-            const int key0 = uniform(walk.tile.first + walk.begin() + u) * C::BLOCK;
-            const int last = min(key0 + C::BLOCK, seq.len) - 1;
-            // row tiles that some key of the block is seen by
-            const int r_lo = uniform(paged_key_rows(p.mask, seq, G, key0).lo);
-            const int r_hi = uniform(paged_key_rows(p.mask, seq, G, last).hi);
-            const int rt0 = r_lo / kTile, rt1 = r_hi < 0 ? -1 : r_hi / kTile;
+        {
+            const int key0 = uniform(walk.rt) * C::BLOCK;
+            // this share's of the row tiles that some key of the block is seen by
+            const int rt0 = uniform(walk.tile.first + walk.begin());
+            const int rt1 = uniform(walk.tile.hi >= walk.tile.lo ? rt0 + walk.count() - 1 : rt0 - 1);
 
             // row of a tile that this lane loads
             float lse_next = 0.0f;
@@ -350,32 +354,75 @@ __global__ __launch_bounds__((ManyCfg<D>::THREADS), (ManyCfg<D>::WAVES_PER_SIMD)
             }
             __syncthreads();
             if (tid < C::BLOCK) {
-                const LaneKey key = lane_key<false>(p, seq, table, h, key0 + tid);
                 float x = 0.0f;
 #pragma unroll
                 for (int w = 0; w < C::WAVES; w++) {
                     x += sums[w][tid];
                 }
-                if (key.w != nullptr) {
-                    *key.w = new_weight(p, key, x, key.old ? *key.w : 0.0f);
+                if (walk.whole()) {
+                    const LaneKey key = lane_key<false>(p, seq, table, h, key0 + tid);
+                    if (key.w != nullptr) {
+                        *key.w = new_weight(p, key, x, key.old ? *key.w : 0.0f);
+                    }
+                } else {
+                    p.parts[(int64_t)walk.slot() * C::BLOCK + tid] = x;
                 }
+            }
+            if (!walk.whole() && walk.begin() == 0) {
+                rec = PagedRecord{C::BLOCK, walk.b, key0, h, walk.last_wg(), {}};
             }
             __syncthreads(); // before the sums of the next block
         }
         walk.next();
     }
+    if (tid == 0) {
+        p.records[walk.part.wg] = rec;
+    }
+}
+
+// Workgroup w: the block that starts in worker w's share and goes on behind it, if there is
+// one: its parts' sums, in order.
+__global__ __launch_bounds__(128) void paged_weights_merge(WeightsParams p) {
+    const int w = blockIdx.x;
+    const PagedRecord rec = p.records[w];
+    const int i = threadIdx.x;
+    if (i >= rec.rows) {
+        return;
+    }
+    const PagedSeq seq = paged_seq(p.work.seqs, rec.q0);
+    const LaneKey key = lane_key<false>(p, seq, p.c.table + rec.q0 * p.c.table_s, rec.h, rec.r0 + i);
+    const float old = key.w != nullptr && key.old ? *key.w : 0.0f;
+    float sum = p.parts[(int64_t)(p.work.n_wg + w) * rec.rows + i];
+    for (int s = w + 1; s <= rec.w_last; s++) {
+        sum += p.parts[(int64_t)s * rec.rows + i];
+    }
+    if (key.w != nullptr) {
+        *key.w = new_weight(p, key, sum, old);
+    }
 }
 
 template <class T, int D, bool I8>
 int launch_weights(const PagedWeightsArgs& a, WeightsParams& p, hipStream_t stream, std::string& err) {
-    auto go = [&](auto* kernel, int threads, int64_t units, int min_units) {
+    auto go = [&](auto* kernel, int threads, int64_t units, int min_units, int block) {
         const int64_t resident = resident_workgroups(reinterpret_cast<const void*>(kernel), threads, err);
         if (resident <= 0) {
             return -1;
         }
         p.work.min_units = min_units;
         p.work.n_wg = paged_workgroups(resident, units, min_units);
+        StreamScratch ws(ScratchUse::PagedPartials);
+        if (block > 0) {
+            const size_t sums = (size_t)2 * p.work.n_wg * block * sizeof(float);
+            if (ws.alloc(sums + p.work.n_wg * sizeof(PagedRecord), stream, err) != 0) {
+                return -1;
+            }
+            p.parts = static_cast<float*>(ws.ptr);
+            p.records = reinterpret_cast<PagedRecord*>(static_cast<char*>(ws.ptr) + sums);
+        }
         hipLaunchKernelGGL(kernel, dim3((uint32_t)p.work.n_wg), dim3(threads), 0, stream, p);
+        if (block > 0) {
+            hipLaunchKernelGGL(paged_weights_merge, dim3((uint32_t)p.work.n_wg), dim3(128), 0, stream, p);
+        }
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) {
             err = hipGetErrorString(e);
@@ -390,22 +437,24 @@ int launch_weights(const PagedWeightsArgs& a, WeightsParams& p, hipStream_t stre
     if (any_many && any_few) {
         few.max_rows = many.min_rows = kFewRows;
     }
-    const PagedWork wf = paged_work(p.work, few), wm = paged_work(p.work, many);
+    PagedWork wf = paged_work(p.work, few), wm = paged_work(p.work, many);
+    wm.mask = p.mask;
     const int64_t cf = any_few ? paged_max_cost<kAllRows, kTile, 0>(wf) : 0;
-    const int64_t cm = any_many ? paged_max_cost<kAllRows, ManyCfg<D>::BLOCK, 0>(wm) : 0;
+    using C = ManyCfg<D, I8>;
+    const int64_t cm = any_many ? paged_max_key_cost<C::BLOCK, kTile, C::COST>(wm) : 0;
     if (std::max(cf, cm) > INT32_MAX) {
-        err = "too many sequences x heads x keys that the page table covers (at most 2^31 - 1 key tiles)";
+        err = "too many rows x heads x keys that the page table covers (at most 2^31 - 1 key tiles)";
         return -1;
     }
     if (any_many) {
         p.work = wm;
-        if (go(&paged_weights_many<T, D, I8>, ManyCfg<D>::THREADS, cm, 1) != 0) {
+        if (go(&paged_weights_many<T, D, I8>, C::THREADS, cm, 2 * C::COST, C::BLOCK) != 0) {
             return -1;
         }
     }
     if (any_few) {
         p.work = wf;
-        return go(&paged_weights_few<T, D, I8>, 256, cf, 4);
+        return go(&paged_weights_few<T, D, I8>, 256, cf, 4, 0);
     }
     return 0;
 }

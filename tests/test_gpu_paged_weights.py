@@ -218,7 +218,10 @@ def test_pages_outside_the_cache(gpu, ns, i8):
     for b in range(3):
         pg, off = (i.to(gpu) for i in pool.where(b, torch.arange(pool.lens[b])))
         if b != 1:
-            assert torch.equal(bad[pg, off], good[pg, off])
+            # other lengths are other shares: the same weights, none negative, summed in another
+            # order, each order off by at most (rows x heads / 16 + 8) 2^-24 (see reference)
+            off_by = 2 * (ns[b] * 2 / 16 + 8) * 2.0 ** -24 * good[pg, off]
+            assert ((bad[pg, off] - good[pg, off]).abs() <= off_by).all()
         else:
             gone = (torch.arange(64, device=gpu) // 16 == 0) | (torch.arange(64, device=gpu) // 16 == 2)
             assert torch.equal(bad[pg, off][gone], before[pg, off][gone])
