@@ -144,6 +144,13 @@ __device__ __forceinline__ int paged_swz(int r) {
     }
 }
 
+// 16-byte chunk swizzle of row r of an int8 tile: rows of 64 or 128 bytes, the 64
+// banks 256, so rows r and r + 4 or r + 2 start in the same bank
+template <int D>
+__device__ __forceinline__ int swz8(int r) {
+    return D == 64 ? (r >> 2) & 3 : (r >> 1) & 7;
+}
+
 // A row of zeros: stands for keys that no row of the item sees, so that what the
 // pages hold there (a key behind the sequence's last may be anything) never
 // meets a weight of zero as infinity or NaN.

@@ -65,13 +65,6 @@ struct StreamCfg {
     static_assert(K_COPIES + V_COPIES + 1 < 64, "vmcnt counts them");
 };
 
-// 16-byte chunk swizzle of row r of an int8 tile: rows of 64 or 128 bytes, the 64
-// banks 256, so rows r and r + 4 or r + 2 start in the same bank
-template <int D>
-__device__ __forceinline__ int swz8(int r) {
-    return D == 64 ? (r >> 2) & 3 : (r >> 1) & 7;
-}
-
 template <class T, int D, bool I8, int WV>
 __global__ __launch_bounds__((StreamCfg<D, I8, WV>::THREADS), (StreamCfg<D, I8, WV>::WAVES_PER_SIMD)) void paged_stream(
     PagedAttnParams p) {

@@ -6,8 +6,7 @@
 // so that a key's sum stays in its lane, whatever its page holds reaches no other key,
 // and two workgroups that share a key leave their sums in order: no atomics, the same bits
 // every time.
-//   * few rows (up to 32 of a kv head): bound by HBM, K is read once.  The waves take 32-key
-//     tiles, straight into the MFMA layout, one tile ahead
+//   * few rows (up to 32 of a kv head): bound by HBM, K is read once
 //   * more rows: bound by the exponentials beside the products.  A workgroup keeps a block of
 //     keys in registers and its waves take the row tiles in turn, Q through LDS one tile
 //     ahead
@@ -36,7 +35,7 @@ struct WeightsParams {
     const char* q;
     int64_t q_st, q_sh; // bytes
     const float* lse;
-    int32_t Hq;
+    int32_t Hq, Hkv;
     float scale_log2e; // |scale| log2(e)
     float q_sign;
     float decay;
@@ -61,31 +60,30 @@ __device__ __forceinline__ RowLse row_lse(float lse) {
     return lse == -INFINITY ? RowLse{INFINITY, 1.0f} : RowLse{hi, fast_exp2(-lo)};
 }
 
-// What a lane needs of key `key`: where its row and weight are, and which rows see it.
+// What a lane needs of key `key`, given its entry of the page table.
 struct LaneKey {
     const char* k;
     float* w;      // null: no key, or no page
     float k_scale; // int8 pages
-    PagedKeyRows rows;
-    bool old;
 };
 
+__device__ __forceinline__ int32_t key_entry(const WeightsParams& p, const PagedSeq& seq, const int32_t* table,
+                                             int key) {
+    return key < seq.len ? paged_page(p.c, table, key >> p.c.lps) : -1;
+}
+
 template <bool I8>
-__device__ __forceinline__ LaneKey lane_key(const WeightsParams& p, const PagedSeq& seq, const int32_t* table, int h,
-                                            int key) {
+__device__ __forceinline__ LaneKey lane_key(const WeightsParams& p, int32_t entry, int h, int key) {
     LaneKey r;
-    const int32_t pg = key < seq.len ? paged_page(p.c, table, key >> p.c.lps) : -1;
-    const int64_t page = pg >= 0 ? pg : 0;
+    const int64_t page = entry >= 0 ? entry : 0;
     const int64_t off = key & ((1 << p.c.lps) - 1);
-    r.k = pg >= 0 ? p.c.k + page * p.c.k_sp + off * p.c.k_st + h * p.c.k_sh
-                  : reinterpret_cast<const char*>(kPagedZeroRow);
-    r.w = pg >= 0 ? p.w + page * p.w_sp + off * p.w_st + h * p.w_sh : nullptr;
+    r.k = entry >= 0 ? p.c.k + page * p.c.k_sp + off * p.c.k_st + h * p.c.k_sh
+                     : reinterpret_cast<const char*>(kPagedZeroRow);
+    r.w = entry >= 0 ? p.w + page * p.w_sp + off * p.w_st + h * p.w_sh : nullptr;
     r.k_scale = 1.0f;
     if constexpr (I8) {
-        r.k_scale = pg >= 0 ? p.c.ks[page * p.c.ks_sp + off * p.c.ks_st + h * p.c.ks_sh] : 0.0f;
+        r.k_scale = entry >= 0 ? p.c.ks[page * p.c.ks_sp + off * p.c.ks_st + h * p.c.ks_sh] : 0.0f;
     }
-    r.rows = paged_key_rows(p.mask, seq, p.work.G, key);
-    r.old = key < seq.len - seq.n;
     return r;
 }
 
@@ -133,29 +131,132 @@ __device__ __forceinline__ float sum_weights(const f16x& s, float c, const f4 (&
     return (part[0] + part[1]) + (part[2] + part[3]);
 }
 
-__device__ __forceinline__ float new_weight(const WeightsParams& p, const LaneKey& k, float sum, float old) {
-    return k.old && p.decay != 0.0f ? fmaf(p.decay, old, sum) : sum;
+// The weight of a key from before the newest rows (is_old), or of one of theirs.
+__device__ __forceinline__ float new_weight(const WeightsParams& p, bool is_old, float sum, float old) {
+    return is_old && p.decay != 0.0f ? fmaf(p.decay, old, sum) : sum;
 }
 
+// Few rows.  The waves of a workgroup have the kv heads, eight at a time, of the same 32 keys
+// (and of the next 32 where there are fewer heads), since the keys of a token lie side by
+// side and a line of weights holds those of its heads.  Keys come by non-temporal HBM ->
+// LDS copies, one tile ahead, each of whole rows, and so do the old weights, the scales
+// of int8 and, 64 at a time, the page table's entries: no wait of the compiler's drains them.
+// us for 16 bf16 sequences of 4000 to 32768 keys, 8 heads, D = 128: 107; with a workgroup's
+// waves on one head 146 (30 of it for the weights' lines), keys loaded straight into the
+// MFMA layout (32 bytes of each of 32 rows at a time) 133 to 137, one to three tiles ahead.
+template <int D, bool I8>
+struct FewCfg {
+    static constexpr int WAVES = D <= 128 ? 8 : 4;
+    static constexpr int RB = I8 ? D : 2 * D; // row bytes
+    static constexpr int KCH = RB / 16;
+    static constexpr int TILE_BYTES = kTile * RB;
+    static constexpr int DMA = TILE_BYTES / 1024;
+    // two tiles; two batches of 64 table entries; of both tiles 32 old weights and 32 scales;
+    // row addresses; the rows' log-sum-exps
+    static constexpr int TABS = 2 * TILE_BYTES, AUX = TABS + 2 * 256, ROWS = AUX + 2 * 256, LSE = ROWS + 256;
+    static constexpr int WAVE_BYTES = LSE + 256;
+    static_assert(WAVES * WAVE_BYTES <= 160 * 1024, "tiles fit the LDS");
+};
+
 template <class T, int D, bool I8>
-__global__ __launch_bounds__(256) void paged_weights_few(WeightsParams p) {
+__global__ __launch_bounds__((64 * FewCfg<D, I8>::WAVES)) void paged_weights_few(WeightsParams p) {
+    using C = FewCfg<D, I8>;
     using V8 = typename PagedVec<T>::v8;
-    constexpr int NS = D / 16;
-    __shared__ __attribute__((aligned(16))) float rows_lse[4][2][kTile];
+    constexpr int NS = D / 16, WAVES = C::WAVES;
+    __shared__ __attribute__((aligned(16))) char dsm[WAVES * C::WAVE_BYTES];
     const int wave = uniform(threadIdx.x >> 6);
     const int lane = threadIdx.x & 63;
     const int l32 = lane & 31, g = lane >> 5;
-    PagedWalk<kAllRows, kTile, false, 0> walk(p.work, I8 ? by_xcd(blockIdx.x, p.work.n_wg) : (int32_t)blockIdx.x);
+    char* const wsm = dsm + wave * C::WAVE_BYTES;
+    const uint32_t lds_w = (uint32_t)reinterpret_cast<uintptr_t>(wsm);
+    uint64_t* const rows_at = reinterpret_cast<uint64_t*>(wsm + C::ROWS);
+    float* const rows_lse = reinterpret_cast<float*>(wsm + C::LSE);
+    const int side = min(p.Hkv, WAVES); // heads side by side,
+    const int step = WAVES / side;      // and tiles
+    const int slot = wave / side;
+    const uint32_t page_mask = (1u << p.c.lps) - 1u;
+    const uint64_t zero = reinterpret_cast<uint64_t>(kPagedZeroRow);
+    // lane i of copy d writes bytes 1024 d + 16 i of a tile: stored chunk n % KCH of row n /
+    // KCH, n = 64 d + i, which holds chunk (n % KCH) ^ swz(row)
+    uint32_t src[C::DMA]; // row * 8 | chunk byte << 16
+#pragma unroll
+    for (int d = 0; d < C::DMA; d++) {
+        const int n = 64 * d + lane;
+        const int r = n / C::KCH;
+        src[d] = (uint32_t)(r * 8) | (uint32_t)(((n - r * C::KCH) ^ (I8 ? swz8<D>(r) : paged_swz<D>(r))) * 16) << 16;
+    }
+    const int log_n = max(0, 5 - p.c.lps); // table entries of a tile
+    const int log_b = 6 - log_n;           // tiles of a batch of 64
+    PagedWalk<kAllRows, kTile, false, 0> walk(p.work, by_xcd(blockIdx.x, p.work.n_wg));
     while (walk.more()) {
         const PagedSeq seq = walk.seq;
-        const int h = uniform(walk.h), G = p.work.G;
+        const int G = p.work.G;
+        const int h = uniform(walk.h) * WAVES + wave - slot * side;
         const int rows = uniform(seq.n * G);
         const int t0 = uniform(walk.tile.first + walk.begin());
-        const int nt = uniform(walk.tile.hi >= walk.tile.lo ? walk.count() : 0);
-        const int32_t* const table = p.c.table + walk.b * p.c.table_s;
+        const int nt = uniform(walk.tile.hi >= walk.tile.lo && slot < step && h < p.Hkv ? walk.count() : 0);
+        const int mine = nt > slot ? (nt - slot + step - 1) / step : 0;
+        auto tile_key = [&](int j) { return (t0 + slot + step * j) * kTile; };
+        i32x4_t tab_rsrc = make_rsrc_v(p.c.table + walk.b * p.c.table_s, (uint32_t)p.c.width * 4u);
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            tab_rsrc[e] = uniform(tab_rsrc[e]);
+        }
+        auto issue_tab = [&](int batch) __attribute__((always_inline)) {
+            const int t = (batch << log_b) + (lane >> log_n);
+            const int key = tile_key(t) + ((lane & ((1 << log_n) - 1)) << p.c.lps);
+            dma_load4(tab_rsrc, (uint32_t)(key >> p.c.lps) * 4u,
+                      (uint32_t)uniform((int)lds_w + C::TABS + 256 * (batch & 1)));
+        };
 
         // one row tile (more only where the caller has said that there were fewer rows)
-        for (int base = 0; base < rows; base += kTile) {
+        for (int base = 0; base < rows && mine > 0; base += kTile) {
+            const bool later = base > 0;
+            // Of tile j: the keys' rows, and from lanes 0 - 31 their weights, from the others their
+            // scales.  `w` is where the lane's key has its weight, 0 for none.
+            uint64_t w = 0, w_next = 0, small = 0;
+            auto find = [&](int j) __attribute__((always_inline)) {
+                const int key = tile_key(j) + l32;
+                const uint32_t pg = reinterpret_cast<const uint32_t*>(
+                    wsm + C::TABS)[64 * ((j >> log_b) & 1) + ((j & ((1 << log_b) - 1)) << log_n) + (l32 >> p.c.lps)];
+                const bool there = key < seq.len && pg < (uint32_t)p.c.pages;
+                const uint64_t pe = there ? pg : 0u;
+                const uint64_t off = (uint32_t)key & page_mask;
+                const uint64_t row = reinterpret_cast<uint64_t>(p.c.k) + pe * (uint64_t)p.c.k_sp +
+                                     off * (uint64_t)p.c.k_st + (uint64_t)h * (uint64_t)p.c.k_sh;
+                rows_at[l32] = there ? row : zero;
+                w_next = there ? reinterpret_cast<uint64_t>(p.w) + 4 * (pe * (uint64_t)p.w_sp + off * (uint64_t)p.w_st +
+                                                                        (uint64_t)h * (uint64_t)p.w_sh)
+                               : 0;
+                small = g == 0 && w_next != 0 && (later || key < seq.len - seq.n) ? w_next : zero;
+                if constexpr (I8) {
+                    const uint64_t at = reinterpret_cast<uint64_t>(p.c.ks) +
+                                        4 * (pe * (uint64_t)p.c.ks_sp + off * (uint64_t)p.c.ks_st +
+                                             (uint64_t)h * (uint64_t)p.c.ks_sh);
+                    small = g == 0 ? small : there ? at : zero;
+                }
+            };
+            auto issue = [&](int j) __attribute__((always_inline)) {
+                const uint32_t to = lds_w + (uint32_t)(j & 1) * C::TILE_BYTES;
+                uint64_t from[C::DMA];
+#pragma unroll
+                for (int d = 0; d < C::DMA; d++) {
+                    from[d] = *reinterpret_cast<const uint64_t*>(reinterpret_cast<const char*>(rows_at) +
+                                                                 (src[d] & 0xffffu)) +
+                              (src[d] >> 16);
+                }
+#pragma unroll
+                for (int d = 0; d < C::DMA; d++) {
+                    dma_gather16_nt(from[d], to + 1024 * d);
+                }
+                dma_gather4(small, lds_w + C::AUX + 256 * (j & 1));
+            };
+            issue_tab(0);
+            issue_tab(1);
+            __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
+            find(0);
+            issue(0);
+
             const bool valid = base + l32 < rows;
             const int tok = valid ? (base + l32) / G : 0;
             const int head = h * G + (valid ? base + l32 - tok * G : 0);
@@ -164,62 +265,68 @@ __global__ __launch_bounds__(256) void paged_weights_few(WeightsParams p) {
                 const char* const row = p.q + (int64_t)(seq.q0 + tok) * p.q_st + head * p.q_sh;
 #pragma unroll
                 for (int s = 0; s < NS; s++) {
-                    const V8 x = *reinterpret_cast<const V8*>(row + 16 * chunk_of_q<I8>(s, g));
-                    q[s] = valid ? (p.q_sign < 0.0f ? -x : x) : V8{};
+                    const V8 v = *reinterpret_cast<const V8*>(row + 16 * chunk_of_q<I8>(s, g));
+                    q[s] = valid ? (p.q_sign < 0.0f ? -v : v) : V8{};
                 }
                 const RowLse r = row_lse(valid ? p.lse[(int64_t)(seq.q0 + tok) * p.Hq + head] : -INFINITY);
-                rows_lse[wave][0][l32] = r.sub;
-                rows_lse[wave][1][l32] = r.factor;
+                rows_lse[l32] = r.sub;
+                rows_lse[kTile + l32] = r.factor;
             }
             f4 sub[4], factor[4];
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                sub[i] = *reinterpret_cast<const f4*>(&rows_lse[wave][0][8 * i + 4 * g]);
-                factor[i] = *reinterpret_cast<const f4*>(&rows_lse[wave][1][8 * i + 4 * g]);
+                sub[i] = *reinterpret_cast<const f4*>(rows_lse + 8 * i + 4 * g);
+                factor[i] = *reinterpret_cast<const f4*>(rows_lse + kTile + 8 * i + 4 * g);
             }
-            auto key_of = [&](int j) { return (t0 + wave + 4 * j) * kTile + l32; };
-            const int mine = nt > wave ? (nt - wave + 3) / 4 : 0;
-            KeyRegs<D, I8> k0, k1;
-            LaneKey a, b;
-            auto tile = [&](const LaneKey& key, const KeyRegs<D, I8>& k) __attribute__((always_inline)) {
-                const bool later = base > 0;
-                const float old = g == 0 && key.w != nullptr && (key.old || later) ? *key.w : 0.0f;
-                f16x s = f16x{};
-#pragma unroll
-                for (int i = 0; i < NS; i++) {
-                    s = paged_mfma<T>(q[i], k.template operand<T>(i), s);
-                }
-                const float c = p.scale_log2e * key.k_scale;
-                const int lo = key.rows.lo - base - 4 * g, hi = key.rows.hi - base - 4 * g;
-                float sum;
-                if (wave_any(key.rows.lo > base || key.rows.hi < base + kTile - 1)) {
-                    sum = sum_weights<true>(s, c, sub, factor, lo, hi, 0.0f);
+            __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
+            for (int j = 0; j < mine; j++) {
+                w = w_next;
+                if (j + 1 < mine) {
+                    find(j + 1);
+                    // the batch in front is done with; it lands before tile j + 1 does
+                    if (((j + 1) & ((1 << log_b) - 1)) == 0) {
+                        issue_tab(((j + 1) >> log_b) + 1);
+                    }
+                    __builtin_amdgcn_s_waitcnt(waitcnt_lgkm(0)); // every read of tile j - 1 has returned
+                    issue(j + 1);
+                    __builtin_amdgcn_s_waitcnt(waitcnt_vm(C::DMA + 1)); // tile j has landed
                 } else {
-                    sum = sum_weights<false>(s, c, sub, factor, lo, hi, 0.0f);
+                    __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
+                }
+                asm volatile("" ::: "memory");
+                const char* const row = wsm + (j & 1) * C::TILE_BYTES + l32 * C::RB;
+                f16x s = {};
+                if constexpr (I8) {
+                    operand_stream<NS / 2, 4>(
+                        [&](int i) { return *reinterpret_cast<const i4*>(row + (((2 * i + g) ^ swz8<D>(l32)) << 4)); },
+                        [&](int i, i4 x) {
+                            s = paged_mfma<T>(q[2 * i], widen_int8<T>(i2v{x[0], x[1]}), s);
+                            s = paged_mfma<T>(q[2 * i + 1], widen_int8<T>(i2v{x[2], x[3]}), s);
+                        });
+                } else {
+                    operand_stream<NS, 4>(
+                        [&](int i) {
+                            return *reinterpret_cast<const V8*>(row + (((2 * i + g) ^ paged_swz<D>(l32)) << 4));
+                        },
+                        [&](int i, V8 x) { s = paged_mfma<T>(q[i], x, s); });
+                }
+                const float* const aux = reinterpret_cast<const float*>(wsm + C::AUX + 256 * (j & 1));
+                const float was = aux[l32];
+                const float c = I8 ? p.scale_log2e * aux[kTile + l32] : p.scale_log2e;
+                const int key = tile_key(j) + l32, row0 = base + 4 * g;
+                const PagedKeyRows seen = paged_key_rows(p.mask, seq, G, key);
+                float sum;
+                if (wave_any(seen.lo > base || seen.hi < base + kTile - 1)) {
+                    sum = sum_weights<true>(s, c, sub, factor, seen.lo - row0, seen.hi - row0, 0.0f);
+                } else {
+                    sum = sum_weights<false>(s, c, sub, factor, 0, 0, 0.0f);
                 }
                 sum = pair_sum(sum);
-                if (g == 0 && key.w != nullptr) {
-                    *key.w = later ? old + sum : new_weight(p, key, sum, old);
-                }
-            };
-            if (mine > 0) {
-                a = lane_key<I8>(p, seq, table, h, key_of(0));
-                k0.load(a.k, g);
-            }
-            for (int j = 0; j < mine; j += 2) {
-                if (j + 1 < mine) {
-                    b = lane_key<I8>(p, seq, table, h, key_of(j + 1));
-                    k1.load(b.k, g);
-                }
-                tile(a, k0);
-                if (j + 2 < mine) {
-                    a = lane_key<I8>(p, seq, table, h, key_of(j + 2));
-                    k0.load(a.k, g);
-                }
-                if (j + 1 < mine) {
-                    tile(b, k1);
+                if (g == 0 && w != 0) {
+                    *reinterpret_cast<float*>(w) = later ? was + sum : new_weight(p, key < seq.len - seq.n, sum, was);
                 }
             }
+            __builtin_amdgcn_s_waitcnt(0); // the weights, which the next row tile reads, too
         }
         walk.next();
     }
@@ -300,11 +407,13 @@ __global__ __launch_bounds__((ManyCfg<D, I8>::THREADS), (ManyCfg<D, I8>::WAVES_P
             int lo[C::KT], hi[C::KT];
 #pragma unroll
             for (int t = 0; t < C::KT; t++) {
-                const LaneKey key = lane_key<I8>(p, seq, table, h, key0 + kTile * t + l32);
+                const int at = key0 + kTile * t + l32;
+                const LaneKey key = lane_key<I8>(p, key_entry(p, seq, table, at), h, at);
+                const PagedKeyRows seen = paged_key_rows(p.mask, seq, G, at);
                 k[t].load(key.k, g);
                 scale[t] = p.scale_log2e * key.k_scale * p.q_sign;
-                lo[t] = key.rows.lo - 4 * g;
-                hi[t] = key.rows.hi - 4 * g;
+                lo[t] = seen.lo - 4 * g;
+                hi[t] = seen.hi - 4 * g;
                 sum[t] = 0.0f;
             }
             for (int slot = 0; rt <= rt1; rt += C::WAVES, slot ^= 1) {
@@ -360,9 +469,11 @@ __global__ __launch_bounds__((ManyCfg<D, I8>::THREADS), (ManyCfg<D, I8>::WAVES_P
                     x += sums[w][tid];
                 }
                 if (walk.whole()) {
-                    const LaneKey key = lane_key<false>(p, seq, table, h, key0 + tid);
+                    const int at = key0 + tid;
+                    const LaneKey key = lane_key<false>(p, key_entry(p, seq, table, at), h, at);
+                    const bool is_old = at < seq.len - seq.n;
                     if (key.w != nullptr) {
-                        *key.w = new_weight(p, key, x, key.old ? *key.w : 0.0f);
+                        *key.w = new_weight(p, is_old, x, is_old ? *key.w : 0.0f);
                     }
                 } else {
                     p.parts[(int64_t)walk.slot() * C::BLOCK + tid] = x;
@@ -390,14 +501,16 @@ __global__ __launch_bounds__(128) void paged_weights_merge(WeightsParams p) {
         return;
     }
     const PagedSeq seq = paged_seq(p.work.seqs, rec.q0);
-    const LaneKey key = lane_key<false>(p, seq, p.c.table + rec.q0 * p.c.table_s, rec.h, rec.r0 + i);
-    const float old = key.w != nullptr && key.old ? *key.w : 0.0f;
+    const int at = rec.r0 + i;
+    const LaneKey key = lane_key<false>(p, key_entry(p, seq, p.c.table + rec.q0 * p.c.table_s, at), rec.h, at);
+    const bool is_old = at < seq.len - seq.n;
+    const float old = key.w != nullptr && is_old ? *key.w : 0.0f;
     float sum = p.parts[(int64_t)(p.work.n_wg + w) * rec.rows + i];
     for (int s = w + 1; s <= rec.w_last; s++) {
         sum += p.parts[(int64_t)s * rec.rows + i];
     }
     if (key.w != nullptr) {
-        *key.w = new_weight(p, key, sum, old);
+        *key.w = new_weight(p, is_old, sum, old);
     }
 }
 
@@ -439,6 +552,7 @@ int launch_weights(const PagedWeightsArgs& a, WeightsParams& p, hipStream_t stre
     }
     PagedWork wf = paged_work(p.work, few), wm = paged_work(p.work, many);
     wm.mask = p.mask;
+    wf.Hkv = (p.Hkv + FewCfg<D, I8>::WAVES - 1) / FewCfg<D, I8>::WAVES;
     const int64_t cf = any_few ? paged_max_cost<kAllRows, kTile, 0>(wf) : 0;
     using C = ManyCfg<D, I8>;
     const int64_t cm = any_many ? paged_max_key_cost<C::BLOCK, kTile, C::COST>(wm) : 0;
@@ -454,7 +568,7 @@ int launch_weights(const PagedWeightsArgs& a, WeightsParams& p, hipStream_t stre
     }
     if (any_few) {
         p.work = wf;
-        return go(&paged_weights_few<T, D, I8>, 256, cf, 4, 0);
+        return go(&paged_weights_few<T, D, I8>, 64 * FewCfg<D, I8>::WAVES, cf, 1, 0);
     }
     return 0;
 }
@@ -474,6 +588,7 @@ int paged_key_weights(const PagedWeightsArgs& a, hipStream_t stream, std::string
     p.q_sh = a.q_sh;
     p.lse = a.lse;
     p.Hq = a.Hq;
+    p.Hkv = a.Hkv;
     p.scale_log2e = softmax_log2_scale(a.scale);
     p.q_sign = a.scale < 0.0f ? -1.0f : 1.0f;
     p.decay = a.decay;
