@@ -114,8 +114,10 @@ __device__ __forceinline__ int chunk_of_q(int s, int g) {
     return I8 ? 4 * (s >> 1) + 2 * g + (s & 1) : 2 * s + g;
 }
 
-// Sum over the lane's 16 rows (base + 8 (e / 4) + 4 g + e % 4) of their weights on its key.
-template <bool MASK>
+// Sum over the lane's 16 rows (base + 8 (e / 4) + 4 g + e % 4) of their weights on its key,
+// times the rows' factors.  (Of many rows without: their errors of 2^-24 of an exponent are
+// of either sign, and the registers hold another tile of keys.)
+template <bool MASK, bool FACTOR>
 __device__ __forceinline__ float sum_weights(const f16x& s, float c, const f4 (&sub)[4], const f4 (&factor)[4], int lo,
                                              int hi, float sum) {
     float part[4] = {sum, 0.0f, 0.0f, 0.0f};
@@ -126,7 +128,7 @@ __device__ __forceinline__ float sum_weights(const f16x& s, float c, const f4 (&
             const int off = 8 * (e >> 2) + (e & 3);
             p = off < lo || off > hi ? 0.0f : p;
         }
-        part[e & 3] = fmaf(p, factor[e >> 2][e & 3], part[e & 3]);
+        part[e & 3] = FACTOR ? fmaf(p, factor[e >> 2][e & 3], part[e & 3]) : part[e & 3] + p;
     }
     return (part[0] + part[1]) + (part[2] + part[3]);
 }
@@ -317,9 +319,9 @@ __global__ __launch_bounds__((64 * FewCfg<D, I8>::WAVES)) void paged_weights_few
                 const PagedKeyRows seen = paged_key_rows(p.mask, seq, G, key);
                 float sum;
                 if (wave_any(seen.lo > base || seen.hi < base + kTile - 1)) {
-                    sum = sum_weights<true>(s, c, sub, factor, seen.lo - row0, seen.hi - row0, 0.0f);
+                    sum = sum_weights<true, true>(s, c, sub, factor, seen.lo - row0, seen.hi - row0, 0.0f);
                 } else {
-                    sum = sum_weights<false>(s, c, sub, factor, 0, 0, 0.0f);
+                    sum = sum_weights<false, true>(s, c, sub, factor, 0, 0, 0.0f);
                 }
                 sum = pair_sum(sum);
                 if (g == 0 && w != 0) {
@@ -336,7 +338,7 @@ template <int D, bool I8>
 struct ManyCfg {
     static constexpr int WAVES = 4;
     static constexpr int THREADS = 64 * WAVES;
-    static constexpr int KT = D <= 96 ? 4 : D <= 128 && !I8 ? 3 : 2; // 32-key tiles in registers
+    static constexpr int KT = D <= 64 ? 4 : D <= 128 ? 3 : 2; // 32-key tiles in registers
     static constexpr int BLOCK = kTile * KT;
     static constexpr int WAVES_PER_SIMD = D <= 128 ? 2 : 1;
     static constexpr int COST = 8; // of an item beside its row tiles
@@ -344,7 +346,7 @@ struct ManyCfg {
     static constexpr int KCH = D / 8;
     static constexpr int Q_BYTES = kTile * RB;
     static constexpr int NS = D / 16;
-    static constexpr int LDS_BYTES = WAVES * (2 * Q_BYTES + 2 * kTile * 4);
+    static constexpr int LDS_BYTES = WAVES * (2 * Q_BYTES + kTile * 16); // and row addresses, log-sum-exps
     static_assert(LDS_BYTES + WAVES * BLOCK * 4 <= 160 * 1024 / (D <= 128 ? 2 : 1), "workgroups fit the LDS");
 };
 
@@ -361,7 +363,16 @@ __global__ __launch_bounds__((ManyCfg<D, I8>::THREADS), (ManyCfg<D, I8>::WAVES_P
     const int l32 = lane & 31, g = lane >> 5;
     const uint32_t lds_w = (uint32_t)reinterpret_cast<uintptr_t>(dsm) + wave * 2 * C::Q_BYTES;
     char* const qsm = dsm + wave * 2 * C::Q_BYTES;
-    float* const lsm = reinterpret_cast<float*>(dsm + C::WAVES * 2 * C::Q_BYTES) + wave * 2 * kTile;
+    uint64_t* const rows_at = reinterpret_cast<uint64_t*>(dsm + C::WAVES * 2 * C::Q_BYTES) + wave * 2 * kTile;
+    float* const lsm = reinterpret_cast<float*>(rows_at + kTile);
+    const int tok_step = C::WAVES * kTile / p.work.G, head_step = C::WAVES * kTile - tok_step * p.work.G;
+    uint32_t src[C::NS]; // as in paged_weights_few
+#pragma unroll
+    for (int n = 0; n < C::NS; n++) {
+        const int c = 64 * n + lane;
+        const int x = c / C::KCH;
+        src[n] = (uint32_t)(x * 8) | (uint32_t)(((c - x * C::KCH) ^ paged_swz<D>(x)) * 16) << 16;
+    }
 
     PagedItemWalk<PagedKeyItems<C::BLOCK, kTile>, true, C::COST, false> walk(p.work, by_xcd(blockIdx.x, p.work.n_wg));
     PagedRecord rec = {};
@@ -376,82 +387,98 @@ __global__ __launch_bounds__((ManyCfg<D, I8>::THREADS), (ManyCfg<D, I8>::WAVES_P
             const int rt0 = uniform(walk.tile.first + walk.begin());
             const int rt1 = uniform(walk.tile.hi >= walk.tile.lo ? rt0 + walk.count() - 1 : rt0 - 1);
 
-            // row of a tile that this lane loads
+            // The row of the next tile whose address this lane finds: its token and head (of the
+            // group), which a step of a row tile for each wave moves on.
+            int row = (rt0 + wave) * kTile + l32;
+            int tok = row / G, sub_head = row - tok * G;
             float lse_next = 0.0f;
-            auto prefetch = [&](int rt, int slot) __attribute__((always_inline)) {
-                const int r = min(rt * kTile + l32, rows - 1);
-                const int tok = r / G;
-                const int head = h * G + r - tok * G;
-                const char* const at = p.q + (int64_t)(seq.q0 + tok) * p.q_st + head * p.q_sh;
-                const uint64_t mine = reinterpret_cast<uint64_t>(at);
-                lse_next = p.lse[(int64_t)(seq.q0 + tok) * p.Hq + head];
-                const uint32_t lo = (uint32_t)mine, hi = (uint32_t)(mine >> 32);
-                int ln = lane;
-                asm volatile("" : "+v"(ln));
+            auto prefetch = [&](int slot) __attribute__((always_inline)) {
+                const bool in = row < rows; // the last row again for those behind it
+                const int t = in ? tok : seq.n - 1;
+                const int x = h * G + (in ? sub_head : G - 1);
+                rows_at[l32] = reinterpret_cast<uint64_t>(p.q) + (uint64_t)(uint32_t)(seq.q0 + t) * (uint64_t)p.q_st +
+                               (uint64_t)(uint32_t)x * (uint64_t)p.q_sh;
+                lse_next = p.lse[(int64_t)(seq.q0 + t) * p.Hq + x];
+                row += C::WAVES * kTile;
+                tok += tok_step;
+                sub_head += head_step;
+                tok += sub_head >= G ? 1 : 0;
+                sub_head -= sub_head >= G ? G : 0;
+                uint64_t from[C::NS];
 #pragma unroll
                 for (int n = 0; n < C::NS; n++) {
-                    const int c = 64 * n + ln;
-                    const int x = c / C::KCH;
-                    const uint64_t row = (uint64_t)(uint32_t)__builtin_amdgcn_ds_bpermute(4 * x, (int)hi) << 32 |
-                                         (uint32_t)__builtin_amdgcn_ds_bpermute(4 * x, (int)lo);
-                    dma_gather16(row + (uint32_t)((c - x * C::KCH) ^ paged_swz<D>(x)) * 16u,
-                                 (uint32_t)uniform((int)lds_w + slot * C::Q_BYTES + 1024 * n));
+                    from[n] = *reinterpret_cast<const uint64_t*>(reinterpret_cast<const char*>(rows_at) +
+                                                                 (src[n] & 0xffffu)) +
+                              (src[n] >> 16);
+                }
+#pragma unroll
+                for (int n = 0; n < C::NS; n++) {
+                    dma_gather16(from[n], (uint32_t)uniform((int)lds_w + slot * C::Q_BYTES + 1024 * n));
                 }
             };
             int rt = rt0 + wave;
             if (rt <= rt1) {
-                prefetch(rt, 0);
+                prefetch(0);
             }
-            KeyRegs<D, I8> k[C::KT];
+            V8 k[C::KT][C::NS];
             float scale[C::KT], sum[C::KT];
-            int lo[C::KT], hi[C::KT];
+            int full_lo[C::KT], full_hi[C::KT]; // rows that see all keys of a tile
 #pragma unroll
             for (int t = 0; t < C::KT; t++) {
-                const int at = key0 + kTile * t + l32;
+                const int first = key0 + kTile * t, at = first + l32;
                 const LaneKey key = lane_key<I8>(p, key_entry(p, seq, table, at), h, at);
-                const PagedKeyRows seen = paged_key_rows(p.mask, seq, G, at);
-                k[t].load(key.k, g);
+                KeyRegs<D, I8> raw;
+                raw.load(key.k, g);
+#pragma unroll
+                for (int s = 0; s < C::NS; s++) {
+                    k[t][s] = raw.template operand<T>(s);
+                }
                 scale[t] = p.scale_log2e * key.k_scale * p.q_sign;
-                lo[t] = seen.lo - 4 * g;
-                hi[t] = seen.hi - 4 * g;
+                full_lo[t] = uniform(paged_key_rows(p.mask, seq, G, min(first + kTile, seq.len) - 1).lo);
+                full_hi[t] = uniform(paged_key_rows(p.mask, seq, G, first).hi);
                 sum[t] = 0.0f;
             }
             for (int slot = 0; rt <= rt1; rt += C::WAVES, slot ^= 1) {
-                const RowLse r = row_lse(lse_next);
-                lsm[l32] = r.sub;
-                lsm[kTile + l32] = r.factor;
+                lsm[l32] = row_lse(lse_next).sub;
                 // this tile's Q has landed, and what the next one overwrites has been read
                 __builtin_amdgcn_s_waitcnt(waitcnt_vm(0));
                 __builtin_amdgcn_s_waitcnt(waitcnt_lgkm(0));
                 asm volatile("" ::: "memory");
                 if (rt + C::WAVES <= rt1) {
-                    prefetch(rt + C::WAVES, slot ^ 1);
+                    prefetch(slot ^ 1);
                 }
-                f4 sub[4], factor[4];
+                f4 sub[4];
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     sub[i] = *reinterpret_cast<const f4*>(lsm + 8 * i + 4 * g);
-                    factor[i] = *reinterpret_cast<const f4*>(lsm + kTile + 8 * i + 4 * g);
                 }
-                V8 q[C::NS];
+                f16x acc[C::KT];
+                int ln = lane; // the operands' addresses are made for every tile, not kept
+                asm volatile("" : "+v"(ln));
+                const int x32 = ln & 31;
+                const char* const q = qsm + slot * C::Q_BYTES + x32 * C::RB;
+                operand_stream<C::NS, 2>(
+                    [&](int s) {
+                        return *reinterpret_cast<const V8*>(q + ((chunk_of_q<I8>(s, ln >> 5) ^ paged_swz<D>(x32)) << 4));
+                    },
+                    [&](int s, V8 x) {
 #pragma unroll
-                for (int s = 0; s < C::NS; s++) {
-                    q[s] = *reinterpret_cast<const V8*>(qsm + slot * C::Q_BYTES + l32 * C::RB +
-                                                        ((chunk_of_q<I8>(s, g) ^ paged_swz<D>(l32)) << 4));
-                }
+                        for (int t = 0; t < C::KT; t++) {
+                            acc[t] = paged_mfma<T>(x, k[t][s], s == 0 ? f16x{} : acc[t]);
+                        }
+                    });
                 const int base = rt * kTile;
 #pragma unroll
                 for (int t = 0; t < C::KT; t++) {
-                    f16x s = f16x{};
-#pragma unroll
-                    for (int i = 0; i < C::NS; i++) {
-                        s = paged_mfma<T>(q[i], k[t].template operand<T>(i), s);
-                    }
-                    if (wave_any(lo[t] + 4 * g > base || hi[t] + 4 * g < base + kTile - 1)) {
-                        sum[t] = sum_weights<true>(s, scale[t], sub, factor, lo[t] - base, hi[t] - base, sum[t]);
+                    if (full_lo[t] > base || full_hi[t] < base + kTile - 1) {
+                        const PagedKeyRows seen = paged_key_rows(p.mask, seq, G, key0 + kTile * t + l32);
+                        const int row0 = base + 4 * g;
+                        sum[t] = sum_weights<true, false>(acc[t], scale[t], sub, sub, seen.lo - row0, seen.hi - row0,
+                                                          sum[t]);
                     } else {
-                        sum[t] = sum_weights<false>(s, scale[t], sub, factor, 0, 0, sum[t]);
+                        sum[t] = sum_weights<false, false>(acc[t], scale[t], sub, sub, 0, 0, sum[t]);
                     }
+                    __builtin_amdgcn_sched_barrier(0); // one tile's exponents in registers
                 }
             }
 #pragma unroll
