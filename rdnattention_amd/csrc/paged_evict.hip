@@ -14,7 +14,8 @@ namespace {
 
 constexpr int kSelectThreads = 1024;
 constexpr int kWaves = kSelectThreads / 64;
-constexpr int kMoveThreads = 256;
+constexpr int kMoveThreads = 512;
+constexpr int kHists = 4; // copies of the histogram
 
 struct EvictParams {
     PagedEvictArgs a;
@@ -32,8 +33,8 @@ __device__ __forceinline__ uint32_t ordered(float w) {
 template <int CACHE>
 __global__ __launch_bounds__(kSelectThreads) void paged_evict_choose(EvictParams p) {
     __shared__ uint32_t cache[CACHE];
-    __shared__ int32_t hist[kWaves][256];
-    __shared__ int32_t found[2];
+    __shared__ int32_t hist[kHists][256];
+    __shared__ int32_t found[3];
     __shared__ int32_t counts[2][kWaves];
     const PagedEvictArgs& a = p.a;
     const int h = blockIdx.x, b = blockIdx.y;
@@ -63,19 +64,21 @@ __global__ __launch_bounds__(kSelectThreads) void paged_evict_choose(EvictParams
     for (int32_t i = lo + tid; i < min(hi, CACHE); i += kSelectThreads) {
         cache[i] = load(i);
     }
-    // the smallest weight that stays (`least`), and of those equal to it how many (`more`)
+    // the smallest weight that stays, without its lowest `shift` bits (`least`), and of those equal
+    // to it how many (`more`): all of them where the bits behind do not matter
     uint32_t least = 0xffffffffu;
+    int shift = 0;
     if (more > 0) {
         least = 0;
-        for (int shift = 24; shift >= 0; shift -= 8) {
-            for (int i = lane; i < 256; i += 64) {
-                hist[wave][i] = 0;
+        for (shift = 24;; shift -= 8) {
+            if (tid < kHists * 256) {
+                (&hist[0][0])[tid] = 0;
             }
             __syncthreads();
             for (int32_t i = lo + tid; i < hi; i += kSelectThreads) {
                 const uint32_t u = weight(i);
                 if (shift == 24 || u >> (shift + 8) == least) {
-                    atomicAdd(&hist[wave][(u >> shift) & 255u], 1);
+                    atomicAdd(&hist[wave % kHists][(u >> shift) & 255u], 1);
                 }
             }
             __syncthreads();
@@ -85,7 +88,8 @@ __global__ __launch_bounds__(kSelectThreads) void paged_evict_choose(EvictParams
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
                     c[j] = 0;
-                    for (int w = 0; w < kWaves; w++) {
+#pragma unroll
+                    for (int w = 0; w < kHists; w++) {
                         c[j] += hist[w][255 - 4 * lane - j];
                     }
                     sum += c[j];
@@ -101,6 +105,7 @@ __global__ __launch_bounds__(kSelectThreads) void paged_evict_choose(EvictParams
                     if (above < more && more <= above + c[j]) {
                         found[0] = 255 - 4 * lane - j;
                         found[1] = more - above;
+                        found[2] = c[j];
                     }
                     above += c[j];
                 }
@@ -108,6 +113,9 @@ __global__ __launch_bounds__(kSelectThreads) void paged_evict_choose(EvictParams
             __syncthreads();
             least = least << 8 | (uint32_t)found[0];
             more = found[1];
+            if (shift == 0 || more == found[2]) {
+                break;
+            }
         }
     }
     __syncthreads();
@@ -120,7 +128,7 @@ __global__ __launch_bounds__(kSelectThreads) void paged_evict_choose(EvictParams
             const int32_t i = i0 + lane;
             const bool in = i < to;
             const bool between = in && i >= lo && i < hi;
-            const uint32_t u = between ? weight(i) : 0u;
+            const uint32_t u = between ? weight(i) >> shift : 0u;
             const bool equal = between && u == least;
             use(i, __builtin_amdgcn_ballot_w64(in && (!between || u > least)), __builtin_amdgcn_ballot_w64(equal));
         }
@@ -153,11 +161,11 @@ __global__ __launch_bounds__(kSelectThreads) void paged_evict_choose(EvictParams
     });
 }
 
-// Workgroup x, b: a 64-byte slice of a head's keys or values, or a head's weights.  The
+// Workgroup x, b: a slice of 16 LANES bytes of a head's keys or values, or a head's weights.  The
 // kept rows of a stretch are in registers before the first of them is written, to places
 // at or before their own and behind those of every earlier stretch: later rows are not
 // touched.
-template <int PASSES>
+template <int PASSES, int LANES>
 __global__ __launch_bounds__(kMoveThreads) void paged_evict_move(EvictParams p) {
     const PagedEvictArgs& a = p.a;
     const int b = blockIdx.y;
@@ -211,9 +219,9 @@ __global__ __launch_bounds__(kMoveThreads) void paged_evict_move(EvictParams p) 
         }
         return;
     }
-    const int ch = threadIdx.x & 3;
-    constexpr int kRows = kMoveThreads / 4;
-    char* const base = (keys ? a.c.k + h * a.c.k_sh : a.c.v + h * a.c.v_sh) + 64 * slice + 16 * ch;
+    const int ch = threadIdx.x & (LANES - 1);
+    constexpr int kRows = kMoveThreads / LANES;
+    char* const base = (keys ? a.c.k + h * a.c.k_sh : a.c.v + h * a.c.v_sh) + 16 * (LANES * slice + ch);
     float* const sbase = keys ? a.c.ks + h * a.c.ks_sh : a.c.vs + h * a.c.vs_sh;
     const int64_t sp = keys ? a.c.k_sp : a.c.v_sp, st = keys ? a.c.k_st : a.c.v_st;
     const int64_t ssp = keys ? a.c.ks_sp : a.c.vs_sp, sst = keys ? a.c.ks_st : a.c.vs_st;
@@ -224,7 +232,7 @@ __global__ __launch_bounds__(kMoveThreads) void paged_evict_move(EvictParams p) 
         int32_t to[PASSES];
 #pragma unroll
         for (int i = 0; i < PASSES; i++) {
-            const int32_t r = r0 + i * kRows + (threadIdx.x >> 2);
+            const int32_t r = r0 + i * kRows + (int)threadIdx.x / LANES;
             const int32_t from = r < a.budget ? kept[r] : r;
             to[i] = -1;
             x[i] = i4{0, 0, 0, 0};
@@ -249,7 +257,7 @@ __global__ __launch_bounds__(kMoveThreads) void paged_evict_move(EvictParams p) 
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < PASSES; i++) {
-            const int32_t r = r0 + i * kRows + (threadIdx.x >> 2);
+            const int32_t r = r0 + i * kRows + (int)threadIdx.x / LANES;
             if (to[i] >= 0) {
                 const int64_t off = r & mask;
                 *reinterpret_cast<i4*>(base + to[i] * sp + off * st) = x[i];
@@ -267,7 +275,8 @@ int paged_evict(const PagedEvictArgs& a, hipStream_t stream, std::string& err) {
     EvictParams p;
     p.a = a;
     p.max_keys = (int32_t)((int64_t)a.c.width << a.c.lps);
-    p.slices = a.row_bytes / 64;
+    const int lanes = a.row_bytes % 128 == 0 ? 8 : 4; // of a row: whole lines where it has them
+    p.slices = a.row_bytes / (16 * lanes);
     auto launched = [&]() {
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) {
@@ -281,7 +290,8 @@ int paged_evict(const PagedEvictArgs& a, hipStream_t stream, std::string& err) {
     if (launched() != 0) {
         return -1;
     }
-    auto* const move = a.budget <= 256 ? &paged_evict_move<4> : &paged_evict_move<16>;
+    auto* const move = lanes == 8 ? (a.budget <= 256 ? &paged_evict_move<4, 8> : &paged_evict_move<16, 8>)
+                                  : (a.budget <= 512 ? &paged_evict_move<4, 4> : &paged_evict_move<16, 4>);
     hipLaunchKernelGGL(move, dim3((uint32_t)(a.Hkv * (2 * p.slices + 1)), (uint32_t)a.B), dim3(kMoveThreads), 0, stream,
                        p);
     return launched();

@@ -31,6 +31,34 @@ __device__ __forceinline__ F from_lane(F v, int lane) {
     }
 }
 
+// Sum over a group of LANES lanes, in all of them.
+template <int LANES>
+__device__ __forceinline__ float group_sum(float v) {
+    // neighbours and pairs within quads, then mirrored halves of 8 and 16 lanes
+#define RDNA_DPP(x, ctrl) __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), ctrl, 0xf, 0xf, true))
+    v += RDNA_DPP(v, 0xb1);
+    v += RDNA_DPP(v, 0x4e);
+    if constexpr (LANES >= 8) {
+        v += RDNA_DPP(v, 0x141);
+    }
+    if constexpr (LANES >= 16) {
+        v += RDNA_DPP(v, 0x140);
+    }
+#undef RDNA_DPP
+    if constexpr (LANES == 32) {
+        v += from_lane(v, (int)(threadIdx.x & 63) ^ 16);
+    }
+    return v;
+}
+template <int LANES>
+__device__ __forceinline__ double group_sum(double v) {
+#pragma unroll
+    for (int d = 1; d < LANES; d <<= 1) {
+        v += from_lane(v, (int)(threadIdx.x & 63) ^ d);
+    }
+    return v;
+}
+
 // Eight channels from chunk c of a norm's weights.
 __device__ __forceinline__ void load_weights(const void* w, PagedNormType type, int c, float (&out)[8]) {
     if (type == PagedNormType::F32) {
@@ -61,6 +89,12 @@ struct NormParams {
     PagedNorm n;
     uint32_t per_token; // groups of lanes that a token has
     uint32_t groups;    // of the call
+    float inv_d;
+};
+
+template <class F>
+struct Wide {
+    typedef F v8 __attribute__((ext_vector_type(8)));
 };
 
 // The angles of a lane's channels: of the pairs (2i, 2i + 1) four columns, of the
@@ -69,11 +103,11 @@ struct Angles {
     float c[8], s[8];
 };
 
-// LANES lanes, a power of two that holds a head's D / 8 chunks of 16 bytes, have HEADS
-// heads of one token, PER = per_token apart: its keys', values' and queries'.  They look
-// the token's place and angles up once, and all their rows are loaded before the first
-// is worked on.
-template <class T, bool I8, int LANES, int HEADS>
+// LANES lanes, a power of two that holds a head's D / 8 chunks of 16 bytes, have every
+// per_token'th head of one token, of its keys', values' and queries'.  They look the
+// token's place and angles up once (with several axes 32 loads for a head's one), and
+// work on BATCH heads while the next are loaded.
+template <class T, bool I8, int LANES, int BATCH>
 __global__ __launch_bounds__(kThreads) void paged_append_normed(NormParams p) {
     typedef T V8 __attribute__((ext_vector_type(8)));
     const PagedAppendArgs& a = p.a;
@@ -87,17 +121,21 @@ __global__ __launch_bounds__(kThreads) void paged_append_normed(NormParams p) {
     const bool chunk = 8 * c < a.D;
     const int heads = 2 * a.Hkv + a.Hq;
 
-    V8 x[HEADS];
+    const int per = (int)p.per_token;
+    auto load = [&](V8 (&x)[BATCH], int first) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < HEADS; i++) {
-        int h = min(h0 + i * (int)p.per_token, heads - 1);
-        const int which = h < a.Hkv ? 0 : h < 2 * a.Hkv ? 1 : 2; // keys, values, queries
-        h -= which * a.Hkv;
-        const char* src = which == 0   ? (const char*)a.k + t * a.k_st + h * a.k_sh
-                          : which == 1 ? (const char*)a.v + t * a.v_st + h * a.v_sh
-                                       : (const char*)a.q + t * a.q_st + h * a.q_sh;
-        x[i] = chunk ? *reinterpret_cast<const V8*>(src + 16 * c) : V8{};
-    }
+        for (int i = 0; i < BATCH; i++) {
+            int h = min(first + i * per, heads - 1);
+            const int which = h < a.Hkv ? 0 : h < 2 * a.Hkv ? 1 : 2; // keys, values, queries
+            h -= which * a.Hkv;
+            const char* src = which == 0   ? (const char*)a.k + t * a.k_st + h * a.k_sh
+                              : which == 1 ? (const char*)a.v + t * a.v_st + h * a.v_sh
+                                           : (const char*)a.q + t * a.q_st + h * a.q_sh;
+            x[i] = chunk ? *reinterpret_cast<const V8*>(src + 16 * c) : V8{};
+        }
+    };
+    V8 x[BATCH];
+    load(x, h0);
 
     // the row's sequence and its place there (as in paged_append_rows)
     int32_t b, key;
@@ -173,11 +211,13 @@ __global__ __launch_bounds__(kThreads) void paged_append_normed(NormParams p) {
             for (int e = 0; e < 8; e++) {
                 sum += y[e] * y[e];
             }
-#pragma unroll
-            for (int d = 1; d < LANES; d <<= 1) {
-                sum += from_lane(sum, lane ^ d);
+            sum = group_sum<LANES>(sum);
+            F r;
+            if constexpr (sizeof(F) == 8) {
+                r = F(1) / __builtin_elementwise_sqrt(sum / (F)a.D + (F)p.n.eps);
+            } else { // good to 2^-23 itself
+                r = __builtin_amdgcn_rsqf(fmaf(sum, p.inv_d, p.n.eps));
             }
-            const F r = F(1) / __builtin_elementwise_sqrt(sum / (F)a.D + (F)p.n.eps);
             float w[8];
             load_weights(weights, p.n.type, chunk ? c : 0, w);
 #pragma unroll
@@ -185,9 +225,11 @@ __global__ __launch_bounds__(kThreads) void paged_append_normed(NormParams p) {
                 y[e] = y[e] * r * (F)w[e];
             }
         }
-        F z[8] = {};
         if (a.rot == 0) {
-        } else if (a.interleaved) {
+            return __builtin_convertvector((typename Wide<F>::v8){y[0], y[1], y[2], y[3], y[4], y[5], y[6], y[7]}, V8);
+        }
+        F z[8];
+        if (a.interleaved) {
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 z[2 * e] = y[2 * e] * (F)ang.c[e] - y[2 * e + 1] * (F)ang.s[e];
@@ -208,78 +250,87 @@ __global__ __launch_bounds__(kThreads) void paged_append_normed(NormParams p) {
         return r;
     };
 
+    for (int first = h0; first < heads; first += BATCH * per) {
+        V8 now[BATCH];
 #pragma unroll
-    for (int i = 0; i < HEADS; i++) {
-        int h = h0 + i * (int)p.per_token;
-        const bool has = live && h < heads; // else the last head again, for its lanes' sake
-        h = min(h, heads - 1);
-        const int which = h < a.Hkv ? 0 : h < 2 * a.Hkv ? 1 : 2;
-        h -= which * a.Hkv;
-        // Every lane of a head's group takes the same branches; what the groups of a
-        // wave exchange stays within each.
-        V8 y = x[i];
-        if (which != 1) {
-            const void* w = which == 0 ? p.n.key : p.n.query;
-            if (I8 && which == 0) {
-                // keys that are quantised: in fp64, so that the row before is the nearest one
-                // and a value at a border of two int8 steps falls the way of the definition
-                y = turned(y, w, double{});
+        for (int i = 0; i < BATCH; i++) {
+            now[i] = x[i];
+        }
+        if (first + BATCH * per < heads) {
+            load(x, first + BATCH * per);
+        }
+#pragma unroll
+        for (int i = 0; i < BATCH; i++) {
+            int h = first + i * per;
+            const bool has = live && h < heads; // else the last head again, for its lanes' sake
+            h = min(h, heads - 1);
+            const int which = h < a.Hkv ? 0 : h < 2 * a.Hkv ? 1 : 2;
+            h -= which * a.Hkv;
+            // Every lane of a head's group takes the same branches; what the groups of a
+            // wave exchange stays within each.
+            V8 y = now[i];
+            if (which != 1) {
+                const void* w = which == 0 ? p.n.key : p.n.query;
+                if (I8 && which == 0) {
+                    // keys that are quantised: in fp64, so that the row before is the nearest one
+                    // and a value at a border of two int8 steps falls the way of the definition
+                    y = turned(y, w, double{});
+                } else {
+                    y = turned(y, w, float{});
+                }
+            }
+            if (which == 2) {
+                if (has && chunk) {
+                    *reinterpret_cast<V8*>((char*)a.q_out + t * a.qo_st + h * a.qo_sh + 16 * c) = y;
+                }
+                continue;
+            }
+            float scale = 0.0f;
+            if constexpr (I8) {
+                float mx = 0.0f;
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const float v = fabsf((float)y[e]);
+                    mx = v > mx || v != v ? v : mx;
+                }
+#pragma unroll
+                for (int d = 1; d < LANES; d <<= 1) {
+                    const float v = from_lane(mx, lane ^ d);
+                    mx = v > mx || v != v ? v : mx;
+                }
+                scale = mx * (1.0f / 127.0f);
+                scale = scale == 0.0f ? 1.0f : scale;
+            }
+            if (page < 0 || !has || !chunk) {
+                continue;
+            }
+            char* const dst = which == 0 ? a.c.k + page * a.c.k_sp + off * a.c.k_st + h * a.c.k_sh
+                                         : a.c.v + page * a.c.v_sp + off * a.c.v_st + h * a.c.v_sh;
+            if constexpr (I8) {
+                b8 q;
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    q[e] = (int8_t)fminf(fmaxf(rintf((float)y[e] / scale), -127.0f), 127.0f);
+                }
+                *reinterpret_cast<b8*>(dst + 8 * c) = q;
+                if (c == 0) {
+                    float* const sc = which == 0 ? a.c.ks + page * a.c.ks_sp + off * a.c.ks_st + h * a.c.ks_sh
+                                                 : a.c.vs + page * a.c.vs_sp + off * a.c.vs_st + h * a.c.vs_sh;
+                    *sc = scale;
+                }
             } else {
-                y = turned(y, w, float{});
+                *reinterpret_cast<V8*>(dst + 16 * c) = y;
             }
-        }
-        if (which == 2) {
-            if (has && chunk) {
-                *reinterpret_cast<V8*>((char*)a.q_out + t * a.qo_st + h * a.qo_sh + 16 * c) = y;
-            }
-            continue;
-        }
-        float scale = 0.0f;
-        if constexpr (I8) {
-            float mx = 0.0f;
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const float v = fabsf((float)y[e]);
-                mx = v > mx || v != v ? v : mx;
-            }
-#pragma unroll
-            for (int d = 1; d < LANES; d <<= 1) {
-                const float v = from_lane(mx, lane ^ d);
-                mx = v > mx || v != v ? v : mx;
-            }
-            scale = mx * (1.0f / 127.0f);
-            scale = scale == 0.0f ? 1.0f : scale;
-        }
-        if (page < 0 || !has || !chunk) {
-            continue;
-        }
-        char* const dst = which == 0 ? a.c.k + page * a.c.k_sp + off * a.c.k_st + h * a.c.k_sh
-                                     : a.c.v + page * a.c.v_sp + off * a.c.v_st + h * a.c.v_sh;
-        if constexpr (I8) {
-            b8 q;
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                q[e] = (int8_t)fminf(fmaxf(rintf((float)y[e] / scale), -127.0f), 127.0f);
-            }
-            *reinterpret_cast<b8*>(dst + 8 * c) = q;
-            if (c == 0) {
-                float* const sc = which == 0 ? a.c.ks + page * a.c.ks_sp + off * a.c.ks_st + h * a.c.ks_sh
-                                             : a.c.vs + page * a.c.vs_sp + off * a.c.vs_st + h * a.c.vs_sh;
-                *sc = scale;
-            }
-        } else {
-            *reinterpret_cast<V8*>(dst + 16 * c) = y;
         }
     }
 }
 
-template <class T, bool I8, int LANES, int HEADS>
-void launch(NormParams& p, hipStream_t stream) {
-    const uint32_t heads = (uint32_t)(2 * p.a.Hkv + p.a.Hq);
-    p.per_token = (heads + HEADS - 1) / HEADS;
+template <class T, bool I8, int LANES, int BATCH>
+void launch(NormParams& p, uint32_t per_token, hipStream_t stream) {
+    p.per_token = per_token;
     p.groups = (uint32_t)p.a.seqs.total * p.per_token;
     const uint32_t per_block = kThreads / LANES;
-    hipLaunchKernelGGL((paged_append_normed<T, I8, LANES, HEADS>), dim3((p.groups + per_block - 1) / per_block),
+    hipLaunchKernelGGL((paged_append_normed<T, I8, LANES, BATCH>), dim3((p.groups + per_block - 1) / per_block),
                        dim3(kThreads), 0, stream, p);
 }
 
@@ -289,15 +340,19 @@ int paged_append_norm(const PagedAppendArgs& a, const PagedNorm& n, hipStream_t 
     NormParams p;
     p.a = a;
     p.n = n;
-    // Heads per group: four share a token's look-ups once there are lanes enough for the chip's
-    // 256 compute units with one.
-    const int64_t lanes = (int64_t)a.seqs.total * (2 * a.Hkv + a.Hq) * (a.D / 8);
-    const bool many = lanes > (int64_t)256 * 2048;
+    p.inv_d = 1.0f / (float)a.D;
+    // Groups per token: as many as it takes for 1024 lanes (of 2048) on each of the chip's 256
+    // compute units, up to one for each head, and the groups of a wave at least.  us for 4853
+    // bf16 rows of 32 + 16 heads of 128 with three axes: 37 with 4 or 3 heads at a time, 38 with
+    // 2, 43 with 1; 50 with 2048 lanes.
+    const int64_t heads = 2 * a.Hkv + a.Hq;
     auto go = [&](auto t, auto i8, auto lanes_of) {
         using T = decltype(t);
         constexpr bool I8 = decltype(i8)::value;
         constexpr int L = decltype(lanes_of)::value;
-        many ? launch<T, I8, L, 4>(p, stream) : launch<T, I8, L, 1>(p, stream);
+        const int64_t want = std::max<int64_t>((256 * 1024) / ((int64_t)a.seqs.total * L), 64 / L);
+        const uint32_t per = (uint32_t)std::min(want, heads);
+        per * 2 > heads ? launch<T, I8, L, 1>(p, (uint32_t)heads, stream) : launch<T, I8, L, 4>(p, per, stream);
     };
     auto typed = [&](auto t) {
         if (a.i8) {
