@@ -14,7 +14,12 @@ namespace {
 
 constexpr int kSelectThreads = 1024;
 constexpr int kWaves = kSelectThreads / 64;
-constexpr int kMoveThreads = 512;
+// A workgroup of moves has 64 bytes of a row (the narrowest rows are that long) and 512 rows
+// at a time.  6 sequences, 8 heads of 256 bytes, 256-2000 of up to 3900 keys stay, both
+// launches: 26.2 us; 1024 rows at a time 25.8 (4 sequences of 600 keys 17.0 for 16.3), 256
+// 26.6, 32 bytes of a row 28.5; with 512 threads 29 and, 128 bytes of a row, 32-36.
+constexpr int kMoveThreads = 1024;
+constexpr int kMoveLanes = 4, kMovePasses = 2;
 constexpr int kHists = 4; // copies of the histogram
 
 struct EvictParams {
@@ -161,12 +166,12 @@ __global__ __launch_bounds__(kSelectThreads) void paged_evict_choose(EvictParams
     });
 }
 
-// Workgroup x, b: a slice of 16 LANES bytes of a head's keys or values, or a head's weights.  The
+// Workgroup x, b: a slice of 64 bytes of a head's keys or values, or a head's weights.  The
 // kept rows of a stretch are in registers before the first of them is written, to places
 // at or before their own and behind those of every earlier stretch: later rows are not
 // touched.
-template <int PASSES, int LANES>
 __global__ __launch_bounds__(kMoveThreads) void paged_evict_move(EvictParams p) {
+    constexpr int PASSES = kMovePasses, LANES = kMoveLanes;
     const PagedEvictArgs& a = p.a;
     const int b = blockIdx.y;
     const int32_t len = rows_clamp(a.lens[b], 0, p.max_keys);
@@ -177,8 +182,9 @@ __global__ __launch_bounds__(kMoveThreads) void paged_evict_move(EvictParams p) 
     const int32_t mask = (1 << a.c.lps) - 1;
     const int rows = 2 * a.Hkv * p.slices;
     const bool weights = (int)blockIdx.x >= rows;
-    const int slice = weights ? 0 : blockIdx.x % p.slices;
-    const int hv = weights ? 0 : blockIdx.x / p.slices;
+    // the slices of a row on one XCD where the number of heads lets them
+    const int slice = weights ? 0 : blockIdx.x / (2 * a.Hkv);
+    const int hv = weights ? 0 : blockIdx.x % (2 * a.Hkv);
     const int h = weights ? blockIdx.x - rows : hv >> 1;
     const bool keys = (hv & 1) == 0;
     const int32_t* const kept = a.kept + ((int64_t)b * a.Hkv + h) * a.budget;
@@ -275,8 +281,7 @@ int paged_evict(const PagedEvictArgs& a, hipStream_t stream, std::string& err) {
     EvictParams p;
     p.a = a;
     p.max_keys = (int32_t)((int64_t)a.c.width << a.c.lps);
-    const int lanes = a.row_bytes % 128 == 0 ? 8 : 4; // of a row: whole lines where it has them
-    p.slices = a.row_bytes / (16 * lanes);
+    p.slices = a.row_bytes / (16 * kMoveLanes);
     auto launched = [&]() {
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) {
@@ -285,14 +290,14 @@ int paged_evict(const PagedEvictArgs& a, hipStream_t stream, std::string& err) {
         }
         return 0;
     };
+    // 34816 weights are nearly all LDS, so that a CU has one workgroup: 64 x 8000 keys of 8
+    // heads 182 us with 8192 weights and 190 with 34816; 64 x 30000 keys 456 and 307.
     auto* const choose = p.max_keys <= 8192 ? &paged_evict_choose<8192> : &paged_evict_choose<34816>;
     hipLaunchKernelGGL(choose, dim3((uint32_t)a.Hkv, (uint32_t)a.B), dim3(kSelectThreads), 0, stream, p);
     if (launched() != 0) {
         return -1;
     }
-    auto* const move = lanes == 8 ? (a.budget <= 256 ? &paged_evict_move<4, 8> : &paged_evict_move<16, 8>)
-                                  : (a.budget <= 512 ? &paged_evict_move<4, 4> : &paged_evict_move<16, 4>);
-    hipLaunchKernelGGL(move, dim3((uint32_t)(a.Hkv * (2 * p.slices + 1)), (uint32_t)a.B), dim3(kMoveThreads), 0, stream,
+    hipLaunchKernelGGL(paged_evict_move, dim3((uint32_t)(a.Hkv * (2 * p.slices + 1)), (uint32_t)a.B), dim3(kMoveThreads), 0, stream,
                        p);
     return launched();
 }
