@@ -289,15 +289,20 @@ int paged_attention(const PagedAttnArgs& a, hipStream_t stream, std::string& err
     if (any_many && any_few) {
         few.max_rows = many.min_rows = kFew;
     }
-    // The prefixes' rows are those of all their sequences.  Up to kShared of them per kv head (a
-    // row tile is 32, each of which reads the prefix again) and with few of every sequence, one
-    // launch has the prefixes and the sequences; else the prefixes have one, by tiles, of
-    // their own before the sequences'.
+    // The prefixes' rows are those of all their sequences.  One launch has the prefixes and
+    // the sequences, or the prefixes have one, by tiles, of their own before the sequences'.
+    // The one saves two launches and a pass over the rows, but its row tiles are 32 rows, each
+    // of which reads the prefix again, and every sequence's kv head is an item of it with a
+    // begin and an end of its own: for few rows of every sequence, up to kItems sequences x
+    // kv heads and kSharedRows rows x heads.  8192 keys of one prefix, 300 of each sequence, D
+    // 128, us in one launch / by tiles first: 8 sequences of 32 heads on 8 kv heads 24 / 44,
+    // 32 35 / 54, 64 52 / 67, 96 92 / 80, 128 87 / 86, 256 174 / 129; 32 on 32 16 sequences 58
+    // / 60, 32 91 / 77; 32 on 1 64 42 / 70; 64 on 8 32 53 / 60, 64 81 / 73.
     PagedAttnParams shared = p;
     bool together = false;
     if (a.prefix.n > 0) {
-        constexpr int64_t kShared = 512;
-        together = !any_many && (int64_t)a.seqs.total * p.work.G <= kShared;
+                constexpr int64_t kItems = 512, kSharedRows = 2048;
+        together = !any_many && (int64_t)a.seqs.B * a.Hkv <= kItems && (int64_t)a.seqs.total * a.Hq <= kSharedRows;
         PagedSeqs& s = shared.work.seqs;
         s.prefixes = a.prefix.n;
         s.members = a.seqs.B;
