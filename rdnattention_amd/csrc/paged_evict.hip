@@ -15,9 +15,10 @@ namespace {
 constexpr int kSelectThreads = 1024;
 constexpr int kWaves = kSelectThreads / 64;
 // A workgroup of moves has 64 bytes of a row (the narrowest rows are that long) and 512 rows
-// at a time.  6 sequences, 8 heads of 256 bytes, 256-2000 of up to 3900 keys stay, both
-// launches: 26.2 us; 1024 rows at a time 25.8 (4 sequences of 600 keys 17.0 for 16.3), 256
-// 26.6, 32 bytes of a row 28.5; with 512 threads 29 and, 128 bytes of a row, 32-36.
+// at a time, and the next ones on their way.  64 sequences of 3900 keys, 8 heads of 256 bytes,
+// 1000 stay, both launches: 146 us; one stretch at a time 162; 256 rows at a time 158, 1024
+// 182, 32 bytes of a row 181, 512 threads 152.  2 x 8120 int8 keys, of which 7267 stay: 64 us;
+// 69, 70, 60, 54, 72.
 constexpr int kMoveThreads = 1024;
 constexpr int kMoveLanes = 4, kMovePasses = 2;
 constexpr int kHists = 4; // copies of the histogram
@@ -40,6 +41,7 @@ __global__ __launch_bounds__(kSelectThreads) void paged_evict_choose(EvictParams
     __shared__ uint32_t cache[CACHE];
     __shared__ int32_t hist[kHists][256];
     __shared__ int32_t found[3];
+    __shared__ uint32_t ends[2][kWaves];
     __shared__ int32_t counts[2][kWaves];
     const PagedEvictArgs& a = p.a;
     const int h = blockIdx.x, b = blockIdx.y;
@@ -66,24 +68,70 @@ __global__ __launch_bounds__(kSelectThreads) void paged_evict_choose(EvictParams
     // between the first and the newest: 0 < more <= lo .. hi's number where any of them stay
     const int32_t lo = a.first, hi = len - a.recent;
     int32_t more = a.budget - a.first - a.recent;
-    for (int32_t i = lo + tid; i < min(hi, CACHE); i += kSelectThreads) {
-        cache[i] = load(i);
+    uint32_t low = 0xffffffffu, high = 0;
+    constexpr int NB = 4; // loads in flight: 64 x 30000 keys 276 -> 272 us
+    for (int32_t i0 = lo + tid; i0 < hi; i0 += NB * kSelectThreads) {
+        int32_t pg[NB];
+        float w[NB];
+#pragma unroll
+        for (int j = 0; j < NB; j++) {
+            const int32_t i = i0 + j * kSelectThreads;
+            pg[j] = i < hi ? paged_page(a.c, table, i >> a.c.lps) : -1;
+        }
+#pragma unroll
+        for (int j = 0; j < NB; j++) {
+            const int32_t i = i0 + j * kSelectThreads;
+            w[j] = pg[j] >= 0 ? a.w[pg[j] * a.w_sp + (int64_t)(i & mask) * a.w_st + h * a.w_sh] : 0.0f;
+        }
+#pragma unroll
+        for (int j = 0; j < NB; j++) {
+            const int32_t i = i0 + j * kSelectThreads;
+            if (i < hi) {
+                const uint32_t u = pg[j] >= 0 ? ordered(w[j]) : 0u;
+                if (i < CACHE) {
+                    cache[i] = u;
+                }
+                low = min(low, u);
+                high = max(high, u);
+            }
+        }
     }
     // the smallest weight that stays, without its lowest `shift` bits (`least`), and of those equal
     // to it how many (`more`): all of them where the bits behind do not matter
     uint32_t least = 0xffffffffu;
     int shift = 0;
     if (more > 0) {
-        least = 0;
-        for (shift = 24;; shift -= 8) {
+        // The digits begin at the first bit in which two weights differ: at bit 31 most weights of
+        // a softmax would have one of two or three digits, and their atomics take turns.  One
+        // sequence of 8000 keys 27.9 -> 25.9 us, of 30000 66.9 -> 59.9.
+        for (int d = 1; d < 64; d <<= 1) {
+            low = min(low, (uint32_t)__shfl_xor((int32_t)low, d));
+            high = max(high, (uint32_t)__shfl_xor((int32_t)high, d));
+        }
+        if (lane == 0) {
+            ends[0][wave] = low;
+            ends[1][wave] = high;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < kWaves; w++) {
+            low = min(low, ends[0][w]);
+            high = max(high, ends[1][w]);
+        }
+        shift = 32 - __builtin_clz((low ^ high) | 1u);
+        least = (uint32_t)((uint64_t)high >> shift);
+        for (bool all = true; shift > 0; all = false) {
+            const int bits = min(8, shift);
+            const int from = shift;
+            shift -= bits;
             if (tid < kHists * 256) {
                 (&hist[0][0])[tid] = 0;
             }
             __syncthreads();
             for (int32_t i = lo + tid; i < hi; i += kSelectThreads) {
                 const uint32_t u = weight(i);
-                if (shift == 24 || u >> (shift + 8) == least) {
-                    atomicAdd(&hist[wave % kHists][(u >> shift) & 255u], 1);
+                if (all || u >> from == least) {
+                    atomicAdd(&hist[wave % kHists][(u >> shift) & ((1u << bits) - 1)], 1);
                 }
             }
             __syncthreads();
@@ -116,9 +164,9 @@ __global__ __launch_bounds__(kSelectThreads) void paged_evict_choose(EvictParams
                 }
             }
             __syncthreads();
-            least = least << 8 | (uint32_t)found[0];
+            least = least << bits | (uint32_t)found[0];
             more = found[1];
-            if (shift == 0 || more == found[2]) {
+            if (more == found[2]) {
                 break;
             }
         }
@@ -166,10 +214,10 @@ __global__ __launch_bounds__(kSelectThreads) void paged_evict_choose(EvictParams
     });
 }
 
-// Workgroup x, b: a slice of 64 bytes of a head's keys or values, or a head's weights.  The
-// kept rows of a stretch are in registers before the first of them is written, to places
-// at or before their own and behind those of every earlier stretch: later rows are not
-// touched.
+// Workgroup x, b: a slice of 64 bytes of a head's keys or values, or a head's weights.  A
+// stretch of kept rows is written when it and all rows in front are in registers, to places
+// at or before their own and behind those of every earlier stretch: rows of later stretches,
+// already on their way, lie behind all places written so far.
 __global__ __launch_bounds__(kMoveThreads) void paged_evict_move(EvictParams p) {
     constexpr int PASSES = kMovePasses, LANES = kMoveLanes;
     const PagedEvictArgs& a = p.a;
@@ -232,46 +280,80 @@ __global__ __launch_bounds__(kMoveThreads) void paged_evict_move(EvictParams p) 
     const int64_t sp = keys ? a.c.k_sp : a.c.v_sp, st = keys ? a.c.k_st : a.c.v_st;
     const int64_t ssp = keys ? a.c.ks_sp : a.c.vs_sp, sst = keys ? a.c.ks_st : a.c.vs_st;
     const bool scales = a.i8 && slice == 0 && ch == 0;
-    for (int32_t r0 = 0; r0 < a.budget; r0 += PASSES * kRows) {
+    // Stretch s is written while the rows of s + 1 are loaded, the pages of s + 2 and the
+    // numbers of s + 3.
+    struct Stretch {
         i4 x[PASSES];
         float sc[PASSES];
-        int32_t to[PASSES];
+        int32_t from[PASSES], pf[PASSES], pt[PASSES];
+    };
+    const int32_t row = (int32_t)threadIdx.x / LANES;
+    auto number = [&](Stretch& t, int32_t s) {
 #pragma unroll
         for (int i = 0; i < PASSES; i++) {
-            const int32_t r = r0 + i * kRows + (int)threadIdx.x / LANES;
-            const int32_t from = r < a.budget ? kept[r] : r;
-            to[i] = -1;
-            x[i] = i4{0, 0, 0, 0};
-            sc[i] = 0.0f;
-            if (from != r) {
-                const int32_t pf = page(from);
-                if (pf >= 0) {
-                    to[i] = page(r);
-                    const int64_t off = from & mask;
-                    x[i] = *reinterpret_cast<const i4*>(base + pf * sp + off * st);
-                    if (scales) {
-                        sc[i] = sbase[pf * ssp + off * sst];
-                    }
-                }
-            }
+            const int32_t r = (s * PASSES + i) * kRows + row;
+            t.from[i] = r < a.budget ? kept[r] : r;
         }
-        // every load has returned before any wave stores
+    };
+    auto find = [&](Stretch& t, int32_t s) {
 #pragma unroll
         for (int i = 0; i < PASSES; i++) {
-            asm volatile("" ::"v"(x[i]), "v"(sc[i]));
+            const int32_t r = (s * PASSES + i) * kRows + row;
+            const bool moves = t.from[i] != r;
+            t.pf[i] = moves ? page(t.from[i]) : -1;
+            t.pt[i] = moves ? page(r) : -1;
         }
-        __syncthreads();
+    };
+    auto load = [&](Stretch& t) {
 #pragma unroll
         for (int i = 0; i < PASSES; i++) {
-            const int32_t r = r0 + i * kRows + (int)threadIdx.x / LANES;
-            if (to[i] >= 0) {
-                const int64_t off = r & mask;
-                *reinterpret_cast<i4*>(base + to[i] * sp + off * st) = x[i];
+            t.x[i] = i4{0, 0, 0, 0};
+            t.sc[i] = 0.0f;
+            if (t.pf[i] >= 0) {
+                const int64_t off = t.from[i] & mask;
+                t.x[i] = *reinterpret_cast<const i4*>(base + t.pf[i] * sp + off * st);
                 if (scales) {
-                    sbase[to[i] * ssp + off * sst] = sc[i];
+                    t.sc[i] = sbase[t.pf[i] * ssp + off * sst];
                 }
             }
         }
+    };
+    auto step = [&](int32_t s, Stretch& now, Stretch& next, Stretch& third, Stretch& fourth) {
+        load(next);
+        find(third, s + 2);
+        number(fourth, s + 3);
+        // every wave's rows up to this stretch's are in registers before any is written
+#pragma unroll
+        for (int i = 0; i < PASSES; i++) {
+            asm volatile("" ::"v"(now.x[i]), "v"(now.sc[i]) : "memory");
+        }
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+#pragma unroll
+        for (int i = 0; i < PASSES; i++) {
+            const int32_t r = (s * PASSES + i) * kRows + row;
+            if (now.pf[i] >= 0 && now.pt[i] >= 0) {
+                const int64_t off = r & mask;
+                *reinterpret_cast<i4*>(base + now.pt[i] * sp + off * st) = now.x[i];
+                if (scales) {
+                    sbase[now.pt[i] * ssp + off * sst] = now.sc[i];
+                }
+            }
+        }
+    };
+    Stretch t0, t1, t2, t3;
+    number(t0, 0);
+    number(t1, 1);
+    number(t2, 2);
+    find(t0, 0);
+    find(t1, 1);
+    load(t0);
+    const int32_t n = (a.budget + PASSES * kRows - 1) / (PASSES * kRows);
+    for (int32_t s = 0; s < n; s += 4) { // places from the budget on do not move
+        step(s, t0, t1, t2, t3);
+        step(s + 1, t1, t2, t3, t0);
+        step(s + 2, t2, t3, t0, t1);
+        step(s + 3, t3, t0, t1, t2);
     }
 }
 
@@ -291,7 +373,8 @@ int paged_evict(const PagedEvictArgs& a, hipStream_t stream, std::string& err) {
         return 0;
     };
     // 34816 weights are nearly all LDS, so that a CU has one workgroup: 64 x 8000 keys of 8
-    // heads 182 us with 8192 weights and 190 with 34816; 64 x 30000 keys 456 and 307.
+    // heads 182 us with 8192 weights and 190 with 34816; 64 x 30000 keys 456 and 307 (both
+    // before the moves overlapped their stretches).
     auto* const choose = p.max_keys <= 8192 ? &paged_evict_choose<8192> : &paged_evict_choose<34816>;
     hipLaunchKernelGGL(choose, dim3((uint32_t)a.Hkv, (uint32_t)a.B), dim3(kSelectThreads), 0, stream, p);
     if (launched() != 0) {
