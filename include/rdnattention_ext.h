@@ -350,9 +350,10 @@ RDNA_API int32_t rdna_paged_commit(const rdna_paged_cache* cache, const int32_t*
  * with lse [num_rows, num_heads] as rdna_paged_attention_lse gives it (a row of -inf adds
  * nothing) and scores, causal and window_size as there; over the cache's own keys alone
  * where the rows saw a prefix too.  key_weights: float (page, token, head) with
- * key_weights_stride in floats.  decay at least 0; with 0 the old weights are not read.
- * Sequences without rows, and places without a key, are left as they are.  The values of
- * the cache are not looked at.  The same bits every time. */
+ * key_weights_stride in floats, none of them 0 where there are several.  decay at least 0; with 0
+ * the old weights are not read.  Sequences without rows, and places without a key, are left
+ * as they are.  No page may belong to two sequences with rows: the sums of one of them could
+ * be lost.  The values of the cache are not looked at.  The same bits every time. */
 RDNA_API int32_t rdna_paged_key_weights(
     const rdna_paged_cache* cache, const void* query, int64_t query_stride_row, int64_t query_stride_h,
     uint32_t num_rows, uint32_t num_heads, int32_t dtype, uint32_t max_rows_per_seq, const float* lse, float scale,

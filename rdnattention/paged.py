@@ -41,6 +41,7 @@ _CACHE = struct.Struct("=7Q13q6Ii")
 # rdna_paged_norm: 3 pointers, the positions' row stride, axes, eps, dtype
 _NORM = struct.Struct("=3QqIfi")
 _STRIDES = struct.Struct("=3q")
+_F32_MAX = 3.4028234663852886e38
 # rdna_paged_prefix: 3 pointers, the table's row stride, its width, prefixes
 _PREFIX = struct.Struct("=3Qq2I")
 
@@ -228,7 +229,7 @@ def _norm(query_norm, key_norm, eps, head_dim, dtype, device, rot_axes, cols, ax
             raise ValueError("query_norm and key_norm must have the same dtype")
         code = 3 if t.dtype is torch.float32 else _dtypes[dtype]
         at[i] = t.data_ptr()
-    if not 0.0 <= eps < float("inf"):
+    if not 0.0 <= eps <= _F32_MAX:
         raise ValueError(f"norm_eps must be finite and not negative, got {eps}")
     where = 0
     if rot_axes is not None:
@@ -495,6 +496,8 @@ def _key_weights(t, shape, device):
     if t.dtype is not _torch.float32 or t.shape != shape or t.get_device() != device:
         raise ValueError(f"key_weights must be a float32 tensor of shape {tuple(shape)} on the device of key_cache, got "
                          f"{t.dtype} {tuple(t.shape)}")
+    if any(n > 1 and st == 0 for n, st in zip(t.shape, t.stride())):
+        raise ValueError("key_weights must not be expanded: every weight has memory of its own")
     return t.data_ptr(), _STRIDES.pack(*t.stride())
 
 
@@ -510,9 +513,10 @@ def paged_key_weights(query, lse, key_cache, block_tables, seq_lens, key_weights
     window_size and scale as the step's paged_attention or paged_prefix_attention
     had them, lse (float32 [rows, heads]) as it returned it; behind a prefix the
     weights are of the sequences' own keys.  key_weights: float32 [num_pages,
-    page_size, kv_heads], any strides.  The rows' own keys begin at 0, so weights
+    page_size, kv_heads], any strides but those of an expanded tensor.  The rows' own keys begin at 0, so weights
     of pages that are handed out again need no clearing.  decay: at least 0; with
-    0 old weights are not read.  Sequences without rows are left as they are.
+    0 old weights are not read.  Sequences without rows are left as they are.  No page
+    may belong to two sequences with rows: the sums of one of them could be lost.
     Returns None."""
     torch = _torch or _init()
     if not isinstance(query, torch.Tensor):
@@ -531,7 +535,7 @@ def paged_key_weights(query, lse, key_cache, block_tables, seq_lens, key_weights
     if not lse.is_contiguous():
         raise ValueError("lse must be contiguous")
     w, w_stride = _key_weights(key_weights, key_cache.shape[:3], device)
-    if not 0.0 <= decay < float("inf"):
+    if not 0.0 <= decay <= _F32_MAX:
         raise ValueError(f"decay must be finite and not negative, got {decay}")
     if rows == 0 or heads == 0 or seqs == 0:
         return

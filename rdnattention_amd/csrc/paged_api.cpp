@@ -527,6 +527,10 @@ std::string check_weights(const rdna_paged_cache* in, const float* w, const int6
         !stride_fits(stride[2], 4, in->num_kv_heads)) {
         return "the strides of key_weights must not be negative, and stay within 2^56 bytes";
     }
+    if ((in->num_pages > 1 && stride[0] == 0) || (in->page_size > 1 && stride[1] == 0) ||
+        (in->num_kv_heads > 1 && stride[2] == 0)) {
+        return "a stride of key_weights is zero: every weight has memory of its own";
+    }
     return "";
 }
 

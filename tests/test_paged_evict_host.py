@@ -136,3 +136,30 @@ def test_rows_that_see_a_key(tmp_path):
     r = subprocess.run([str(exe)], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0, r.stdout + r.stderr
     assert r.stdout.startswith("ok ")
+
+
+def test_refuses_expanded_weights(lib):  # noqa: F811
+    import rdnattention as ra
+
+    for i in range(3):  # one memory for several weights
+        stride = (ctypes.c_int64 * 3)(*(0 if j == i else s for j, s in enumerate((32, 2, 1))))
+        for call in (weights, evict):
+            rc, err = call(lib, cache(value=_P + 1024), stride=ctypes.addressof(stride))
+            assert rc == -3 and "memory of its own" in err, err
+        shape = [1 if j == i else n for j, n in enumerate(W.shape)]
+        w = torch.zeros(shape).expand(W.shape)
+        with pytest.raises(ValueError, match="expanded"):
+            ra.paged_evict(**tensors(), key_weights=w, budget=8)
+        with pytest.raises(ValueError, match="expanded"):
+            a = dict(tensors(), query=torch.zeros(4, 4, 64).half(), lse=torch.zeros(4, 4), key_weights=w)
+            a.pop("value_cache")
+            ra.paged_key_weights(**a)
+
+
+def test_refuses_a_decay_beyond_float():
+    import rdnattention as ra
+
+    a = dict(tensors(), query=torch.zeros(4, 4, 64).half(), lse=torch.zeros(4, 4), key_weights=W)
+    a.pop("value_cache")
+    with pytest.raises(ValueError, match="decay"):
+        ra.paged_key_weights(**a, decay=1e300)

@@ -115,3 +115,11 @@ def test_nothing_to_do():
     rows = torch.zeros(4, 2, 64, dtype=H)
     got = ra.paged_append(rows, rows, **t, query=q, query_norm=w, key_norm=w, cu_seqlens_q=i32(1))
     assert torch.equal(got, q)
+
+
+def test_refuses_an_eps_beyond_float():
+    import rdnattention as ra
+
+    rows = torch.zeros(4, 2, 64, dtype=H)
+    with pytest.raises(ValueError, match="norm_eps"):
+        ra.paged_append(rows, rows, **tensors(), key_norm=torch.ones(64), norm_eps=1e300)
