@@ -6,7 +6,7 @@
 // so that a key's sum stays in its lane, whatever its page holds reaches no other key,
 // and two workgroups that share a key leave their sums in order: no atomics, the same bits
 // every time.
-//   * few rows (up to 32 of a kv head): bound by HBM, K is read once
+//   * few rows (up to 128 of a kv head): bound by HBM up to 32, K is read once
 //   * more rows: bound by the exponentials beside the products.  A workgroup keeps a block of
 //     keys in registers and its waves take the row tiles in turn, Q through LDS one tile
 //     ahead
@@ -23,7 +23,10 @@ float softmax_log2_scale(float scale);
 namespace {
 
 constexpr int kTile = 32;    // keys and rows of a product
-constexpr int kFewRows = 32; // one row tile
+// Up to this many rows x heads of a kv head by paged_weights_few, which multiplies a key tile by
+// each row tile in turn.  16 sequences of 8192 bf16 keys, 8 kv heads of 128, us by few / many: 32
+// rows 47 / 156, 64 91 / 165, 128 174 / 192, 512 702 / 292.
+constexpr int kFewMax = 128;
 // one item per kv head of a sequence, its units blocks of keys
 constexpr int kAllRows = 1 << 30;
 constexpr float kLog2e = 1.4426950408889634f;
@@ -338,7 +341,9 @@ template <int D, bool I8>
 struct ManyCfg {
     static constexpr int WAVES = 4;
     static constexpr int THREADS = 64 * WAVES;
-    static constexpr int KT = D <= 64 ? 4 : D <= 128 ? 3 : 2; // 32-key tiles in registers
+    // 32-key tiles in registers (us of 2 prompts of 2048 rows, 32 heads, with one less: D 64 44.6 -> 46.8,
+    // D 128 61.8 -> 64.5, D 256 124 -> 181; with one more they do not fit)
+    static constexpr int KT = D <= 64 ? 4 : D <= 128 ? 3 : 2;
     static constexpr int BLOCK = kTile * KT;
     static constexpr int WAVES_PER_SIMD = D <= 128 ? 2 : 1;
     // of an item beside its row tiles (us of 2 prompts of 4096 rows with 8 / 16 / 24 / 32 / 40: 214 / 197 /
@@ -581,11 +586,11 @@ int launch_weights(const PagedWeightsArgs& a, WeightsParams& p, hipStream_t stre
         return 0;
     };
     // as in paged_attention: each launch takes the sequences of its kind
-    const bool any_many = (int64_t)a.max_rows_seq * p.work.G > kFewRows;
+    const bool any_many = (int64_t)a.max_rows_seq * p.work.G > kFewMax;
     const bool any_few = !any_many || a.seqs.cu != nullptr;
     PagedLaunch few, many;
     if (any_many && any_few) {
-        few.max_rows = many.min_rows = kFewRows;
+        few.max_rows = many.min_rows = kFewMax;
     }
     PagedWork wf = paged_work(p.work, few), wm = paged_work(p.work, many);
     wm.mask = p.mask;
