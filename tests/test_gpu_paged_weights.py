@@ -318,3 +318,13 @@ def test_offsets_past_32_bits(gpu):
         ra.paged_key_weights(q, lse, k, pool.table.to(gpu), lens, a)
         ra.paged_key_weights(q, lse, big, table, lens, b)
         assert torch.equal(b[table[0].long()], a[pool.table[0, :n].to(gpu).long()])
+
+
+@pytest.mark.parametrize("dtype,i8", TYPES)
+@pytest.mark.parametrize("window", [-1, 50])
+def test_between_one_row_tile_and_many(gpu, dtype, i8, window):
+    ns = [8, 9, 16, 17, 31, 32, 33, 40]  # with 4 heads of a kv head: 32 to 160 rows
+    lens = [300, 9, 700, 64, 31, 1000, 333, 50]
+    run(gpu, lens, ns, 8, 2, 64, dtype, i8, window=window, name=f"mixed rows {dtype} {i8}")
+    for n in (9, 32, 33):
+        run(gpu, lens, [n] * len(lens), 8, 2, 64, dtype, i8, window=window, uniform=True, name=f"{n} rows {dtype} {i8}")
