@@ -423,7 +423,8 @@ def paged_attention(query, key_cache, value_cache, block_tables, seq_lens, *, cu
     out: optional tensor like query to write to, whose padding rows stay as they
     are; a new tensor's are zeros.  Returns the output, with return_lse (output,
     lse): float32 [rows, heads], the logarithm of the sum of exp(score) over the
-    keys that the row sees, -inf where it sees none and of padding rows."""
+    keys that the row sees, -inf where it sees none and of padding rows.  The output
+    may differ in its last bit from the call without."""
     return _attend("paged_attention", query, key_cache, value_cache, block_tables, seq_lens, cu_seqlens_q, max_seqlen_q,
                    is_causal, window_size, scale, None, key_scale, value_scale, out, return_lse)
 

@@ -325,6 +325,7 @@
             oacc[dt] = f16x{};
         }
         float m_run = -INFINITY, l_run = 0.0f;
+        float p_run = 0.0f; // JOIN, 16-bit pages: the sum of the weights as the products take them
         f16x sacc[2] = {f16x{}, f16x{}};
         P8 pb[4] = {P8{}, P8{}, P8{}, P8{}};
         ValueScale vscale;
@@ -421,6 +422,9 @@
                     m_run = m_new;
                 }
                 l_run *= alpha;
+                if constexpr (JOIN && !I8) {
+                    p_run *= alpha;
+                }
 #pragma unroll
                 for (int dt = 0; dt < C::NDT; dt++) {
                     oacc[dt] *= alpha;
@@ -447,6 +451,7 @@
                     pb[e >> 3][e & 7] = (P)pv[e];
                 }
             } else {
+                float pr[4];
 #pragma unroll
                 for (int u = 0; u < 4; u++) {
 #pragma unroll
@@ -458,9 +463,13 @@
                             ps[u] += w;
                         }
                     }
+                    pr[u] = sum8<P>(pb[u], 0.0f); // of the weights as the products take them
                     if constexpr (!JOIN) {
-                        ps[u] = sum8<P>(pb[u], 0.0f); // of the weights as the products take them
+                        ps[u] = pr[u];
                     }
+                }
+                if constexpr (JOIN) {
+                    p_run += (pr[0] + pr[1]) + (pr[2] + pr[3]);
                 }
             }
             l_run += (ps[0] + ps[1]) + (ps[2] + ps[3]);
@@ -514,7 +523,13 @@
         }
 
         const float l_tot = pair_sum(l_run);
-        const float unit = I8 ? vscale.factor() : 1.0f; // of O
+        float unit = I8 ? vscale.factor() : 1.0f; // of O
+        if constexpr (JOIN && !I8) {
+            // O over the sum of the weights that made it, so that their rounding cancels where few
+            // keys count; l goes on to the log-sum-exp and weighs the parts
+            const float p_tot = pair_sum(p_run);
+            unit = p_tot > 0.0f ? l_tot / p_tot : 1.0f;
+        }
         if (JOIN && whole) {
             const PagedJoin& join = p.join;
             const int64_t row = (int64_t)(seq.q0 + tok) * join.Hq + head;
