@@ -17,6 +17,11 @@ namespace {
 
 constexpr int kThreads = 256;
 
+// Mean squares (with eps) that fp32 holds: squares below its normal range, off by up to 2^-150
+// each, are 2^-50 of the least at most, and above the most the sum is infinite.  bf16 rows can
+// be smaller or larger.
+constexpr float kLeastMean = 0x1p-100f, kMostMean = 0x1.fffffep127f;
+
 typedef int8_t b8 __attribute__((ext_vector_type(8)));
 
 template <class F>
@@ -96,6 +101,30 @@ template <class F>
 struct Wide {
     typedef F v8 __attribute__((ext_vector_type(8)));
 };
+
+// A head x, and eps, by a power of two such that the larger of |x| and sqrt(eps) is near 1: the
+// mean square and eps.
+template <int LANES>
+__device__ __forceinline__ float in_range(float (&x)[8], const NormParams& p) {
+    float mx = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        mx = fmaxf(mx, fabsf(x[e]));
+    }
+#pragma unroll
+    for (int d = 1; d < LANES; d <<= 1) {
+        mx = fmaxf(mx, from_lane(mx, (int)(threadIdx.x & 63) ^ d));
+    }
+    int by = mx > 0.0f ? -__builtin_amdgcn_frexp_expf(mx) : 1000;
+    by = min(by, p.n.eps > 0.0f ? -(__builtin_amdgcn_frexp_expf(p.n.eps) >> 1) : by);
+    float sum = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        x[e] = ldexpf(x[e], by);
+        sum = fmaf(x[e], x[e], sum);
+    }
+    return fmaf(group_sum<LANES>(sum), p.inv_d, ldexpf(p.n.eps, 2 * by));
+}
 
 // The angles of a lane's channels: of the pairs (2i, 2i + 1) four columns, of the
 // halves eight.
@@ -215,8 +244,12 @@ __global__ __launch_bounds__(kThreads) void paged_append_normed(NormParams p) {
             F r;
             if constexpr (sizeof(F) == 8) {
                 r = F(1) / __builtin_elementwise_sqrt(sum / (F)a.D + (F)p.n.eps);
-            } else { // good to 2^-23 itself
-                r = __builtin_amdgcn_rsqf(fmaf(sum, p.inv_d, p.n.eps));
+            } else {
+                float mean = fmaf(sum, p.inv_d, p.n.eps);
+                if (!(mean >= kLeastMean && mean <= kMostMean)) { // the lanes of a head are of one mind
+                    mean = in_range<LANES>(y, p);
+                }
+                r = __builtin_amdgcn_rsqf(mean); // good to 2^-23 itself
             }
             float w[8];
             load_weights(weights, p.n.type, chunk ? c : 0, w);
@@ -343,8 +376,8 @@ int paged_append_norm(const PagedAppendArgs& a, const PagedNorm& n, hipStream_t 
     p.inv_d = 1.0f / (float)a.D;
     // Groups per token: as many as it takes for 1024 lanes (of 2048) on each of the chip's 256
     // compute units, up to one for each head, and the groups of a wave at least.  us for 4853
-    // bf16 rows of 32 + 16 heads of 128 with three axes: 37 with 4 or 3 heads at a time, 38 with
-    // 2, 43 with 1; 50 with 2048 lanes.
+    // bf16 rows of 32 + 16 heads of 128 with three axes: 37 with 3 heads at a time, 38 with 2, 43
+    // with 1, 50 with 4 (more than the 96 registers of five waves on a SIMD); 50 with 2048 lanes.
     const int64_t heads = 2 * a.Hkv + a.Hq;
     auto go = [&](auto t, auto i8, auto lanes_of) {
         using T = decltype(t);
@@ -352,7 +385,7 @@ int paged_append_norm(const PagedAppendArgs& a, const PagedNorm& n, hipStream_t 
         constexpr int L = decltype(lanes_of)::value;
         const int64_t want = std::max<int64_t>((256 * 1024) / ((int64_t)a.seqs.total * L), 64 / L);
         const uint32_t per = (uint32_t)std::min(want, heads);
-        per * 2 > heads ? launch<T, I8, L, 1>(p, (uint32_t)heads, stream) : launch<T, I8, L, 4>(p, per, stream);
+        per * 2 > heads ? launch<T, I8, L, 1>(p, (uint32_t)heads, stream) : launch<T, I8, L, 3>(p, per, stream);
     };
     auto typed = [&](auto t) {
         if (a.i8) {
