@@ -6,7 +6,8 @@
 // so that a key's sum stays in its lane, whatever its page holds reaches no other key,
 // and two workgroups that share a key leave their sums in order: no atomics, the same bits
 // every time.
-//   * few rows (up to 128 of a kv head): bound by HBM up to 32, K is read once
+//   * few rows (up to 128 of a kv head): bound by HBM; K is read once for every 32 rows, by
+//     those that see it
 //   * more rows: bound by the exponentials beside the products.  A workgroup keeps a block of
 //     keys in registers and its waves take the row tiles in turn, Q through LDS one tile
 //     ahead
@@ -23,9 +24,17 @@ float softmax_log2_scale(float scale);
 namespace {
 
 constexpr int kTile = 32;    // keys and rows of a product
-// Up to this many rows x heads of a kv head by paged_weights_few, which multiplies a key tile by
-// each row tile in turn.  16 sequences of 8192 bf16 keys, 8 kv heads of 128, us by few / many: 32
-// rows 47 / 156, 64 91 / 165, 128 174 / 192, 512 702 / 292.
+// Up to this many rows x heads of a kv head by paged_weights_few, which goes over the keys for
+// each 32 of them.  Sequences of 8192 keys, 8 kv heads, us by few / many for 32 rows, 64, 96, 128 (at 16 sequences K stays in the last-level
+// cache, at 64, or 32 of D = 256, it does not):
+//   16, bf16, D 64          28 / 98   53 / 103   76 / 108   99 / 113
+//   16, bf16, D 128         48 / 154  91 / 166   132 / 181  174 / 192
+//   16, the same, window 1024  28 / 136  52 / 142   78 / 146   103 / 151
+//   16, int8, D 128         39 / 141  73 / 172   105 / 176  136 / 178
+//   64, bf16, D 64          111       222 / 424  333 / 446  443 / 464
+//   64, bf16, D 128         200       402 / 660  602 / 719  800 / 763
+//   64, int8, D 128         130       255 / 674  379 / 668  506 / 690
+//   32, bf16, D 256         175       345 / 764  519 / 834  693 / 929
 constexpr int kFewMax = 128;
 // one item per kv head of a sequence, its units blocks of keys
 constexpr int kAllRows = 1 << 30;
@@ -200,23 +209,33 @@ __global__ __launch_bounds__((64 * FewCfg<D, I8>::WAVES)) void paged_weights_few
         const int rows = uniform(seq.n * G);
         const int t0 = uniform(walk.tile.first + walk.begin());
         const int nt = uniform(walk.tile.hi >= walk.tile.lo && slot < step && h < p.Hkv ? walk.count() : 0);
-        const int mine = nt > slot ? (nt - slot + step - 1) / step : 0;
-        auto tile_key = [&](int j) { return (t0 + slot + step * j) * kTile; };
         i32x4_t tab_rsrc = make_rsrc_v(p.c.table + walk.b * p.c.table_s, (uint32_t)p.c.width * 4u);
 #pragma unroll
         for (int e = 0; e < 4; e++) {
             tab_rsrc[e] = uniform(tab_rsrc[e]);
         }
-        auto issue_tab = [&](int batch) __attribute__((always_inline)) {
-            const int t = (batch << log_b) + (lane >> log_n);
-            const int key = tile_key(t) + ((lane & ((1 << log_n) - 1)) << p.c.lps);
-            dma_load4(tab_rsrc, (uint32_t)(key >> p.c.lps) * 4u,
-                      (uint32_t)uniform((int)lds_w + C::TABS + 256 * (batch & 1)));
-        };
-
-        // one row tile (more only where the caller has said that there were fewer rows)
-        for (int base = 0; base < rows && mine > 0; base += kTile) {
+        // Row tiles in turn, each over the keys again.  The first has all of them, of which it reads
+        // those that a row of it sees and the others' weights alone, the later ones those tiles
+        // (each key's in the same wave).
+        for (int base = 0; base < rows; base += kTile) {
             const bool later = base > 0;
+            int key_lo, key_hi;
+            visible_key_range(paged_mask(p.mask, seq), base / G, (min(base + kTile, rows) - 1) / G, key_lo, key_hi);
+            key_lo = uniform(key_lo);
+            key_hi = uniform(key_hi);
+            const int first = t0 + (later ? max(key_lo / kTile - t0, 0) / step * step : 0) + slot;
+            const int end = later ? min(t0 + nt, key_hi >= key_lo ? key_hi / kTile + 1 : 0) : t0 + nt;
+            const int mine = end > first ? (end - first + step - 1) / step : 0;
+            if (mine == 0) {
+                continue;
+            }
+            auto tile_key = [&](int j) { return (first + step * j) * kTile; };
+            auto issue_tab = [&](int batch) __attribute__((always_inline)) {
+                const int t = (batch << log_b) + (lane >> log_n);
+                const int key = tile_key(t) + ((lane & ((1 << log_n) - 1)) << p.c.lps);
+                dma_load4(tab_rsrc, (uint32_t)(key >> p.c.lps) * 4u,
+                          (uint32_t)uniform((int)lds_w + C::TABS + 256 * (batch & 1)));
+            };
             // Of tile j: the keys' rows, and from lanes 0 - 31 their weights, from the others their
             // scales.  `w` is where the lane's key has its weight, 0 for none.
             uint64_t w = 0, w_next = 0, small = 0;
@@ -229,7 +248,7 @@ __global__ __launch_bounds__((64 * FewCfg<D, I8>::WAVES)) void paged_weights_few
                 const uint64_t off = (uint32_t)key & page_mask;
                 const uint64_t row = reinterpret_cast<uint64_t>(p.c.k) + pe * (uint64_t)p.c.k_sp +
                                      off * (uint64_t)p.c.k_st + (uint64_t)h * (uint64_t)p.c.k_sh;
-                rows_at[l32] = there ? row : zero;
+                rows_at[l32] = there && key >= key_lo && key <= key_hi ? row : zero;
                 w_next = there ? reinterpret_cast<uint64_t>(p.w) + 4 * (pe * (uint64_t)p.w_sp + off * (uint64_t)p.w_st +
                                                                         (uint64_t)h * (uint64_t)p.w_sh)
                                : 0;
