@@ -25,7 +25,8 @@ namespace {
 
 constexpr int kTile = 32;    // keys and rows of a product
 // Up to this many rows x heads of a kv head by paged_weights_few, which goes over the keys for
-// each 32 of them.  Sequences of 8192 keys, 8 kv heads, us by few / many for 32 rows, 64, 96, 128 (at 16 sequences K stays in the last-level
+// each 32 of them (launch_weights: fewer where waves of it are idle).  Sequences of 8192 keys, 8 kv
+// heads, us by few / many for 32 rows, 64, 96, 128 (at 16 sequences K stays in the last-level
 // cache, at 64, or 32 of D = 256, it does not):
 //   16, bf16, D 64          28 / 98   53 / 103   76 / 108   99 / 113
 //   16, bf16, D 128         48 / 154  91 / 166   132 / 181  174 / 192
@@ -604,16 +605,23 @@ int launch_weights(const PagedWeightsArgs& a, WeightsParams& p, hipStream_t stre
         }
         return 0;
     };
+    // Beyond 8 kv heads the last waves of a group of heads may be idle, which costs every row tile
+    // their share: us for 32 sequences of 8192 bf16 keys of 9 heads, D 128, few / many: 64 rows 286 /
+    // 372, 96 428 / 405; of 12 heads 96 512 / 551, 128 681 / 571; 16 of 9 heads, int8, 96 176 / 196,
+    // 128 232 / 203.  (With fewer heads HBM is busy all the same: 5 heads, 128 rows 242 / 252.
+    // Above D = 128 few is faster with idle waves too: 8 of 9 heads, D 256, 128 rows 213 / 261.)
+    constexpr int W = FewCfg<D, I8>::WAVES;
+    const int few_max = D > 128 || p.Hkv <= W ? kFewMax : (int)((int64_t)kFewMax * p.Hkv / ((p.Hkv + W - 1) / W * W));
     // as in paged_attention: each launch takes the sequences of its kind
-    const bool any_many = (int64_t)a.max_rows_seq * p.work.G > kFewMax;
+    const bool any_many = (int64_t)a.max_rows_seq * p.work.G > few_max;
     const bool any_few = !any_many || a.seqs.cu != nullptr;
     PagedLaunch few, many;
     if (any_many && any_few) {
-        few.max_rows = many.min_rows = kFewMax;
+        few.max_rows = many.min_rows = few_max;
     }
     PagedWork wf = paged_work(p.work, few), wm = paged_work(p.work, many);
     wm.mask = p.mask;
-    wf.Hkv = (p.Hkv + FewCfg<D, I8>::WAVES - 1) / FewCfg<D, I8>::WAVES;
+    wf.Hkv = (p.Hkv + W - 1) / W;
     const int64_t cf = any_few ? paged_max_cost<kAllRows, kTile, 0>(wf) : 0;
     using C = ManyCfg<D, I8>;
     const int64_t cm = any_many ? paged_max_key_cost<C::BLOCK, kTile, C::COST>(wm) : 0;
