@@ -44,11 +44,23 @@ RDNA_API int32_t rdna_attention_forward_path(
 RDNA_API int32_t rdna_scratch_trim(void);
 
 /* The scratch cache of HIP device `device`: bytes it holds, buffers it holds,
- * and the allocator calls (hipMallocAsync) the library has made for that
- * device's scratch since it was loaded.  For tests and monitoring; no
- * reference counterpart.  Returns 0, or -3 if an output pointer is null. */
+ * and the allocator calls (hipMallocAsync; hipMalloc for captured calls) the library
+ * has made for that device's scratch since it was loaded.  For tests and monitoring;
+ * no reference counterpart.  Returns 0, or -3 if an output pointer is null. */
 RDNA_API int32_t rdna_scratch_stats(int32_t device, uint64_t* cached_bytes, int64_t* entries,
                                     int64_t* allocations);
+
+/* Scratch of calls under stream capture is memory whose address is part of the graph:
+ * each graph has its own, the calls captured on one stream share it, and it is handed on
+ * to later captures, or freed by rdna_scratch_trim(), when the graph and its executables
+ * are destroyed.  So two graphs may be replayed side by side, but not two copies
+ * of one (executables instantiated from it, clones, child nodes), and a graph is
+ * destroyed after its last replay has finished.  A larger call of the same capture
+ * gets a block of its own, the smaller one stays for the graph's life.  The caps of
+ * the cache do not count these blocks: this reads the bytes and the number of those
+ * on `device`, owned or to be handed on.  Returns 0, or -3 if an output pointer is
+ * null. */
+RDNA_API int32_t rdna_graph_scratch_stats(int32_t device, uint64_t* bytes, int64_t* blocks);
 
 /* rdna_attention_forward() for callers that cannot allocate device memory
  * (code under HIP graph capture, tight serving loops, harnesses that forbid

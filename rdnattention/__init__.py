@@ -132,6 +132,9 @@ def _lib_handle():
             lib.rdna_scratch_stats.argtypes = [_I32, ctypes.POINTER(ctypes.c_uint64), ctypes.POINTER(_I64),
                                                ctypes.POINTER(_I64)]
             lib.rdna_scratch_stats.restype = _I32
+            if hasattr(lib, "rdna_graph_scratch_stats"):
+                lib.rdna_graph_scratch_stats.argtypes = [_I32, ctypes.POINTER(ctypes.c_uint64), ctypes.POINTER(_I64)]
+                lib.rdna_graph_scratch_stats.restype = _I32
         except AttributeError:
             pass
         lib.rdna_kernel_timer_enable.argtypes = [_I32]
@@ -435,12 +438,17 @@ def trim_scratch() -> None:
 def scratch_stats(device: int = 0) -> dict:
     """The scratch cache of HIP device `device`: {"cached_bytes", "entries",
     "allocations"}, the last being the allocator calls the library has made
-    for that device's scratch since it was loaded.  An extension."""
+    for that device's scratch since it was loaded, and the scratch of captured
+    calls, {"graph_bytes", "graph_blocks"}, whose graphs own it.  An extension."""
+    lib = _lib_handle()
     nbytes, entries, allocs = ctypes.c_uint64(), _I64(), _I64()
-    if _lib_handle().rdna_scratch_stats(int(device), ctypes.byref(nbytes), ctypes.byref(entries),
-                                        ctypes.byref(allocs)) != 0:
+    if lib.rdna_scratch_stats(int(device), ctypes.byref(nbytes), ctypes.byref(entries), ctypes.byref(allocs)) != 0:
         raise RDNAttentionError(f"scratch_stats failed: {last_error()}")
-    return {"cached_bytes": nbytes.value, "entries": entries.value, "allocations": allocs.value}
+    stats = {"cached_bytes": nbytes.value, "entries": entries.value, "allocations": allocs.value}
+    if hasattr(lib, "rdna_graph_scratch_stats"):  # absent from libraries built before it existed
+        lib.rdna_graph_scratch_stats(int(device), ctypes.byref(nbytes), ctypes.byref(entries))
+        stats.update(graph_bytes=nbytes.value, graph_blocks=entries.value)
+    return stats
 
 
 class KernelTimer:

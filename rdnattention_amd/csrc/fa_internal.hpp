@@ -31,7 +31,14 @@ constexpr size_t region_bytes(size_t bytes) {
 
 // What a scratch buffer holds; calls keep one cached buffer per (device,
 // stream, purpose), so buffers of one call never alias.
-enum class ScratchUse : int { RotatedK = 0, SplitKPartials = 1, QuantPartials = 2, Int8Scores = 3, PagedPartials = 4, PagedPrefix = 5 };
+enum class ScratchUse : int {
+    RotatedK = 0,
+    SplitKPartials = 1,
+    QuantPartials = 2,
+    Int8Scores = 3,
+    PagedPartials = 4,
+    PagedPrefix = 5
+};
 
 // Scratch memory for one call (scratch.cpp).  Without a region: the buffer
 // cached for (device, stream, use); a call that finds it large enough makes
@@ -79,6 +86,9 @@ int scratch_trim(std::string& err);
 // Cached scratch of `device`: bytes held, buffers held, and the allocator
 // calls made for it so far (cache growth and per-call blocks).  Always 0.
 int scratch_stats(int device, uint64_t& cached_bytes, int64_t& entries, int64_t& allocations);
+// Scratch of captured calls on `device`: bytes and blocks of graphs, those of graphs that
+// are gone and of no later one among them.
+void graph_scratch_stats(int device, uint64_t& bytes, int64_t& blocks);
 
 // The no-allocation entry point's region on the current device: the
 // library's static scratch array (fa_noalloc.hip), its device address looked

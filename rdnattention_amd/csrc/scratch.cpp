@@ -21,7 +21,9 @@
 //     and its executables are destroyed.  A memory node (hipMallocAsync under
 //     capture) will not do: the runtime gives the nodes of one graph the
 //     addresses of another's, so that two graphs replayed side by side on two streams
-//     use one buffer, and the records read from it lead anywhere.
+//     use one buffer, and the records read from it lead anywhere.  The address is part
+//     of the graph: copies of it must not run at the same time, nor its last replay
+//     behind its destruction.  These blocks are outside of the caps above.
 // rdna_scratch_trim() (the one synchronising path) frees every idle entry and
 // returns the default pool's free blocks to the device.
 #include "fa_internal.hpp"
@@ -90,11 +92,35 @@ struct GraphBlocks {
     std::mutex mu;
     std::map<GraphBlock::Key, GraphBlock*> held; // of each key the last
     std::vector<GraphBlock*> free;
+    std::map<int, std::pair<uint64_t, int64_t>> made; // by device: bytes and blocks, held and free
 };
 // Never destroyed: a graph may outlive the library's static objects.
 GraphBlocks& graph_blocks() {
     static auto* const blocks = new GraphBlocks;
     return *blocks;
+}
+
+// Returns the blocks that no graph owns to the devices (device < 0: all of them).
+void free_graph_blocks(int device) {
+    GraphBlocks& g = graph_blocks();
+    std::vector<GraphBlock*> blocks;
+    {
+        std::lock_guard<std::mutex> lock(g.mu);
+        const auto kept = std::partition(g.free.begin(), g.free.end(), [&](const GraphBlock* b) {
+            return device >= 0 && b->device != device;
+        });
+        blocks.assign(kept, g.free.end());
+        g.free.erase(kept, g.free.end());
+        for (const GraphBlock* b : blocks) {
+            auto& made = g.made[b->device];
+            made.first -= b->bytes;
+            made.second--;
+        }
+    }
+    for (GraphBlock* b : blocks) {
+        (void)hipFree(b->ptr);
+        delete b;
+    }
 }
 
 // User object's destructor: no HIP calls here.
@@ -126,6 +152,7 @@ int graph_block(size_t bytes, hipStream_t s, int use, int device, GraphBlock*& o
     }
     GraphBlocks& g = graph_blocks();
     GraphBlock* b = nullptr;
+    const size_t want = (bytes + kGranule - 1) / kGranule * kGranule;
     {
         std::lock_guard<std::mutex> lock(g.mu);
         const auto it = g.held.find({id, s, use});
@@ -134,9 +161,11 @@ int graph_block(size_t bytes, hipStream_t s, int use, int device, GraphBlock*& o
             out->busy = true;
             return 0;
         }
+        // the smallest that holds it, of up to twice the size: a graph keeps it for its life
         auto best = g.free.end();
         for (auto f = g.free.begin(); f != g.free.end(); ++f) {
-            if ((*f)->device == device && (*f)->bytes >= bytes && (best == g.free.end() || (*f)->bytes < (*best)->bytes)) {
+            if ((*f)->device == device && (*f)->bytes >= bytes && (*f)->bytes <= 2 * want &&
+                (best == g.free.end() || (*f)->bytes < (*best)->bytes)) {
                 best = f;
             }
         }
@@ -147,11 +176,15 @@ int graph_block(size_t bytes, hipStream_t s, int use, int device, GraphBlock*& o
     }
     if (b == nullptr) {
         void* ptr = nullptr;
-        const size_t want = (bytes + kGranule - 1) / kGranule * kGranule;
         hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed; // hipMalloc is no part of the capture
         e = hipThreadExchangeStreamCaptureMode(&mode);
         if (e == hipSuccess) {
             e = hipMalloc(&ptr, want);
+            if (e == hipErrorOutOfMemory) {
+                (void)hipGetLastError();
+                free_graph_blocks(device);
+                e = hipMalloc(&ptr, want);
+            }
             (void)hipThreadExchangeStreamCaptureMode(&mode);
         }
         if (e != hipSuccess) {
@@ -162,6 +195,10 @@ int graph_block(size_t bytes, hipStream_t s, int use, int device, GraphBlock*& o
         b->ptr = ptr;
         b->bytes = want;
         b->device = device;
+        std::lock_guard<std::mutex> lock(g.mu);
+        auto& made = g.made[device];
+        made.first += want;
+        made.second++;
     }
     b->key = {id, s, use};
     b->busy = true;
@@ -356,16 +393,7 @@ StreamScratch::~StreamScratch() {
 }
 
 int scratch_trim(std::string& err) {
-    // blocks of graphs that are gone
-    std::vector<GraphBlock*> blocks;
-    {
-        std::lock_guard<std::mutex> lock(graph_blocks().mu);
-        blocks.swap(graph_blocks().free);
-    }
-    for (GraphBlock* b : blocks) {
-        (void)hipFree(b->ptr);
-        delete b;
-    }
+    free_graph_blocks(-1);
     std::lock_guard<std::mutex> lock(g_mu);
     if (g_devices.empty()) {
         return 0; // nothing cached, no HIP call needed
@@ -433,6 +461,14 @@ int scratch_stats(int device, uint64_t& cached_bytes, int64_t& entries, int64_t&
         allocations = it->second.allocations;
     }
     return 0;
+}
+
+void graph_scratch_stats(int device, uint64_t& bytes, int64_t& blocks) {
+    GraphBlocks& g = graph_blocks();
+    std::lock_guard<std::mutex> lock(g.mu);
+    const auto it = g.made.find(device);
+    bytes = it != g.made.end() ? it->second.first : 0;
+    blocks = it != g.made.end() ? it->second.second : 0;
 }
 
 } // namespace rdna_amd
