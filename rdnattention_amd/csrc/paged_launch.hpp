@@ -107,6 +107,10 @@ int paged_stream_attention(const PagedAttnArgs& a, PagedAttnParams& p, const Pag
                            std::string& err);
 int paged_tile_attention(const PagedAttnArgs& a, PagedAttnParams& p, const PagedLaunch& l, hipStream_t stream,
                          std::string& err);
+// ... of rows whose keys are in two parts, or with the log-sum-exp (paged_stream_out.hip,
+// paged_tiles_join.hip)
+int paged_out_stream_attention(const PagedAttnArgs& a, PagedAttnParams& p, const PagedLaunch& l, hipStream_t stream,
+                               std::string& err);
 int paged_join_tile_attention(const PagedAttnArgs& a, PagedAttnParams& p, const PagedLaunch& l, hipStream_t stream,
                               std::string& err);
 // ... of few rows with their prefixes, in one launch

@@ -70,15 +70,61 @@ struct StreamCfg {
 template <class T, int D, bool I8, int WV>
 __global__ __launch_bounds__((StreamCfg<D, I8, WV>::THREADS), (StreamCfg<D, I8, WV>::WAVES_PER_SIMD)) void paged_stream(
     PagedAttnParams p) {
-    constexpr bool JOIN = false;
+    constexpr bool JOIN = false, OUT = false;
+#include "paged_stream_body.inl"
+}
+
+// A kernel of its own: asked for at the end of every item, the two ways out of a row cost
+// calls without a log-sum-exp 1.1 of 9.9 us (1 x 2048 keys, 8 heads of 128).
+template <class T, int D, bool I8, int WV>
+__global__ __launch_bounds__((StreamCfg<D, I8, WV>::THREADS), (StreamCfg<D, I8, WV>::WAVES_PER_SIMD)) void
+paged_out_stream(PagedAttnParams p) {
+    constexpr bool JOIN = false, OUT = true;
 #include "paged_stream_body.inl"
 }
 
 template <class T, int D, bool I8, int WV>
 __global__ __launch_bounds__((StreamCfg<D, I8, WV>::THREADS), (StreamCfg<D, I8, WV>::WAVES_PER_SIMD)) void
 paged_join_stream(PagedAttnParams p) {
-    constexpr bool JOIN = true;
+    constexpr bool JOIN = true, OUT = false;
 #include "paged_stream_body.inl"
+}
+
+// Workers are workgroups; smallest share: a tile for every wave.
+template <bool OUT>
+int paged_stream_launch(const PagedAttnArgs& a, PagedAttnParams& p, const PagedLaunch& l, hipStream_t stream,
+                        std::string& err) {
+    return paged_for_type(a, [&](auto t, auto d, auto i8) {
+        using T = decltype(t);
+        constexpr int D = decltype(d)::value;
+        constexpr bool I8 = decltype(i8)::value;
+        auto run = [&](auto* kernel, int waves) {
+            return paged_launch<kRows, kTile, 0>(
+                a, reinterpret_cast<const void*>(kernel), 64 * waves, waves, p, l, stream, err,
+                [&](dim3 grid) { hipLaunchKernelGGL(kernel, grid, dim3(64 * waves), 0, stream, p); });
+        };
+        auto go = [&](auto waves) {
+            constexpr int WV = decltype(waves)::value;
+            if constexpr (OUT) {
+                return run(&paged_out_stream<T, D, I8, WV>, WV);
+            } else {
+                return run(&paged_stream<T, D, I8, WV>, WV);
+            }
+        };
+        // Eight waves on a CU where there are few heads: one workgroup, which streams
+        // a head's keys in one front; where there are many, two of four waves, of
+        // which one begins and ends heads while the other streams.  us of eight / four,
+        // 8 heads, 16 x 18432 keys, 64 x 375 to 3000 keys, 128 x 512: D = 128 192 / 200, 101 /
+        // 94, 57 / 52; D = 96 190 / 192, 96 / 92, 55 / 50; int8 at D = 128, 32 x 8192 keys 115 /
+        // 120, 64 x 375 to 3000 78 / 63.  At D = 64 four are faster with few heads too (16 x
+        // 18432 117 / 107), but for int8 (75 / 79).
+        if constexpr (D == 96 || D == 128) {
+            if ((int64_t)a.seqs.B * a.Hkv < kManyHeads) {
+                return go(std::integral_constant<int, 8>{});
+            }
+        }
+        return go(std::integral_constant<int, 4>{});
+    });
 }
 
 } // namespace

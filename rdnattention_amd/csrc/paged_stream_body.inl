@@ -1,6 +1,7 @@
 // Body of the paged_stream kernels (paged_stream.hpp), included into each of them.  In
 // scope: T, D, I8, WV, JOIN (prefixes and sequences in one launch, every row's parts
-// left for paged_merge_parts) and the parameters p.
+// left for paged_merge_parts), OUT (rows whose keys are in two parts, or whose log-sum-exp
+// is asked for) and the parameters p.
     using C = StreamCfg<D, I8, WV>;
     using V8 = typename PagedVec<T>::v8;
     using V4 = typename PagedVec<T>::v4;
@@ -398,7 +399,7 @@
                     if (d == 0) {
                         *reinterpret_cast<float2*>(p.join.whole_ml + row * 2) = float2{mref, lsum};
                     }
-                } else if (whole && p.join.any()) {
+                } else if (OUT && whole) {
                     const int tk = (r0 + col) / G, hd = h * G + r0 + col - tk * G;
                     const int64_t row = (int64_t)(seq.q0 + tk) * p.Hq + hd;
                     const PagedRowOut out = paged_row_out(p.join, row, mref, lsum);
