@@ -398,10 +398,7 @@ struct PagedItemWalk {
                     u = n * (Items::all(s).units + EXTRA);
                 }
             } else if (!MANY || n <= kFewTiles) {
-                for (int32_t x = 0; x < n; x++) {
-                    u += Items::tile(w, s, x).units;
-                }
-                u += n * EXTRA;
+                u = Items::units(w, s, n) + n * EXTRA;
             }
             if constexpr (MANY) {
                 for (uint64_t more = __builtin_amdgcn_ballot_w64(n > kFewTiles); more != 0; more &= more - 1) {

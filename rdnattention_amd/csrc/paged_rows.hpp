@@ -175,15 +175,19 @@ RDNA_MASK_FN PagedTile paged_tile(const PagedWork& w, const PagedSeq& s, int32_t
     return t;
 }
 
-// Units of one kv head of a sequence.
+// Units of one kv head of a sequence, which has n row tiles.  (A caller that knows n to be small
+// tells the compiler so: counted again here, it is a loop of 1.2 us at a kernel's begin.)
 template <int ROWS, int BN>
-RDNA_MASK_FN int32_t paged_head_units(const PagedWork& w, const PagedSeq& s) {
-    const int32_t n = paged_row_tiles<ROWS>(w, s.n);
+RDNA_MASK_FN int32_t paged_head_units(const PagedWork& w, const PagedSeq& s, int32_t n) {
     int32_t u = 0;
     for (int32_t rt = 0; rt < n; rt++) {
         u += paged_tile<ROWS, BN>(w, s, rt).units;
     }
     return u;
+}
+template <int ROWS, int BN>
+RDNA_MASK_FN int32_t paged_head_units(const PagedWork& w, const PagedSeq& s) {
+    return paged_head_units<ROWS, BN>(w, s, paged_row_tiles<ROWS>(w, s.n));
 }
 
 // Items of a call: of a sequence and kv head its row tiles, whose units are key tiles.
@@ -194,6 +198,10 @@ struct PagedRowItems {
     }
     static RDNA_MASK_FN PagedTile tile(const PagedWork& w, const PagedSeq& s, int32_t i) {
         return paged_tile<ROWS, BN>(w, s, i);
+    }
+    // of one kv head with n items
+    static RDNA_MASK_FN int32_t units(const PagedWork& w, const PagedSeq& s, int32_t n) {
+        return paged_head_units<ROWS, BN>(w, s, n);
     }
     // any of those whose rows see all keys
     static RDNA_MASK_FN PagedTile all(const PagedSeq& s) {
@@ -213,6 +221,13 @@ struct PagedKeyItems {
         const int32_t lo = paged_key_rows(w.mask, s, w.G, i * BLOCK).lo;
         const int32_t hi = paged_key_rows(w.mask, s, w.G, mask_imin((i + 1) * BLOCK, s.len) - 1).hi;
         return lo <= hi ? PagedTile{lo, hi, lo / ROWS, hi / ROWS + 1 - lo / ROWS} : PagedTile{0, -1, 0, 1};
+    }
+    static RDNA_MASK_FN int32_t units(const PagedWork& w, const PagedSeq& s, int32_t n) {
+        int32_t u = 0;
+        for (int32_t i = 0; i < n; i++) {
+            u += tile(w, s, i).units;
+        }
+        return u;
     }
 };
 
