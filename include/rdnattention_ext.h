@@ -30,8 +30,8 @@ RDNA_API int32_t rdna_attention_forward_path(
     int32_t path, void* hip_stream);
 
 /* Releases the device memory the library keeps for reuse: the scratch
- * buffers (RoPE-rotated K copies, split-K and paged partials, quantiser
- * partials, INT8 decode scores) it caches per (device, stream, use), grown to the largest
+ * buffers (RoPE-rotated K copies, split-K and paged partials, prefixes' parts,
+ * quantiser partials, INT8 decode scores) it caches per (device, stream, use), grown to the largest
  * call so far (at most 256 MiB each, at most 1 GiB per device over all
  * streams and uses), the scratch of captured graphs that have been destroyed,
  * and the free blocks of the devices' default memory pools.  A call never frees or
@@ -340,7 +340,11 @@ typedef struct rdna_paged_prefix {
  * prefix is read once for all of its sequences.  lse, if not null: float [num_rows,
  * num_heads], the logarithm of the sum of exp(score) over the keys that a row sees, -inf
  * where there is none; of the rows behind the last sequence (where cu_seqlens is given)
- * -inf whether or not zero_tail is set. */
+ * -inf whether or not zero_tail is set.  The prefixes' part of every row is scratch: num_rows
+ * x num_heads x (head_dim + 1) floats (unless there are few: up to 32 rows of a kv head, 2048
+ * rows x heads and 512 sequences x kv heads), above 256 MiB allocated anew by every call
+ * (hipMallocAsync); without that memory the call fails with -3, before it has written
+ * anything. */
 RDNA_API int32_t rdna_paged_attention_lse(
     const rdna_paged_cache* cache, const rdna_paged_prefix* prefix, const void* query, void* output,
     int64_t query_stride_row, int64_t query_stride_h, int64_t output_stride_row, int64_t output_stride_h,

@@ -443,7 +443,8 @@ def paged_prefix_attention(query, key_cache, value_cache, prefix_tables, prefix_
     keys alone, all else as in paged_attention: every row sees the whole prefix,
     and its own keys as is_causal says.  Each prefix is read once for all of its
     sequences.  A length of 0 is no prefix.  (A position in the text is the
-    prefix's length more than the row's index: paged_append's positions.)"""
+    prefix's length more than the row's index: paged_append's positions.)  Calls of
+    many rows take scratch of rows * heads * (head_dim + 1) float32."""
     return _attend("paged_prefix_attention", query, key_cache, value_cache, block_tables, seq_lens, cu_seqlens_q,
                    max_seqlen_q, is_causal, -1, scale, None, key_scale, value_scale, out, return_lse,
                    (prefix_tables, prefix_lens, prefix_seqs))
