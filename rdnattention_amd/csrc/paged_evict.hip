@@ -380,8 +380,8 @@ int paged_evict(const PagedEvictArgs& a, hipStream_t stream, std::string& err) {
     if (launched() != 0) {
         return -1;
     }
-    hipLaunchKernelGGL(paged_evict_move, dim3((uint32_t)(a.Hkv * (2 * p.slices + 1)), (uint32_t)a.B), dim3(kMoveThreads), 0, stream,
-                       p);
+    hipLaunchKernelGGL(paged_evict_move, dim3((uint32_t)(a.Hkv * (2 * p.slices + 1)), (uint32_t)a.B),
+                       dim3(kMoveThreads), 0, stream, p);
     return launched();
 }
 

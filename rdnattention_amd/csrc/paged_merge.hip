@@ -301,7 +301,7 @@ int paged_attention(const PagedAttnArgs& a, hipStream_t stream, std::string& err
     PagedAttnParams shared = p;
     bool together = false;
     if (a.prefix.n > 0) {
-                constexpr int64_t kItems = 512, kSharedRows = 2048;
+        constexpr int64_t kItems = 512, kSharedRows = 2048;
         together = !any_many && (int64_t)a.seqs.B * a.Hkv <= kItems && (int64_t)a.seqs.total * a.Hq <= kSharedRows;
         PagedSeqs& s = shared.work.seqs;
         s.prefixes = a.prefix.n;

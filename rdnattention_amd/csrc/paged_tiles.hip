@@ -11,7 +11,7 @@ int64_t paged_tile_cost(const PagedAttnArgs& a, const PagedWork& w) {
 int paged_tile_attention(const PagedAttnArgs& a, PagedAttnParams& p, const PagedLaunch& l, hipStream_t stream,
                          std::string& err) {
     return p.join.any() ? paged_join_tile_attention(a, p, l, stream, err)
-                     : paged_tile_launch<false>(a, p, l, stream, err);
+                        : paged_tile_launch<false>(a, p, l, stream, err);
 }
 
 } // namespace rdna_amd
