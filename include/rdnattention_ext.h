@@ -341,10 +341,9 @@ typedef struct rdna_paged_prefix {
  * num_heads], the logarithm of the sum of exp(score) over the keys that a row sees, -inf
  * where there is none; of the rows behind the last sequence (where cu_seqlens is given)
  * -inf whether or not zero_tail is set.  The prefixes' part of every row is scratch: num_rows
- * x num_heads x (head_dim + 1) floats (unless there are few: up to 32 rows of a kv head, 2048
- * rows x heads and 512 sequences x kv heads), above 256 MiB allocated anew by every call
- * (hipMallocAsync); without that memory the call fails with -3, before it has written
- * anything. */
+ * x num_heads x (head_dim + 1) floats (of calls with few rows up to 18 MB), above 256 MiB
+ * allocated anew by every call (hipMallocAsync); without that memory the call fails with
+ * -3, before it has written anything. */
 RDNA_API int32_t rdna_paged_attention_lse(
     const rdna_paged_cache* cache, const rdna_paged_prefix* prefix, const void* query, void* output,
     int64_t query_stride_row, int64_t query_stride_h, int64_t output_stride_row, int64_t output_stride_h,

@@ -293,24 +293,34 @@ int paged_attention(const PagedAttnArgs& a, hipStream_t stream, std::string& err
     // the sequences, or the prefixes have one, by tiles, of their own before the sequences'.
     // The one saves two launches and a pass over the rows, but its row tiles are 32 rows, each
     // of which reads the prefix again, and every sequence's kv head is an item of it with a
-    // begin and an end of its own: for few rows of every sequence, up to kItems sequences x
-    // kv heads and kSharedRows rows x heads.  8192 keys of one prefix, 300 of each sequence, D
-    // 128, us in one launch / by tiles first: 8 sequences of 32 heads on 8 kv heads 24 / 44,
-    // 32 35 / 54, 64 52 / 67, 96 92 / 80, 128 87 / 86, 256 174 / 129; 32 on 32 16 sequences 58
-    // / 60, 32 91 / 77; 32 on 1 64 42 / 70; 64 on 8 32 53 / 60, 64 81 / 73.
+    // begin and an end of its own: up to kItems sequences x kv heads and kUnits key tiles of all
+    // the prefixes' row tiles, as far as their table's width tells.  us by tiles first / in one
+    // launch, one token of each sequence, bf16, 32 heads on 8, D 128, 300 own keys, prefixes of
+    // 500, 8192 and 32768 keys: 8 sequences 42 / 21, 49 / 29, 64 / 44; 32 41 / 30, 58 / 38, 75 / 106;
+    // 64 54 / 43, 72 / 58, 98 / 199; 96 67 / 56, 86 / 103, 131 / 293; 128 71 / 69, 92 / 94, 142 /
+    // 387; of 32 heads on 32, D 64, 32 53 / 39, 69 / 57; 128 96 / 118, 111 / 184; 32 on 1, D 128, 128
+    // 66 / 42, 85 / 75; 16 on 8, D 256, 64 74 / 61, 102 / 110.  Over 600 calls of 2 to 300
+    // sequences, 1 to 12 prefixes of 100 to 60000 keys, 10 to 3000 own ones, this rule is 1.2 % off
+    // the faster form (geometric mean), kItems 512 without kUnits was 3.8 %.
     PagedAttnParams shared = p;
     bool together = false;
     if (a.prefix.n > 0) {
-        constexpr int64_t kItems = 512, kSharedRows = 2048;
-        together = !any_many && (int64_t)a.seqs.B * a.Hkv <= kItems && (int64_t)a.seqs.total * a.Hq <= kSharedRows;
+        constexpr int64_t kItems = 1024, kUnits = 32768, kSharedRows = 8192;
+        const double tiles = (double)a.seqs.total * p.work.G / 32 + a.prefix.n;
+        const double units = tiles * a.Hkv * ((int64_t)a.prefix.width << a.c.lps) / 32;
+        together = !any_many && (int64_t)a.seqs.B * a.Hkv <= kItems && units * a.D <= (double)kUnits * 128 &&
+                   (int64_t)a.seqs.total * a.Hq <= kSharedRows;
         PagedSeqs& s = shared.work.seqs;
         s.prefixes = a.prefix.n;
         s.members = a.seqs.B;
         s.prefix_lens = a.prefix.lens;
         s.prefix_keys = (int32_t)((int64_t)a.prefix.width << a.c.lps);
         s.group = a.prefix.seqs;
-        s.B = a.prefix.n + (together ? a.seqs.B : 0);
+        s.B = a.prefix.n + a.seqs.B;
+        // (with more key tiles than it can count, each launch may still count its own)
+        together = together && paged_join_cost(paged_work(shared.work, PagedLaunch{})) <= INT32_MAX;
         if (!together) {
+            s.B = a.prefix.n;
             shared.c.table = a.prefix.table;
             shared.c.table_s = a.prefix.table_s;
             shared.c.width = a.prefix.width;
@@ -320,17 +330,12 @@ int paged_attention(const PagedAttnArgs& a, hipStream_t stream, std::string& err
         }
     }
     // refused before the first of the launches has written anything
-    int64_t cost;
-    if (together) {
-        cost = paged_join_cost(paged_work(shared.work, PagedLaunch{}));
-    } else {
-        cost = std::max(any_many ? paged_tile_cost(a, paged_work(p.work, many)) : 0,
-                        any_few ? paged_stream_cost(a, paged_work(p.work, few)) : 0);
-        if (a.prefix.n > 0) {
-            cost = std::max(cost, paged_tile_cost(a, paged_work(shared.work, PagedLaunch{})));
-        }
+    int64_t cost = std::max(any_many ? paged_tile_cost(a, paged_work(p.work, many)) : 0,
+                            any_few ? paged_stream_cost(a, paged_work(p.work, few)) : 0);
+    if (a.prefix.n > 0 && !together) {
+        cost = std::max(cost, paged_tile_cost(a, paged_work(shared.work, PagedLaunch{})));
     }
-    if (cost > INT32_MAX) {
+    if (!together && cost > INT32_MAX) {
         err = "too many rows x heads x keys that the page table covers (up to " +
               (cost == INT64_MAX ? std::string("2^63") : std::to_string(cost)) + " key tiles, at most 2^31 - 1)";
         return -1;
