@@ -265,9 +265,9 @@ typedef struct rdna_paged_cache {
  * (2i, 2i + 1) by column i (rot_interleaved) or (i, i + rot_dim / 2); positions
  * outside the tables are taken as their first or last row.  With query, the query
  * rows [num_rows, num_heads, head_dim] are rotated likewise into query_out (query itself
- * with its strides, or memory that does not overlap it).  Rows without a place write nothing; their query rows come out as they
- * are (rotated if positions are given, and the row is a sequence's).  rot_dim is a
- * multiple of 16. */
+ * with its strides, or memory that does not overlap it).  Rows without a place write
+ * nothing; their query rows come out as they are (rotated if positions are given, and the
+ * row is a sequence's).  rot_dim is a multiple of 16. */
 RDNA_API int32_t rdna_paged_append(
     const rdna_paged_cache* cache, const void* key, const void* value, int64_t key_stride_row, int64_t key_stride_h,
     int64_t value_stride_row, int64_t value_stride_h, uint32_t num_rows, int32_t dtype, const void* query,

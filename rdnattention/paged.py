@@ -319,8 +319,8 @@ def paged_append(key, value, key_cache, value_cache, block_tables, seq_lens, *, 
     elif query_norm is not None:
         raise ValueError("query_norm needs query")
     if query_norm is not None or key_norm is not None or rot_axes is not None:
-        norm = _norm(query_norm if query is None or heads else None, key_norm, norm_eps, head_dim, dtype, device, rot_axes,
-                     rot_dim // 2, axes, pos_stride)
+        norm = _norm(query_norm if query is None or heads else None, key_norm, norm_eps, head_dim, dtype, device,
+                     rot_axes, rot_dim // 2, axes, pos_stride)
     if rows == 0:
         return out
     if seqs == 0:  # nothing but padding
@@ -339,7 +339,8 @@ def _prefix(tables, lens, seqs, device):
     table, (n, width), stride = _index("prefix_tables", tables, 2, device)
     at, shape, _ = _index("prefix_lens", lens, 1, device)
     if n == 0 or shape[0] != n:
-        raise ValueError(f"prefix_lens must have one entry per row of prefix_tables ({n}, at least one), got {shape[0]}")
+        raise ValueError(f"prefix_lens must have one entry per row of prefix_tables ({n}, at least one), got "
+                         f"{shape[0]}")
     of = 0
     if seqs is not None:
         of, shape, _ = _index("prefix_seqs", seqs, 1, device)
@@ -496,8 +497,8 @@ def _key_weights(t, shape, device):
     if not isinstance(t, _torch.Tensor):
         raise TypeError("key_weights must be a torch.Tensor")
     if t.dtype is not _torch.float32 or t.shape != shape or t.get_device() != device:
-        raise ValueError(f"key_weights must be a float32 tensor of shape {tuple(shape)} on the device of key_cache, got "
-                         f"{t.dtype} {tuple(t.shape)}")
+        raise ValueError(f"key_weights must be a float32 tensor of shape {tuple(shape)} on the device of key_cache, "
+                         f"got {t.dtype} {tuple(t.shape)}")
     if any(n > 1 and st == 0 for n, st in zip(t.shape, t.stride())):
         raise ValueError("key_weights must not be expanded: every weight has memory of its own")
     return t.data_ptr(), _STRIDES.pack(*t.stride())
@@ -542,8 +543,8 @@ def paged_key_weights(query, lse, key_cache, block_tables, seq_lens, key_weights
     if rows == 0 or heads == 0 or seqs == 0:
         return
     most = rows if max_seqlen_q is None else max(0, min(rows, int(max_seqlen_q)))
-    _call(device, "paged_key_weights", _newer("rdna_paged_key_weights"), c, q, qs[0], qs[1], rows, heads, _dtypes[dtype],
-          most, lse.data_ptr(), head_dim ** -0.5 if scale is None else float(scale), 1 if is_causal else 0,
+    _call(device, "paged_key_weights", _newer("rdna_paged_key_weights"), c, q, qs[0], qs[1], rows, heads,
+          _dtypes[dtype], most, lse.data_ptr(), head_dim ** -0.5 if scale is None else float(scale), 1 if is_causal else 0,
           max(-1, min(int(window_size), 2 ** 31 - 1)), decay, w, w_stride)
 
 
@@ -569,7 +570,8 @@ def paged_evict(key_cache, value_cache, block_tables, seq_lens, key_weights, bud
     if not 0 < budget <= 1 << 28:
         raise ValueError(f"budget must be 1 to 2^28, got {budget}")
     if first < 0 or recent < 0 or first + recent > budget:
-        raise ValueError(f"first ({first}) and recent ({recent}) must not be negative, nor exceed budget ({budget}) together")
+        raise ValueError(f"first ({first}) and recent ({recent}) must not be negative, nor exceed budget ({budget}) "
+                         "together")
     lens = torch.empty(seqs, dtype=torch.int32, device=key_cache.device)
     kept = torch.empty(seqs, kv_heads, budget, dtype=torch.int32, device=key_cache.device)
     if seqs:

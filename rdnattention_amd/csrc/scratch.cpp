@@ -147,7 +147,8 @@ int graph_block(size_t bytes, hipStream_t s, int use, int device, GraphBlock*& o
     size_t n_deps = 0;
     hipError_t e = hipStreamGetCaptureInfo_v2(s, &status, &id, &graph, &deps, &n_deps);
     if (e != hipSuccess || graph == nullptr) {
-        err = hip_err("scratch allocation under capture failed", e != hipSuccess ? e : hipErrorStreamCaptureInvalidated);
+        err = hip_err("scratch allocation under capture failed",
+                      e != hipSuccess ? e : hipErrorStreamCaptureInvalidated);
         return -1;
     }
     GraphBlocks& g = graph_blocks();

@@ -23,10 +23,11 @@ def test_windows_and_heads(gpu, hq, hkv, causal, window):
 @pytest.mark.parametrize("window", [-1, 50])
 def test_more_row_tiles_than_said(gpu, d, i8, dtype, window):
     """A max_seqlen_q below the rows: any number of row tiles, on sequences split over workers."""
-    run(gpu, [6000, 900, 300], [70, 300, 300], 8, 2, d, dtype, i8, window=window, max_q=1, name=f"said 1, window {window}")
+    run(gpu, [6000, 900, 300], [70, 300, 300], 8, 2, d, dtype, i8, window=window, max_q=1,
+        name=f"said 1, window {window}")
 
 
 @pytest.mark.parametrize("window", [40, 300])
 def test_long_sequences(gpu, window):
-    run(gpu, [30000, 20011], [60, 31], 8, 4, 64, BF16, window=window, decay=0.9, spoil=True, name=f"long, window {window}")
-    run(gpu, [30000, 20011], [60, 31], 8, 4, 64, BF16, window=window, causal=False, page=1, name=f"pages of 1, window {window}")
+    run(gpu, [30000, 20011], [60, 31], 8, 4, 64, BF16, window=window, decay=0.9, spoil=True, name=f"long {window}")
+    run(gpu, [30000, 20011], [60, 31], 8, 4, 64, BF16, window=window, causal=False, page=1, name=f"pages of 1 {window}")
