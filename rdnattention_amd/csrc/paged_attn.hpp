@@ -82,11 +82,15 @@ struct PagedAttnParams {
     int64_t tree_sb, tree_sr;
     int32_t tree_n;
     int32_t slot_rows; // rows of a slot
+    int32_t zero_tail; // kTailOut, kTailLse (read at the begin, with what is above)
     float* part_o;
     float* part_ml;
     PagedRecord* records;
+};
+// ... of the kernels that join parts or give log-sum-exps.  (Arguments of their own: 104 bytes
+// more of each launch cost calls without them 0.2 us of the host.)
+struct PagedJoinParams : PagedAttnParams {
     PagedJoin join;
-    int32_t zero_tail; // kTailOut, kTailLse
 };
 
 // zero_tail
@@ -614,7 +618,7 @@ __device__ __forceinline__ void tree_mask_scores(f16x (&s)[N], const uint8_t* ro
 
 // Zeros (log-sum-exp: -inf) for the rows behind the last sequence, dealt to the workgroups.
 template <int D>
-__device__ __forceinline__ void zero_tail_rows(const PagedAttnParams& p) {
+__device__ __forceinline__ void zero_tail_rows(const PagedAttnParams& p, float* lse) {
     constexpr int CH = D / 8;
     const int32_t per_row = p.Hq * CH;
     for (int32_t t = paged_rows_end(p.work.seqs) + blockIdx.x; t < p.work.seqs.total; t += gridDim.x) {
@@ -626,7 +630,7 @@ __device__ __forceinline__ void zero_tail_rows(const PagedAttnParams& p) {
         }
         if ((p.zero_tail & kTailLse) != 0) {
             for (int32_t h = threadIdx.x; h < p.Hq; h += blockDim.x) {
-                p.join.lse[(int64_t)t * p.Hq + h] = -INFINITY;
+                lse[(int64_t)t * p.Hq + h] = -INFINITY;
             }
         }
     }

@@ -29,7 +29,7 @@ inline PagedWork paged_work(const PagedWork& call, const PagedLaunch& l) {
 
 // The merge of the items that several workgroups share (paged_merge.hip), or of every row's
 // parts where p.join.parts says where they are.
-int paged_merge(const PagedAttnArgs& a, const PagedAttnParams& p, hipStream_t stream, std::string& err);
+int paged_merge(const PagedAttnArgs& a, const PagedJoinParams& p, hipStream_t stream, std::string& err);
 
 // Workers (workgroups) for at most `units` units in shares of min_units at least.
 inline int paged_workgroups(int64_t resident, int64_t units, int min_units) {
@@ -43,7 +43,7 @@ constexpr size_t paged_scratch_bytes(int n_wg, int rows, int D) {
 }
 
 template <int ROWS, int BN, int EXTRA, class Go>
-int paged_launch(const PagedAttnArgs& a, const void* kernel, int threads, int min_units, PagedAttnParams& p,
+int paged_launch(const PagedAttnArgs& a, const void* kernel, int threads, int min_units, PagedJoinParams& p,
                  const PagedLaunch& l, hipStream_t stream, std::string& err, Go&& go) {
     const int64_t resident = resident_workgroups(kernel, threads, err);
     if (resident <= 0) {
@@ -103,18 +103,18 @@ int paged_for_type(const PagedAttnArgs& a, F&& f) {
 }
 
 // The kernels of few rows (paged_stream.hip) and of many (paged_tiles.hip).
-int paged_stream_attention(const PagedAttnArgs& a, PagedAttnParams& p, const PagedLaunch& l, hipStream_t stream,
+int paged_stream_attention(const PagedAttnArgs& a, PagedJoinParams& p, const PagedLaunch& l, hipStream_t stream,
                            std::string& err);
-int paged_tile_attention(const PagedAttnArgs& a, PagedAttnParams& p, const PagedLaunch& l, hipStream_t stream,
+int paged_tile_attention(const PagedAttnArgs& a, PagedJoinParams& p, const PagedLaunch& l, hipStream_t stream,
                          std::string& err);
 // ... of rows whose keys are in two parts, or with the log-sum-exp (paged_stream_out.hip,
 // paged_tiles_join.hip)
-int paged_out_stream_attention(const PagedAttnArgs& a, PagedAttnParams& p, const PagedLaunch& l, hipStream_t stream,
+int paged_out_stream_attention(const PagedAttnArgs& a, PagedJoinParams& p, const PagedLaunch& l, hipStream_t stream,
                                std::string& err);
-int paged_join_tile_attention(const PagedAttnArgs& a, PagedAttnParams& p, const PagedLaunch& l, hipStream_t stream,
+int paged_join_tile_attention(const PagedAttnArgs& a, PagedJoinParams& p, const PagedLaunch& l, hipStream_t stream,
                               std::string& err);
 // ... of few rows with their prefixes, in one launch
-int paged_join_stream_attention(const PagedAttnArgs& a, PagedAttnParams& p, hipStream_t stream, std::string& err);
+int paged_join_stream_attention(const PagedAttnArgs& a, PagedJoinParams& p, hipStream_t stream, std::string& err);
 int64_t paged_join_cost(const PagedWork& w);
 // ... and what a launch of them may cost at most (paged_max_cost).
 int64_t paged_stream_cost(const PagedAttnArgs& a, const PagedWork& w);

@@ -5,6 +5,7 @@
 #include <algorithm>
 #include <cstdint>
 #include <string>
+#include <type_traits>
 
 namespace rdna_amd {
 
@@ -15,8 +16,9 @@ namespace {
 constexpr int kMergeThreads = 256;
 constexpr int kMergeRows = 8; // rows of a merge workgroup at most
 
+template <bool JOIN>
 struct MergeParams {
-    PagedAttnParams p;
+    std::conditional_t<JOIN, PagedJoinParams, PagedAttnParams> p;
     int32_t n_wg, rows, D, G; // rows of a slot
     int32_t rpb;              // rows of a workgroup
     int32_t weights;          // room for each in LDS
@@ -29,7 +31,7 @@ struct MergeParams {
 // flight each.  A part without a visible key (l = 0) adds nothing.
 // JOIN: the rows come out as paged_row_out says.
 template <class T, bool JOIN>
-__global__ __launch_bounds__(kMergeThreads) void paged_merge_rows(MergeParams p) {
+__global__ __launch_bounds__(kMergeThreads) void paged_merge_rows(MergeParams<JOIN> p) {
     using V4 = typename PagedVec<T>::v4;
     __shared__ PagedRowOut outs[JOIN ? kMergeRows : 1];
     __shared__ __attribute__((aligned(16))) float wgt[kPagedMaxWorkers];
@@ -133,7 +135,7 @@ __global__ __launch_bounds__(kMergeThreads) void paged_merge_rows(MergeParams p)
 // own, joined as above.  Garbage in `parts` (rows that no prefix's sequences have) leads to
 // no access outside the scratch.
 template <class T>
-__global__ __launch_bounds__(kMergeThreads) void paged_merge_parts(MergeParams p) {
+__global__ __launch_bounds__(kMergeThreads) void paged_merge_parts(MergeParams<true> p) {
     using V4 = typename PagedVec<T>::v4;
     __shared__ float wgt[2 * (kPagedMaxWorkers + 1)];
     __shared__ __attribute__((aligned(16))) f4 red[kMergeThreads];
@@ -221,42 +223,35 @@ __global__ __launch_bounds__(kMergeThreads) void paged_merge_parts(MergeParams p
 
 } // namespace
 
-int paged_merge(const PagedAttnArgs& a, const PagedAttnParams& p, hipStream_t stream, std::string& err) {
-    MergeParams m;
-    m.p = p;
-    m.n_wg = p.work.n_wg;
-    m.rows = p.slot_rows;
-    m.D = a.D;
-    m.G = p.work.G;
+int paged_merge(const PagedAttnArgs& a, const PagedJoinParams& p, hipStream_t stream, std::string& err) {
     // few rows with many parts: a row per workgroup
-    m.rpb = p.slot_rows <= 32 ? 1 : std::min({kMergeRows, kMergeThreads / (a.D / 4), kPagedMaxWorkers / m.n_wg});
-    m.weights = kPagedMaxWorkers / m.rpb;
-    if (p.join.parts != nullptr) {
-        auto* const kernel = a.type == PagedType::F16 ? &paged_merge_parts<_Float16> : &paged_merge_parts<__bf16>;
-        hipLaunchKernelGGL(kernel, dim3((uint32_t)p.join.rows), dim3(kMergeThreads), 0, stream, m);
+    const int rpb =
+        p.slot_rows <= 32 ? 1 : std::min({kMergeRows, kMergeThreads / (a.D / 4), kPagedMaxWorkers / p.work.n_wg});
+    auto launch = [&](auto* kernel, auto join, dim3 grid) {
+        const MergeParams<decltype(join)::value> m{p,        p.work.n_wg, p.slot_rows, a.D,
+                                                   p.work.G, rpb,         kPagedMaxWorkers / rpb};
+        hipLaunchKernelGGL(kernel, grid, dim3(kMergeThreads), 0, stream, m);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) {
             err = hipGetErrorString(e);
             return -1;
         }
         return 0;
+    };
+    const bool f16 = a.type == PagedType::F16;
+    if (p.join.parts != nullptr) {
+        return launch(f16 ? &paged_merge_parts<_Float16> : &paged_merge_parts<__bf16>, std::true_type{},
+                      dim3((uint32_t)p.join.rows));
     }
-    const dim3 grid((uint32_t)m.n_wg, (uint32_t)((m.rows + m.rpb - 1) / m.rpb));
-    const bool join = p.join.any();
-    auto* const kernel = a.type == PagedType::F16
-                             ? (join ? &paged_merge_rows<_Float16, true> : &paged_merge_rows<_Float16, false>)
-                             : (join ? &paged_merge_rows<__bf16, true> : &paged_merge_rows<__bf16, false>);
-    hipLaunchKernelGGL(kernel, grid, dim3(kMergeThreads), 0, stream, m);
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) {
-        err = hipGetErrorString(e);
-        return -1;
-    }
-    return 0;
+    const dim3 grid((uint32_t)p.work.n_wg, (uint32_t)((p.slot_rows + rpb - 1) / rpb));
+    return p.join.any() ? launch(f16 ? &paged_merge_rows<_Float16, true> : &paged_merge_rows<__bf16, true>,
+                                 std::true_type{}, grid)
+                        : launch(f16 ? &paged_merge_rows<_Float16, false> : &paged_merge_rows<__bf16, false>,
+                                 std::false_type{}, grid);
 }
 
 int paged_attention(const PagedAttnArgs& a, hipStream_t stream, std::string& err) {
-    PagedAttnParams p{};
+    PagedJoinParams p{};
     p.c = a.c;
     p.work.seqs = a.seqs;
     p.work.mask = a.mask;
@@ -302,7 +297,7 @@ int paged_attention(const PagedAttnArgs& a, hipStream_t stream, std::string& err
     // 66 / 42, 85 / 75; 16 on 8, D 256, 64 74 / 61, 102 / 110.  Over 600 calls of 2 to 300
     // sequences, 1 to 12 prefixes of 100 to 60000 keys, 10 to 3000 own ones, this rule is 1.2 % off
     // the faster form (geometric mean), kItems 512 without kUnits was 3.8 %.
-    PagedAttnParams shared = p;
+    PagedJoinParams shared = p;
     bool together = false;
     if (a.prefix.n > 0) {
         constexpr int64_t kItems = 1024, kUnits = 32768, kSharedRows = 8192;

@@ -71,6 +71,7 @@ template <class T, int D, bool I8, int WV>
 __global__ __launch_bounds__((StreamCfg<D, I8, WV>::THREADS), (StreamCfg<D, I8, WV>::WAVES_PER_SIMD)) void paged_stream(
     PagedAttnParams p) {
     constexpr bool JOIN = false, OUT = false;
+    constexpr PagedJoin join = {};
 #include "paged_stream_body.inl"
 }
 
@@ -78,21 +79,23 @@ __global__ __launch_bounds__((StreamCfg<D, I8, WV>::THREADS), (StreamCfg<D, I8, 
 // calls without a log-sum-exp 1.1 of 9.9 us (1 x 2048 keys, 8 heads of 128).
 template <class T, int D, bool I8, int WV>
 __global__ __launch_bounds__((StreamCfg<D, I8, WV>::THREADS), (StreamCfg<D, I8, WV>::WAVES_PER_SIMD)) void
-paged_out_stream(PagedAttnParams p) {
+paged_out_stream(PagedJoinParams p) {
     constexpr bool JOIN = false, OUT = true;
+    const PagedJoin& join = p.join;
 #include "paged_stream_body.inl"
 }
 
 template <class T, int D, bool I8, int WV>
 __global__ __launch_bounds__((StreamCfg<D, I8, WV>::THREADS), (StreamCfg<D, I8, WV>::WAVES_PER_SIMD)) void
-paged_join_stream(PagedAttnParams p) {
+paged_join_stream(PagedJoinParams p) {
     constexpr bool JOIN = true, OUT = false;
+    const PagedJoin& join = p.join;
 #include "paged_stream_body.inl"
 }
 
 // Workers are workgroups; smallest share: a tile for every wave.
 template <bool OUT>
-int paged_stream_launch(const PagedAttnArgs& a, PagedAttnParams& p, const PagedLaunch& l, hipStream_t stream,
+int paged_stream_launch(const PagedAttnArgs& a, PagedJoinParams& p, const PagedLaunch& l, hipStream_t stream,
                         std::string& err) {
     return paged_for_type(a, [&](auto t, auto d, auto i8) {
         using T = decltype(t);

@@ -1,7 +1,7 @@
 // Body of the paged_stream kernels (paged_stream.hpp), included into each of them.  In
 // scope: T, D, I8, WV, JOIN (prefixes and sequences in one launch, every row's parts
 // left for paged_merge_parts), OUT (rows whose keys are in two parts, or whose log-sum-exp
-// is asked for) and the parameters p.
+// is asked for), join and the parameters p.
     using C = StreamCfg<D, I8, WV>;
     using V8 = typename PagedVec<T>::v8;
     using V4 = typename PagedVec<T>::v4;
@@ -24,7 +24,7 @@
     uint64_t* const rows_at = reinterpret_cast<uint64_t*>(aux + C::TAB_BYTES + C::SCALE_BYTES); // K rows, V rows
 
     if (p.zero_tail != 0) {
-        zero_tail_rows<D>(p);
+        zero_tail_rows<D>(p, join.lse);
     }
     PagedRecord rec = {};
     // Heads of int8 pages next to each other on one XCD: a line of scales holds those
@@ -81,11 +81,11 @@
         auto tile_key = [&](int j) { return (t0 + wave + C::WAVES * j) * kTile; };
         const char* const kbase = p.c.k + h * p.c.k_sh;
         const char* const vbase = p.c.v + h * p.c.v_sh;
-        const int32_t* const table = shared ? p.join.prefix_table + walk.b * p.join.prefix_table_s
+        const int32_t* const table = shared ? join.prefix_table + walk.b * join.prefix_table_s
                                      : JOIN ? p.c.table + (walk.b - p.work.seqs.prefixes) * p.c.table_s
                                             : p.c.table + walk.b * p.c.table_s;
 
-        i32x4_t tab_rsrc = make_rsrc_v(table, (uint32_t)(shared ? p.join.prefix_width : p.c.width) * 4u);
+        i32x4_t tab_rsrc = make_rsrc_v(table, (uint32_t)(shared ? join.prefix_width : p.c.width) * 4u);
 #pragma unroll
         for (int e = 0; e < 4; e++) {
             tab_rsrc[e] = uniform(tab_rsrc[e]);
@@ -364,8 +364,8 @@
             const int64_t slot = (int64_t)walk.slot() * p.slot_rows;
             if (JOIN && walk.begin() == 0 && tid < n_rows) {
                 const int tk = (r0 + tid) / G;
-                const int64_t row = (int64_t)(seq.q0 + tk) * p.join.Hq + h * G + r0 + tid - tk * G;
-                p.join.parts[(shared ? 0 : p.join.rows) + row] =
+                const int64_t row = (int64_t)(seq.q0 + tk) * join.Hq + h * G + r0 + tid - tk * G;
+                join.parts[(shared ? 0 : join.rows) + row] =
                     PagedParts{whole ? -1 : walk.part.wg, whole ? -1 : walk.last_wg(), tid, 0};
             }
             if (!whole && walk.begin() == 0) {
@@ -393,19 +393,19 @@
                 }
                 if (JOIN && whole) {
                     const int tk = (r0 + col) / G;
-                    const int64_t row = (shared ? 0 : p.join.rows) + (int64_t)(seq.q0 + tk) * p.join.Hq + h * G + r0 + col -
+                    const int64_t row = (shared ? 0 : join.rows) + (int64_t)(seq.q0 + tk) * join.Hq + h * G + r0 + col -
                                         tk * G;
-                    *reinterpret_cast<f4*>(&p.join.whole_o[row * D + d]) = acc;
+                    *reinterpret_cast<f4*>(&join.whole_o[row * D + d]) = acc;
                     if (d == 0) {
-                        *reinterpret_cast<float2*>(p.join.whole_ml + row * 2) = float2{mref, lsum};
+                        *reinterpret_cast<float2*>(join.whole_ml + row * 2) = float2{mref, lsum};
                     }
                 } else if (OUT && whole) {
                     const int tk = (r0 + col) / G, hd = h * G + r0 + col - tk * G;
                     const int64_t row = (int64_t)(seq.q0 + tk) * p.Hq + hd;
-                    const PagedRowOut out = paged_row_out(p.join, row, mref, lsum);
-                    paged_store<T>(p.join, out, row, d, acc, p.o + (int64_t)(seq.q0 + tk) * p.o_st + hd * p.o_sh);
+                    const PagedRowOut out = paged_row_out(join, row, mref, lsum);
+                    paged_store<T>(join, out, row, d, acc, p.o + (int64_t)(seq.q0 + tk) * p.o_st + hd * p.o_sh);
                     if (d == 0) {
-                        paged_store_lse(p.join, out, row);
+                        paged_store_lse(join, out, row);
                     }
                 } else if (whole) {
                     const int tk = (r0 + col) / G;

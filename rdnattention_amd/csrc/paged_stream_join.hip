@@ -7,7 +7,7 @@ int64_t paged_join_cost(const PagedWork& w) {
     return paged_max_cost<kRows, kTile, kJoinCost>(w);
 }
 
-int paged_join_stream_attention(const PagedAttnArgs& a, PagedAttnParams& p, hipStream_t stream, std::string& err) {
+int paged_join_stream_attention(const PagedAttnArgs& a, PagedJoinParams& p, hipStream_t stream, std::string& err) {
     return paged_for_type(a, [&](auto t, auto d, auto i8) {
         using T = decltype(t);
         constexpr int D = decltype(d)::value;

@@ -3,7 +3,7 @@
 
 namespace rdna_amd {
 
-int paged_out_stream_attention(const PagedAttnArgs& a, PagedAttnParams& p, const PagedLaunch& l, hipStream_t stream,
+int paged_out_stream_attention(const PagedAttnArgs& a, PagedJoinParams& p, const PagedLaunch& l, hipStream_t stream,
                                std::string& err) {
     return paged_stream_launch<true>(a, p, l, stream, err);
 }

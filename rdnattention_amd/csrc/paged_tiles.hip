@@ -8,7 +8,7 @@ int64_t paged_tile_cost(const PagedAttnArgs& a, const PagedWork& w) {
                       : paged_max_cost<TileCfg<256, false>::ROWS, kBN, kItemCost>(w);
 }
 
-int paged_tile_attention(const PagedAttnArgs& a, PagedAttnParams& p, const PagedLaunch& l, hipStream_t stream,
+int paged_tile_attention(const PagedAttnArgs& a, PagedJoinParams& p, const PagedLaunch& l, hipStream_t stream,
                          std::string& err) {
     return p.join.any() ? paged_join_tile_attention(a, p, l, stream, err)
                         : paged_tile_launch<false>(a, p, l, stream, err);

@@ -75,6 +75,7 @@ template <class T, int D, bool I8>
 __global__ __launch_bounds__((TileCfg<D, I8>::THREADS), (TileCfg<D, I8>::WAVES_PER_SIMD)) void paged_tiles(
     PagedAttnParams p) {
     constexpr bool JOIN = false;
+    constexpr PagedJoin join = {};
 #include "paged_tiles_body.inl"
 }
 
@@ -82,14 +83,15 @@ __global__ __launch_bounds__((TileCfg<D, I8>::THREADS), (TileCfg<D, I8>::WAVES_P
 // addresses too.)
 template <class T, int D, bool I8>
 __global__ __launch_bounds__((TileCfg<D, I8>::THREADS), (D <= 32 ? 2 : TileCfg<D, I8>::WAVES_PER_SIMD)) void
-paged_join_tiles(PagedAttnParams p) {
+paged_join_tiles(PagedJoinParams p) {
     constexpr bool JOIN = true;
+    const PagedJoin& join = p.join;
 #include "paged_tiles_body.inl"
 }
 
 // Workers are workgroups; smallest share: two key tiles.
 template <bool JOIN>
-int paged_tile_launch(const PagedAttnArgs& a, PagedAttnParams& p, const PagedLaunch& l, hipStream_t stream,
+int paged_tile_launch(const PagedAttnArgs& a, PagedJoinParams& p, const PagedLaunch& l, hipStream_t stream,
                       std::string& err) {
     return paged_for_type(a, [&](auto t, auto d, auto i8) {
         using T = decltype(t);

@@ -1,6 +1,6 @@
 // Body of the paged_tiles kernels (paged_tiles.hpp), included into each of them.  In
 // scope: T, D, I8, JOIN (rows whose keys are in two parts, or whose log-sum-exp is
-// asked for) and the parameters p.
+// asked for), join and the parameters p.
     using C = TileCfg<D, I8>;
     using V8 = typename PagedVec<T>::v8;
     using V4 = typename PagedVec<T>::v4;
@@ -43,7 +43,7 @@
     }
 
     if (p.zero_tail != 0) {
-        zero_tail_rows<D>(p);
+        zero_tail_rows<D>(p, join.lse);
     }
     PagedRecord rec = {};
     // row tiles of one head, which read the same keys, through one L2
@@ -531,7 +531,6 @@
             unit = p_tot > 0.0f ? l_tot / p_tot : 1.0f;
         }
         if (JOIN && whole) {
-            const PagedJoin& join = p.join;
             const int64_t row = (int64_t)(seq.q0 + tok) * join.Hq + head;
             if (l_tot == 0.0f) { // as below
 #pragma unroll

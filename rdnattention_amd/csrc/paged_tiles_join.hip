@@ -3,7 +3,7 @@
 
 namespace rdna_amd {
 
-int paged_join_tile_attention(const PagedAttnArgs& a, PagedAttnParams& p, const PagedLaunch& l, hipStream_t stream,
+int paged_join_tile_attention(const PagedAttnArgs& a, PagedJoinParams& p, const PagedLaunch& l, hipStream_t stream,
                               std::string& err) {
     return paged_tile_launch<true>(a, p, l, stream, err);
 }
